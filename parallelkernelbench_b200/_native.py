@@ -120,6 +120,37 @@ def raw_stream(t) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
+_bound: dict = {}
+
+
+def bound(name: str, argtypes: list):
+    """The entry point ``name`` with its argument types declared (plain integers and floats are passed then), looked up once."""
+    f = _bound.get(name)
+    if f is None:
+        f = getattr(cuda_lib(), name)
+        f.argtypes = argtypes
+        _bound[name] = f
+    return f
+
+
+def on_device(t):
+    """Context in which the device of ``t`` is the current one: launches go to the device of their tensors."""
+    import contextlib
+
+    import torch
+
+    return contextlib.nullcontext() if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+
+
+def same_cuda_device(first, **tensors) -> None:
+    """Every tensor (``None`` is passed over) lives on the CUDA device of ``first``."""
+    if not first.is_cuda:
+        raise ValueError("expected CUDA tensors")
+    for name, t in tensors.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
+
+
 def read_status() -> list[int]:
     buf = (ctypes.c_uint32 * 16)()
     check(cuda_lib().pkb_status_read(buf), "pkb_status_read")

@@ -1,4 +1,4 @@
-"""RMSNorm kernels (csrc/kernels/norm.cu).
+"""RMSNorm (csrc/kernels/norm.cu) and layer norm (csrc/kernels/layernorm.cu) kernels.
 
 ``sum_rmsnorm`` is the consumer end of a reduce-scatter: it adds the per-source partial buffers in
 a fixed order, scales, and normalises, so the reduced tensor is never stored un-normalised
@@ -39,3 +39,88 @@ def sum_rmsnorm(parts: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, sca
              "pkb_sum_rmsnorm")
     nv.count_launch()
     return out
+
+
+# ------------------------------------------------------------------------------------------------ layer norm
+_P, _I, _LL, _F = nv.c_void_p, nv.c_int, nv.c_ll, nv.c_float
+_LN_FWD = [_P, _LL, _P, _P, _I, _P, _P, _P, _LL, _I, _F, _I, _P]
+_LN_BWD = [_P, _LL, _P, _LL, _P, _I, _P, _P, _P, _P, _P, _P, _LL, _I, _I, _P]
+_DT = {torch.bfloat16: 0, torch.float32: 1}
+
+
+def _rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """``[rows, cols]`` with unit inner stride; a view wherever the strides allow one (rows may lie apart, repeat or overlap)."""
+    t = t.reshape(-1, cols) if t.dim() != 2 else t
+    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
+
+
+def _ln_check(x: torch.Tensor, gamma, beta=None) -> int:
+    if x.dtype not in _DT:
+        raise TypeError(f"layer norm takes bf16 or fp32 rows, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("layer norm needs at least one column")
+    cols = x.shape[-1]
+    for name, p in (("gamma", gamma), ("beta", beta)):
+        if p is not None and (p.dtype not in _DT or p.numel() != cols or not p.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous bf16 or fp32 with {cols} values")
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        raise TypeError("gamma and beta must have the same dtype")
+    nv.same_cuda_device(x, gamma=gamma, beta=beta)
+    return cols
+
+
+def _ln_forward(x, gamma, beta, eps, stats: bool):
+    cols = _ln_check(x, gamma, beta)
+    x2 = _rows_of(x, cols)
+    rows = x2.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if stats else None
+    rstd = torch.empty_like(mean) if stats else None
+    if rows:
+        param = gamma if gamma is not None else beta
+        with nv.on_device(x):
+            nv.check(nv.bound("pkb_layer_norm_fwd", _LN_FWD)(
+                x2.data_ptr(), x2.stride(0), 0 if gamma is None else gamma.data_ptr(), 0 if beta is None else beta.data_ptr(),
+                0 if param is None else _DT[param.dtype], y.data_ptr(), mean.data_ptr() if stats else 0, rstd.data_ptr() if stats else 0,
+                rows, cols, eps, _DT[x.dtype], nv.raw_stream(x)), "pkb_layer_norm_fwd")
+        nv.count_launch()
+    return y, mean, rstd
+
+
+def layer_norm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) * rsqrt(var + eps) * gamma + beta`` over the last dimension. ``x`` is bf16 or fp32 ``[..., cols]`` (any row pitch,
+    any width), ``gamma`` and ``beta`` bf16 or fp32 ``[cols]`` or None (1 and 0); fp32 inside, one rounding to the type of ``x``."""
+    return _ln_forward(x, gamma, beta, eps, False)[0]
+
+
+def layer_norm_fwd(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Tensor | None = None, eps: float = 1e-5):
+    """:func:`layer_norm` with what its backward needs: ``(y, mean, rstd)``, the statistics fp32 of shape ``x.shape[:-1]``."""
+    return _ln_forward(x, gamma, beta, eps, True)
+
+
+def layer_norm_bwd(x: torch.Tensor, gamma: torch.Tensor | None, dy: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor):
+    """Backward of :func:`layer_norm_fwd`: ``(dx, dgamma, dbeta)``, ``dx`` in the type of ``x``, the weight gradients fp32 ``[cols]``
+    (what a gain of 1 or a bias of 0 would get where there is none). Sums run in a fixed order: the same inputs give the same bits."""
+    cols = _ln_check(x, gamma)
+    if dy.dtype != x.dtype or dy.shape != x.shape:
+        raise ValueError("dy must have the shape and dtype of x")
+    for name, s in (("mean", mean), ("rstd", rstd)):
+        if s.dtype != torch.float32 or s.numel() * cols != x.numel() or not s.is_contiguous():
+            raise ValueError(f"{name} must be contiguous fp32 with one value per row")
+    nv.same_cuda_device(x, dy=dy, mean=mean, rstd=rstd)
+    x2, dy2 = _rows_of(x, cols), _rows_of(dy, cols)
+    rows = x2.shape[0]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if not rows:
+        zero = torch.zeros((2, cols), dtype=torch.float32, device=x.device)
+        return dx, zero[0], zero[1]
+    dgamma, dbeta = (torch.empty(cols, dtype=torch.float32, device=x.device) for _ in range(2))
+    with nv.on_device(x):
+        blocks = nv.bound("pkb_layer_norm_bwd_partials", [_LL, _I])(rows, cols)
+        part = torch.empty((blocks, 2, cols), dtype=torch.float32, device=x.device)
+        nv.check(nv.bound("pkb_layer_norm_bwd", _LN_BWD)(
+            x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), 0 if gamma is None else gamma.data_ptr(),
+            0 if gamma is None else _DT[gamma.dtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(),
+            part.data_ptr(), rows, cols, _DT[x.dtype], nv.raw_stream(x)), "pkb_layer_norm_bwd")
+    nv.count_launch(2)
+    return dx, dgamma, dbeta
