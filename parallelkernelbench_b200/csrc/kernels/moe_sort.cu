@@ -1,0 +1,436 @@
+// Tokens sorted by expert and back on one GPU: the way of a MoE layer's rows to the grouped GEMM and home, with its gradients.
+//   slots[t, j] = rank of assignment (t, j) among all assignments ordered by expert, then by position (a stable counting sort);
+//                 -1 for an assignment that names no expert (a dropped one)
+//   permute     xp[slots[t, j]] = x[t]                      gradient: dx[t] = sum_j dxp[slots[t, j]]
+//   unpermute   out[t] = sum_j gate[t, j] y[slots[t, j]]    gradient: dy[slots[t, j]] = gate[t, j] dout[t], dgate[t, j] = <dout[t], y[slots[t, j]]>
+// The row kernels are memory bound. All of them walk the tokens, not the sorted rows: a token's row is read (or written) once for its
+// top_k copies, which are scattered (or gathered) as whole rows; sums over a token's experts run in the order of j in fp32, so nothing
+// depends on timing. Rows behind the last expert's (as many as there are dropped assignments) are written as zeros.
+#include <cooperative_groups.h>
+
+#include "pkb/api.h"
+#include "pkb/host.h"
+#include "pkb/ptx.cuh"
+
+namespace pkb {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+// ------------------------------------------------------------------------------------------------ sort
+// One cluster of CTAs, one launch. A warp owns a contiguous run of assignments, 32 at a time. Pass 1 counts its experts in its own row of
+// the CTA's table (lanes with the same expert find one another by match.any; one of them adds for all, so the table needs no atomics);
+// the table is then summed over warps, over CTAs (distributed shared memory) and over experts; pass 2 walks the assignments again and
+// hands out the slots in order.
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortMaxExperts = 1024;
+constexpr int kSortCluster = 8;
+
+__global__ void __launch_bounds__(kSortThreads)
+moe_sort_kernel(const int* __restrict__ idx, int n, int experts, int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ slots) {
+  extern __shared__ int table[];                        // [kSortWarps][experts]
+  __shared__ int total[kSortMaxExperts], base[kSortMaxExperts], warp_sums[kSortWarps + 1];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long rounds = ((long long)n + 32 * kSortWarps * ctas - 1) / (32 * kSortWarps * ctas);
+  const long long first = ((long long)rank * kSortWarps + warp) * rounds * 32;
+  int* mine = table + warp * experts;
+  for (int e = threadIdx.x; e < kSortWarps * experts; e += kSortThreads) table[e] = 0;
+  __syncthreads();
+  for (long long r = 0; r < rounds && first + r * 32 < n; ++r) {
+    const long long i = first + r * 32 + lane;
+    const int e = i < n ? idx[i] : -1;
+    const bool ok = (unsigned)e < (unsigned)experts;
+    const unsigned peers = __match_any_sync(0xffffffffu, ok ? e : -1);
+    if (ok && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
+    __syncwarp();
+  }
+  __syncthreads();
+  const int e = threadIdx.x;
+  if (e < experts) {
+    int run = 0;
+    for (int w = 0; w < kSortWarps; ++w) {
+      const int c = table[w * experts + e];
+      table[w * experts + e] = run;
+      run += c;
+    }
+    total[e] = run;
+  }
+  cluster.sync();
+  int before = 0, all = 0;
+  if (e < experts) {
+    for (int c = 0; c < ctas; ++c) {
+      const int v = cluster.map_shared_rank(total, c)[e];
+      if (c < rank) before += v;
+      all += v;
+    }
+  }
+  // exclusive sum over the experts, one per thread
+  int incl = all;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += v;
+  }
+  if (lane == 31) warp_sums[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int s = warp_sums[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += v;
+    }
+    warp_sums[lane] = s;
+  }
+  __syncthreads();
+  const int start = incl - all + (warp > 0 ? warp_sums[warp - 1] : 0);
+  const int kept = warp_sums[kSortWarps - 1];
+  if (e < experts) {
+    base[e] = start + before;
+    if (rank == 0) {
+      offsets[e] = start;
+      if (e == experts - 1) offsets[experts] = kept;
+    }
+  }
+  __syncthreads();
+  for (long long r = 0; r < rounds && first + r * 32 < n; ++r) {
+    const long long i = first + r * 32 + lane;
+    const int x = i < n ? idx[i] : -1;
+    const bool ok = (unsigned)x < (unsigned)experts;
+    const unsigned peers = __match_any_sync(0xffffffffu, ok ? x : -1);
+    const int slot = ok ? base[x] + mine[x] + __popc(peers & ((1u << lane) - 1u)) : -1;
+    __syncwarp();
+    if (ok && lane == __ffs(peers) - 1) mine[x] += __popc(peers);
+    __syncwarp();
+    if (i < n) slots[i] = slot;
+    if (ok) order[slot] = (int)i;
+  }
+  for (long long i = kept + (long long)rank * kSortThreads + threadIdx.x; i < n; i += (long long)ctas * kSortThreads) order[i] = -1;
+  cluster.sync();      // nobody leaves while its totals may still be read
+}
+
+// ------------------------------------------------------------------------------------------------ rows
+// 16 bytes (VEC = 8 bf16 or 4 fp32 values) or one value of a row, as it is or as fp32
+template <typename T, int VEC>
+struct RowVec {
+  using Raw = typename std::conditional<VEC == 1, T, U4>::type;
+  static __device__ __forceinline__ Raw load(const T* p) {
+    if constexpr (VEC == 1) return *p;
+    else return ld_global_nc_v4(p);
+  }
+  static __device__ __forceinline__ void store(T* p, const Raw& v) {
+    if constexpr (VEC == 1) *p = v;
+    else st_global_v4(p, v);
+  }
+  static __device__ __forceinline__ Raw zero() {
+    if constexpr (VEC == 1) return T(0.f);
+    else return U4{0u, 0u, 0u, 0u};
+  }
+  static __device__ __forceinline__ void unpack(const Raw& v, float (&f)[VEC]) {
+    if constexpr (VEC == 1) {
+      f[0] = static_cast<float>(v);
+    } else if constexpr (VEC == 4) {
+      f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+    } else {
+      const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
+      f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+    }
+  }
+  static __device__ __forceinline__ Raw pack(const float (&f)[VEC]) {
+    if constexpr (VEC == 1) {
+      if constexpr (sizeof(T) == 2) return __float2bfloat16_rn(f[0]);
+      else return f[0];
+    } else if constexpr (VEC == 4) {
+      return U4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+    } else {
+      return U4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+    }
+  }
+};
+
+constexpr int kRowThreads = 256;
+
+// Where a thread works: blocks are split into teams of `team` threads (a power of two); a team takes one token and one piece of
+// team * unroll accesses of its row.
+struct RowGrid {
+  int team_log2, pieces;
+  __device__ __forceinline__ bool place(long long tokens, long long& token, int& first, int unroll) const {
+    const int team = 1 << team_log2;
+    const long long unit = (long long)blockIdx.x * (kRowThreads >> team_log2) + (threadIdx.x >> team_log2);
+    token = unit / pieces;
+    first = (int)(unit - token * pieces) * team * unroll + (threadIdx.x & (team - 1));
+    return token < tokens;
+  }
+};
+
+// zeros into the rows from `kept` on, by all blocks
+template <typename T, int VEC>
+__device__ __forceinline__ void zero_rows(T* rows, long long n, int nvec, const int* kept) {
+  const long long from = max(*kept, 0), count = (n - from) * nvec;
+  for (long long i = (long long)blockIdx.x * kRowThreads + threadIdx.x; i < count; i += (long long)gridDim.x * kRowThreads) {
+    const long long r = i / nvec;
+    RowVec<T, VEC>::store(rows + ((from + r) * nvec + (i - r * nvec)) * VEC, RowVec<T, VEC>::zero());
+  }
+}
+
+constexpr int kRowUnroll = 2;
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kRowThreads)
+moe_permute_kernel(const T* __restrict__ x, long long ldx, const int* __restrict__ slots, const int* __restrict__ kept, T* __restrict__ xp,
+                   long long tokens, int top_k, int nvec, const RowGrid grid) {
+  using V = RowVec<T, VEC>;
+  long long t;
+  int first;
+  if (grid.place(tokens, t, first, kRowUnroll)) {
+    const int team = 1 << grid.team_log2;
+    const unsigned n = (unsigned)(tokens * top_k);
+    typename V::Raw v[kRowUnroll];
+#pragma unroll
+    for (int u = 0; u < kRowUnroll; ++u)
+      if (first + u * team < nvec) v[u] = V::load(x + t * ldx + (long long)(first + u * team) * VEC);
+    for (int j = 0; j < top_k; ++j) {
+      const unsigned s = (unsigned)slots[t * top_k + j];
+      if (s < n) {
+#pragma unroll
+        for (int u = 0; u < kRowUnroll; ++u)
+          if (first + u * team < nvec) V::store(xp + ((long long)s * nvec + first + u * team) * VEC, v[u]);
+      }
+    }
+  }
+  zero_rows<T, VEC>(xp, tokens * top_k, nvec, kept);
+}
+
+// out[t] = sum_j gate[t, j] y[slots[t, j]]; GATED = false: weights of one
+constexpr int kGatherAhead = 4;   // rows whose loads are issued before the first of them is added
+
+template <typename T, int VEC, bool GATED>
+__global__ void __launch_bounds__(kRowThreads)
+moe_unpermute_kernel(const T* __restrict__ y, long long ldy, const int* __restrict__ slots, const float* __restrict__ gates, T* __restrict__ out,
+                     long long tokens, int top_k, int nvec, const RowGrid grid) {
+  using V = RowVec<T, VEC>;
+  long long t;
+  int first;
+  if (!grid.place(tokens, t, first, kRowUnroll)) return;
+  const int team = 1 << grid.team_log2;
+  const unsigned n = (unsigned)(tokens * top_k);
+  float acc[kRowUnroll][VEC] = {};
+  for (int j0 = 0; j0 < top_k; j0 += kGatherAhead) {
+    typename V::Raw v[kGatherAhead][kRowUnroll];
+    float g[kGatherAhead];
+    bool there[kGatherAhead];
+#pragma unroll
+    for (int a = 0; a < kGatherAhead; ++a) {
+      const int j = j0 + a;
+      const unsigned s = j < top_k ? (unsigned)slots[t * top_k + j] : n;
+      there[a] = s < n;
+      g[a] = 1.f;
+      if (there[a]) {
+        if constexpr (GATED) g[a] = gates[t * top_k + j];
+#pragma unroll
+        for (int u = 0; u < kRowUnroll; ++u)
+          if (first + u * team < nvec) v[a][u] = V::load(y + (long long)s * ldy + (long long)(first + u * team) * VEC);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < kGatherAhead; ++a) {
+      if (there[a]) {
+#pragma unroll
+        for (int u = 0; u < kRowUnroll; ++u) {
+          if (first + u * team < nvec) {
+            float f[VEC];
+            V::unpack(v[a][u], f);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[u][i] += GATED ? g[a] * f[i] : f[i];
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kRowUnroll; ++u)
+    if (first + u * team < nvec) V::store(out + (t * nvec + first + u * team) * VEC, V::pack(acc[u]));
+}
+
+// One block per token: dy rows and the dot products in one pass over dout and y.
+constexpr int kBwdExperts = 8;    // experts of a token that a pass over its row handles at once
+
+template <typename T, int VEC, int NT>
+__global__ void __launch_bounds__(NT)
+moe_unpermute_bwd_kernel(const T* __restrict__ dout, long long lddo, const T* __restrict__ y, long long ldy, const int* __restrict__ slots,
+                         const float* __restrict__ gates, const int* __restrict__ kept, T* __restrict__ dy, float* __restrict__ dgates,
+                         long long tokens, int top_k, int nvec) {
+  using V = RowVec<T, VEC>;
+  __shared__ float red[NT / 32][kBwdExperts];
+  const unsigned n = (unsigned)(tokens * top_k);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long t = blockIdx.x;
+  for (int j0 = 0; j0 < top_k; j0 += kBwdExperts) {
+    unsigned s[kBwdExperts];
+    float g[kBwdExperts], dot[kBwdExperts] = {};
+#pragma unroll
+    for (int a = 0; a < kBwdExperts; ++a) {
+      const int j = j0 + a;
+      s[a] = j < top_k ? (unsigned)slots[t * top_k + j] : n;
+      g[a] = s[a] < n ? gates[t * top_k + j] : 0.f;
+    }
+    for (int i = threadIdx.x; i < nvec; i += NT) {
+      float d[VEC];
+      V::unpack(V::load(dout + t * lddo + (long long)i * VEC), d);
+      typename V::Raw v[kBwdExperts];
+#pragma unroll
+      for (int a = 0; a < kBwdExperts; ++a)
+        if (s[a] < n) v[a] = V::load(y + (long long)s[a] * ldy + (long long)i * VEC);
+#pragma unroll
+      for (int a = 0; a < kBwdExperts; ++a) {
+        if (s[a] < n) {
+          float f[VEC], o[VEC];
+          V::unpack(v[a], f);
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) {
+            dot[a] += d[c] * f[c];
+            o[c] = g[a] * d[c];
+          }
+          V::store(dy + ((long long)s[a] * nvec + i) * VEC, V::pack(o));
+        }
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < kBwdExperts; ++a) {
+      const float w = warp_sum(dot[a]);
+      if (lane == 0) red[warp][a] = w;
+    }
+    __syncthreads();
+    if (threadIdx.x < kBwdExperts && j0 + (int)threadIdx.x < top_k) {
+      float w = 0.f;
+#pragma unroll
+      for (int k = 0; k < NT / 32; ++k) w += red[k][threadIdx.x];
+      dgates[t * top_k + j0 + threadIdx.x] = w;
+    }
+    __syncthreads();
+  }
+  const long long from = max(*kept, 0), count = ((long long)n - from) * nvec;
+  for (long long i = t * NT + threadIdx.x; i < count; i += tokens * NT) V::store(dy + (from * nvec + i) * VEC, V::zero());
+}
+
+bool rows_aligned(const void* p, long long pitch_bytes) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)pitch_bytes) & 15) == 0; }
+
+// teams of the smallest power of two that covers a row with kRowUnroll accesses per thread, up to the whole block
+RowGrid row_grid(long long tokens, int nvec, unsigned* blocks) {
+  RowGrid g{0, 1};
+  while (g.team_log2 < 8 && (kRowUnroll << g.team_log2) < nvec) ++g.team_log2;
+  const int per = kRowUnroll << g.team_log2;
+  g.pieces = (nvec + per - 1) / per;
+  const long long teams = kRowThreads >> g.team_log2;
+  *blocks = (unsigned)((tokens * g.pieces + teams - 1) / teams);
+  return g;
+}
+
+template <typename T, int VEC>
+int permute_rows(const void* x, long long ldx, const int* slots, const int* kept, void* xp, long long tokens, int top_k, int hidden, cudaStream_t s) {
+  unsigned blocks;
+  const RowGrid g = row_grid(tokens, hidden / VEC, &blocks);
+  moe_permute_kernel<T, VEC><<<blocks, kRowThreads, 0, s>>>(static_cast<const T*>(x), ldx, slots, kept, static_cast<T*>(xp), tokens, top_k, hidden / VEC, g);
+  PKB_CHECK_CUDA(cudaGetLastError());
+  return kApiOk;
+}
+
+template <typename T, int VEC>
+int unpermute_rows(const void* y, long long ldy, const int* slots, const float* gates, void* out, long long tokens, int top_k, int hidden,
+                   cudaStream_t s) {
+  unsigned blocks;
+  const RowGrid g = row_grid(tokens, hidden / VEC, &blocks);
+  const T* yp = static_cast<const T*>(y);
+  T* op = static_cast<T*>(out);
+  if (gates != nullptr) moe_unpermute_kernel<T, VEC, true><<<blocks, kRowThreads, 0, s>>>(yp, ldy, slots, gates, op, tokens, top_k, hidden / VEC, g);
+  else moe_unpermute_kernel<T, VEC, false><<<blocks, kRowThreads, 0, s>>>(yp, ldy, slots, gates, op, tokens, top_k, hidden / VEC, g);
+  PKB_CHECK_CUDA(cudaGetLastError());
+  return kApiOk;
+}
+
+template <typename T, int VEC>
+int unpermute_bwd_rows(const void* dout, long long lddo, const void* y, long long ldy, const int* slots, const float* gates, const int* kept,
+                       void* dy, float* dgates, long long tokens, int top_k, int hidden, cudaStream_t s) {
+  moe_unpermute_bwd_kernel<T, VEC, 256><<<(unsigned)tokens, 256, 0, s>>>(static_cast<const T*>(dout), lddo, static_cast<const T*>(y), ldy, slots, gates,
+                                                                         kept, static_cast<T*>(dy), dgates, tokens, top_k, hidden / VEC);
+  PKB_CHECK_CUDA(cudaGetLastError());
+  return kApiOk;
+}
+
+}  // namespace
+
+}  // namespace pkb
+
+using namespace pkb;
+
+#define PKB_ROWS_ARGS()                                                                                                          \
+  PKB_CHECK_ARG(tokens > 0 && top_k > 0 && hidden > 0 && tokens <= 0x7fffffffll / top_k, "1 .. 2^31 - 1 assignments of at least one column"); \
+  PKB_CHECK_ARG(dtype == 0 || dtype == 1, "dtype must be 0 (bf16) or 1 (fp32)");                                                   \
+  const int vec = dtype ? 4 : 8, esize = dtype ? 4 : 2;                                                                            \
+  cudaStream_t s = static_cast<cudaStream_t>(stream)
+
+// offsets [experts + 1], order [n], slots [n] (int32) of the n assignments idx (int32; values outside [0, experts) are dropped).
+extern "C" int pkb_moe_sort(const void* idx, long long n, int experts, void* offsets, void* order, void* slots, void* stream) {
+  PKB_CHECK_ARG(n > 0 && n <= 0x7fffffffll, "1 .. 2^31 - 1 assignments");
+  PKB_CHECK_ARG(experts >= 1 && experts <= kSortMaxExperts, "1 .. 1024 experts");
+  const int smem = kSortWarps * experts * (int)sizeof(int);
+  PKB_CHECK_CUDA(cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int ctas = n > 8192 ? kSortCluster : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, moe_sort_kernel, static_cast<const int*>(idx), (int)n, experts, static_cast<int*>(offsets),
+                                    static_cast<int*>(order), static_cast<int*>(slots)));
+  return kApiOk;
+}
+
+// xp [tokens * top_k, hidden] (contiguous) from x [tokens, hidden] (ldx elements between rows); kept: offsets[experts] on the device.
+extern "C" int pkb_moe_permute(const void* x, long long ldx, const void* slots, const void* kept, void* xp, long long tokens, int top_k, int hidden,
+                               int dtype, void* stream) {
+  PKB_ROWS_ARGS();
+  const bool v = hidden % vec == 0 && rows_aligned(x, ldx * esize) && rows_aligned(xp, 0);
+  const int *sp = static_cast<const int*>(slots), *kp = static_cast<const int*>(kept);
+  if (dtype) return v ? permute_rows<float, 4>(x, ldx, sp, kp, xp, tokens, top_k, hidden, s) : permute_rows<float, 1>(x, ldx, sp, kp, xp, tokens, top_k, hidden, s);
+  return v ? permute_rows<__nv_bfloat16, 8>(x, ldx, sp, kp, xp, tokens, top_k, hidden, s)
+           : permute_rows<__nv_bfloat16, 1>(x, ldx, sp, kp, xp, tokens, top_k, hidden, s);
+}
+
+// out [tokens, hidden] (contiguous) from y [tokens * top_k, hidden] (ldy elements between rows); gates fp32 [tokens, top_k] or null (ones).
+extern "C" int pkb_moe_unpermute(const void* y, long long ldy, const void* slots, const void* gates, void* out, long long tokens, int top_k,
+                                 int hidden, int dtype, void* stream) {
+  PKB_ROWS_ARGS();
+  const bool v = hidden % vec == 0 && rows_aligned(y, ldy * esize) && rows_aligned(out, 0);
+  const int* sp = static_cast<const int*>(slots);
+  const float* gp = static_cast<const float*>(gates);
+  if (dtype) return v ? unpermute_rows<float, 4>(y, ldy, sp, gp, out, tokens, top_k, hidden, s) : unpermute_rows<float, 1>(y, ldy, sp, gp, out, tokens, top_k, hidden, s);
+  return v ? unpermute_rows<__nv_bfloat16, 8>(y, ldy, sp, gp, out, tokens, top_k, hidden, s)
+           : unpermute_rows<__nv_bfloat16, 1>(y, ldy, sp, gp, out, tokens, top_k, hidden, s);
+}
+
+// dy [tokens * top_k, hidden] (contiguous) and dgates fp32 [tokens, top_k] of pkb_moe_unpermute.
+extern "C" int pkb_moe_unpermute_bwd(const void* dout, long long lddo, const void* y, long long ldy, const void* slots, const void* gates,
+                                     const void* kept, void* dy, void* dgates, long long tokens, int top_k, int hidden, int dtype, void* stream) {
+  PKB_ROWS_ARGS();
+  PKB_CHECK_ARG(gates != nullptr, "the gradient of the weights needs the weights");
+  const bool v = hidden % vec == 0 && rows_aligned(dout, lddo * esize) && rows_aligned(y, ldy * esize) && rows_aligned(dy, 0);
+  const int *sp = static_cast<const int*>(slots), *kp = static_cast<const int*>(kept);
+  const float* gp = static_cast<const float*>(gates);
+  float* dg = static_cast<float*>(dgates);
+  if (dtype)
+    return v ? unpermute_bwd_rows<float, 4>(dout, lddo, y, ldy, sp, gp, kp, dy, dg, tokens, top_k, hidden, s)
+             : unpermute_bwd_rows<float, 1>(dout, lddo, y, ldy, sp, gp, kp, dy, dg, tokens, top_k, hidden, s);
+  return v ? unpermute_bwd_rows<__nv_bfloat16, 8>(dout, lddo, y, ldy, sp, gp, kp, dy, dg, tokens, top_k, hidden, s)
+           : unpermute_bwd_rows<__nv_bfloat16, 1>(dout, lddo, y, ldy, sp, gp, kp, dy, dg, tokens, top_k, hidden, s);
+}

@@ -9,6 +9,7 @@ NVLink. The reference synchronises with the host three times per layer call
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -248,3 +249,133 @@ class MoEExchange:
                  "pkb_moe_combine_from")
         nv.count_launch()
         return out
+
+
+# ------------------------------------------------------------------------------------------------ tokens sorted by expert, one GPU
+_P, _I, _LL = nv.c_void_p, nv.c_int, nv.c_ll
+_SORT = [_P, _LL, _I, _P, _P, _P, _P]
+_PERMUTE = [_P, _LL, _P, _P, _P, _LL, _I, _I, _I, _P]
+_UNPERMUTE = [_P, _LL, _P, _P, _P, _LL, _I, _I, _I, _P]
+_UNPERMUTE_BWD = [_P, _LL, _P, _LL, _P, _P, _P, _P, _P, _LL, _I, _I, _I, _P]
+_DT = {torch.bfloat16: 0, torch.float32: 1}
+MAX_SORTED_EXPERTS = 1024
+
+
+class ExpertSort(NamedTuple):
+    """Order of ``tokens * top_k`` assignments by expert (:func:`sort_by_expert`). All tensors int32 on the device.
+
+    ``offsets [E + 1]``: expert ``e`` owns the sorted rows ``[offsets[e], offsets[e + 1])`` (what :func:`grouped_gemm` takes);
+    ``order [n]``: the assignment (``token * top_k + j``) behind every sorted row, -1 from ``offsets[E]`` on;
+    ``slots [n]``: the sorted row of every assignment, -1 where it was dropped."""
+    offsets: torch.Tensor
+    order: torch.Tensor
+    slots: torch.Tensor
+    tokens: int
+    top_k: int
+
+
+def sort_by_expert(expert_idx: torch.Tensor, num_experts: int) -> ExpertSort:
+    """Stable sort of the assignments ``expert_idx`` (int32 ``[T, k]``) by expert, one launch, without the host. A value outside
+    ``[0, num_experts)`` (say -1) is a dropped assignment: it gets no row. At most 1024 experts."""
+    if expert_idx.dtype != torch.int32 or expert_idx.dim() != 2:
+        raise TypeError("expert_idx must be int32 [T, k]")
+    if not 1 <= num_experts <= MAX_SORTED_EXPERTS:
+        raise ValueError(f"1 .. {MAX_SORTED_EXPERTS} experts")
+    T, k = expert_idx.shape
+    n = T * k
+    if n >= 1 << 31:
+        raise ValueError("at most 2^31 - 1 assignments")
+    nv.same_cuda_device(expert_idx)
+    idx = expert_idx.contiguous()
+    offsets = (torch.empty if n else torch.zeros)(num_experts + 1, dtype=torch.int32, device=idx.device)
+    order, slots = (torch.empty(n, dtype=torch.int32, device=idx.device) for _ in range(2))
+    if n:
+        with nv.on_device(idx):
+            nv.check(nv.bound("pkb_moe_sort", _SORT)(idx.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(), slots.data_ptr(),
+                                                     nv.raw_stream(idx)), "pkb_moe_sort")
+        nv.count_launch()
+    return ExpertSort(offsets, order, slots, T, k)
+
+
+def _rows_arg(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
+    if t.dtype not in _DT:
+        raise TypeError(f"{name} must be bf16 or fp32, got {t.dtype}")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
+        raise ValueError(f"{name} must have {rows} rows of at least one column, got {tuple(t.shape)}")
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _sort_arg(srt: ExpertSort, like: torch.Tensor) -> int:
+    n = srt.tokens * srt.top_k
+    for name, t, numel in (("offsets", srt.offsets, None), ("slots", srt.slots, n)):
+        if t.dtype != torch.int32 or not t.is_contiguous() or (numel is not None and t.numel() != numel):
+            raise ValueError(f"{name} of the sort must be contiguous int32 as sort_by_expert makes it")
+    nv.same_cuda_device(like, offsets=srt.offsets, slots=srt.slots)
+    return n
+
+
+def _kept_ptr(srt: ExpertSort) -> int:
+    return srt.offsets.data_ptr() + 4 * (srt.offsets.numel() - 1)
+
+
+def _gates_arg(gates: torch.Tensor, srt: ExpertSort, like: torch.Tensor) -> torch.Tensor:
+    if gates.dtype != torch.float32 or gates.shape != (srt.tokens, srt.top_k):
+        raise ValueError(f"gates must be fp32 [{srt.tokens}, {srt.top_k}]")
+    nv.same_cuda_device(like, gates=gates)
+    return gates.contiguous()
+
+
+def permute_tokens(x: torch.Tensor, srt: ExpertSort) -> torch.Tensor:
+    """Rows of ``x`` (bf16 or fp32 ``[T, H]``, any row pitch) in the order of the experts: ``[T * k, H]`` with
+    ``out[slots[t, j]] = x[t]``. Rows from ``offsets[E]`` on are zero."""
+    x = _rows_arg(x, srt.tokens, "x")
+    n = _sort_arg(srt, x)
+    out = torch.empty((n, x.shape[1]), dtype=x.dtype, device=x.device)
+    if n:
+        with nv.on_device(x):
+            nv.check(nv.bound("pkb_moe_permute", _PERMUTE)(x.data_ptr(), x.stride(0), srt.slots.data_ptr(), _kept_ptr(srt), out.data_ptr(),
+                                                           srt.tokens, srt.top_k, x.shape[1], _DT[x.dtype], nv.raw_stream(x)), "pkb_moe_permute")
+        nv.count_launch()
+    return out
+
+
+def unpermute_tokens(y: torch.Tensor, srt: ExpertSort, gates: torch.Tensor | None = None) -> torch.Tensor:
+    """The way back: ``out[t] = sum_j gates[t, j] * y[slots[t, j]]`` for ``y`` bf16 or fp32 ``[T * k, H]`` and ``gates`` fp32
+    ``[T, k]`` (None: ones). fp32 sums in the order of ``j``; dropped assignments add nothing, a token without any is zero."""
+    y = _rows_arg(y, srt.tokens * srt.top_k, "y")
+    n = _sort_arg(srt, y)
+    g = None if gates is None else _gates_arg(gates, srt, y)
+    out = (torch.empty if n else torch.zeros)((srt.tokens, y.shape[1]), dtype=y.dtype, device=y.device)
+    if n:
+        with nv.on_device(y):
+            nv.check(nv.bound("pkb_moe_unpermute", _UNPERMUTE)(y.data_ptr(), y.stride(0), srt.slots.data_ptr(), 0 if g is None else g.data_ptr(),
+                                                               out.data_ptr(), srt.tokens, srt.top_k, y.shape[1], _DT[y.dtype], nv.raw_stream(y)),
+                     "pkb_moe_unpermute")
+        nv.count_launch()
+    return out
+
+
+def permute_tokens_bwd(dxp: torch.Tensor, srt: ExpertSort) -> torch.Tensor:
+    """Gradient of :func:`permute_tokens`: ``dx[t] = sum_j dxp[slots[t, j]]``."""
+    return unpermute_tokens(dxp, srt)
+
+
+def unpermute_tokens_bwd(dout: torch.Tensor, y: torch.Tensor, srt: ExpertSort, gates: torch.Tensor):
+    """Gradients of :func:`unpermute_tokens`: ``(dy [T * k, H], dgates fp32 [T, k])`` in one pass over ``dout`` and ``y``. Rows of ``dy``
+    from ``offsets[E]`` on are zero, as is ``dgates`` of a dropped assignment."""
+    dout = _rows_arg(dout, srt.tokens, "dout")
+    y = _rows_arg(y, srt.tokens * srt.top_k, "y")
+    n = _sort_arg(srt, y)
+    if dout.dtype != y.dtype or dout.shape[1] != y.shape[1]:
+        raise ValueError("dout and y must have the same dtype and width")
+    nv.same_cuda_device(y, dout=dout)
+    g = _gates_arg(gates, srt, y)
+    dy = torch.empty((n, y.shape[1]), dtype=y.dtype, device=y.device)
+    dgates = torch.empty((srt.tokens, srt.top_k), dtype=torch.float32, device=y.device)
+    if n:
+        with nv.on_device(y):
+            nv.check(nv.bound("pkb_moe_unpermute_bwd", _UNPERMUTE_BWD)(
+                dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0), srt.slots.data_ptr(), g.data_ptr(), _kept_ptr(srt), dy.data_ptr(),
+                dgates.data_ptr(), srt.tokens, srt.top_k, y.shape[1], _DT[y.dtype], nv.raw_stream(y)), "pkb_moe_unpermute_bwd")
+        nv.count_launch()
+    return dy, dgates
