@@ -123,12 +123,12 @@ def raw_stream(t) -> int:
 _bound: dict = {}
 
 
-def bound(name: str, argtypes: list):
+def bound(name: str, argtypes: list, restype=ctypes.c_int):
     """The entry point ``name`` with its argument types declared (plain integers and floats are passed then), looked up once."""
     f = _bound.get(name)
     if f is None:
         f = getattr(cuda_lib(), name)
-        f.argtypes = argtypes
+        f.argtypes, f.restype = argtypes, restype
         _bound[name] = f
     return f
 

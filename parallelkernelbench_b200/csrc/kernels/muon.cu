@@ -1,0 +1,656 @@
+// Orthogonalising a matrix by Newton-Schulz products, and the optimiser step around it.
+//   X0 = U / (|U|_F + eps);  A = X X^T,  B = b A + c A^2,  X <- a X + B X  (steps times; X^T X and X B where X has more rows than columns)
+// Every singular value s of X goes to a s + b s^3 + c s^5, so all of them approach 1 while the singular vectors stay.
+//
+// Numerics. The iterate is a state and is kept in fp32 (M = k X, k a power of two near the square root of the longer side, so that its
+// entries are of the order of one); products run on the tensor cores from a copy of it rounded to fp16, with fp32 accumulation, and a X is
+// added in fp32: what rounding adds to the small singular directions is not fed back through the linear term. fp16 because its 11 bits
+// are 8 times as fine as bf16's at the same rate and nothing here leaves its range: |X|_2 <= 1 at the start and stays under the bound that the
+// host checks for the coefficients, the Gram matrix A and B are O(1). Against 64 bits five steps are 1e-3 to 2e-3 off (2-norm) with fp16
+// and 1e-2 to 2e-2 with bf16; with the iterate itself in fp16 a matrix of rank 16 in noise was 4e-2 off.
+//
+// Work: per step m (m + 1) n + m^2 (m + 1) + 2 m^2 n flops on the smaller side m: A and B are symmetric, so only the tiles on and below the
+// diagonal are computed and each is stored twice. Tensor-core bound from about m = 1000 on, bound by the latency of its launches below.
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "pkb/api.h"
+#include "pkb/gemm_umma.cuh"
+#include "pkb/host.h"
+
+namespace pkb {
+
+namespace {
+
+constexpr int kNsTile = 256;                                  // rows and columns of a CTA pair's tile
+constexpr int kNsStages = 6;
+constexpr int kNsOperandBytes = 128 * kGemmBlockK * 2;        // a CTA's half of an operand
+constexpr int kNsStageBytes = 2 * kNsOperandBytes;
+constexpr int kNsSmem = kNsStages * kNsStageBytes + 256 + 1024;
+constexpr uint32_t kNsKernelId = 111;
+
+enum NsEpilogue : int {
+  kNsGram = 0,      // A = alpha acc, both triangles
+  kNsPoly = 1,      // B = b A + c acc, both triangles
+  kNsUpdate = 2,    // M = a M + acc, X16 = fp16(M)
+  kNsResult = 3,    // out = bf16(scale (a M + acc))
+  kNsStep = 4,      // p = decay p - scale (a M + acc), p_bf16 = bf16(p)
+};
+
+struct NsParams {
+  int rows, cols, K, batch;     // output rows and columns of one matrix, inner extent
+  __half* out16;                // fp16 result (A, B or the next X), pitch16 halves per row
+  const __half* a16;            // A, read by kNsPoly
+  long long pitch16;
+  float* master;                // M, pitch_m floats per row
+  long long pitch_m;
+  void* final_out;              // kNsResult: bf16 [batch, rows, cols]; kNsStep: p, fp32 of that shape
+  __nv_bfloat16* p_bf16;        // kNsStep: optional
+  float alpha, beta;            // see NsEpilogue: (alpha, -), (c, b), (1, a), (scale, a), (scale, a)
+  float decay;
+  int vec_out;                  // the final result's rows start on 16 bytes
+  uint32_t* status;
+  uint64_t wait_budget_ns;
+};
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+
+__device__ __forceinline__ void tma_load_3d_pair_p(uint32_t smem_dst, const CUtensorMap* desc, uint32_t bar, int32_t c0, int32_t c1, int32_t c2,
+                                                   uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}\n"
+      :
+      : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(desc)), "r"(bar & kPeerBitMask), "r"(c0), "r"(c1), "r"(c2), "r"(lead)
+      : "memory");
+}
+
+// the row of the triangle's t-th element (rows of 1, 2, 3, ... elements)
+__host__ __device__ inline int tri_row(int t) {
+  int r = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+  while ((r + 1) * (r + 2) / 2 <= t) ++r;
+  while (r * (r + 1) / 2 > t) --r;
+  return r;
+}
+
+// Tile order: groups of eight tile rows, columns outermost inside a group, so that the tiles in flight share operand panels in L2. For the
+// symmetric products only tiles with row >= column.
+constexpr int kNsGroup = 8;
+template <bool SYM>
+__device__ __forceinline__ void ns_tile(int t, int num_m, int num_n, int& i, int& j) {
+  if constexpr (SYM) {
+    const int first = tri_row(t) / kNsGroup * kNsGroup;
+    const int gm = min(kNsGroup, num_m - first);
+    const int local = t - first * (first + 1) / 2;
+    if (local < first * gm) {
+      j = local / gm;
+      i = first + local - j * gm;
+    } else {
+      const int rem = local - first * gm, r = tri_row(rem);
+      i = first + r;
+      j = first + rem - r * (r + 1) / 2;
+    }
+  } else {
+    const int first = t / (kNsGroup * num_n) * kNsGroup;
+    const int gm = min(kNsGroup, num_m - first);
+    const int local = t - first * num_n;
+    j = local / gm;
+    i = first + local - j * gm;
+  }
+}
+
+// Persistent GEMM on clusters of two CTAs, tiles of 256 x 256 (tcgen05.mma.cta_group::2, M = 256): warp 0 of both CTAs loads, warp 1 of
+// the leader issues the products into two accumulators in tensor memory, warps 2 to 5 of both CTAs turn the finished one into results
+// meanwhile. A_MN / B_MN: the operand is [K, rows] row-major and is described to the tensor core as MN-major.
+template <bool A_MN, bool B_MN, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const NsParams p) {
+  constexpr bool kSym = EPI == kNsGram || EPI == kNsPoly;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t bar_base = smem_base + kNsStages * kNsStageBytes;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (kNsStages + s); };
+  auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * kNsStages + a); };
+  auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * kNsStages + 2 + a); };
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem_gen + kNsStages * kNsStageBytes + 8 * (2 * kNsStages + 4));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta_rank = cluster_ctarank();
+  const bool leader = cta_rank == 0;
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const int num_m = (p.rows + kNsTile - 1) / kNsTile, num_n = (p.cols + kNsTile - 1) / kNsTile;
+  const int num_k = (p.K + kGemmBlockK - 1) / kGemmBlockK;
+  const int per_matrix = kSym ? num_m * (num_m + 1) / 2 : num_m * num_n;
+  const int num_tiles = per_matrix * p.batch;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < kNsStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), 8);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_holder), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_holder;
+
+  if (warp == 0) {
+    const uint32_t lead = elect_one() ? 1u : 0u;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+      const int b = tile / per_matrix;
+      int ti, tj;
+      ns_tile<kSym>(tile - b * per_matrix, num_m, num_n, ti, tj);
+      const int row0 = ti * kNsTile + (int)cta_rank * 128, col0 = tj * kNsTile + (int)cta_rank * 128;
+      for (int kb = 0; kb < num_k; ++kb) {
+        if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_budget_ns)) {
+          if (lane == 0) record_status(p.status, kStatusMbarTimeout, kNsKernelId, 0, stage, 11, tile);
+          ok = false;
+          break;
+        }
+        mbar_expect_tx_p(full_bar(stage), 2 * kNsStageBytes, leader ? lead : 0u);
+        const uint32_t sa = smem_base + stage * kNsStageBytes, sb = sa + kNsOperandBytes;
+        const int k0 = kb * kGemmBlockK;
+        if constexpr (A_MN) {
+          tma_load_3d_pair_p(sa, &tmap_a, full_bar(stage), row0, k0, b, lead);
+          tma_load_3d_pair_p(sa + 8192, &tmap_a, full_bar(stage), row0 + 64, k0, b, lead);
+        } else {
+          tma_load_3d_pair_p(sa, &tmap_a, full_bar(stage), k0, row0, b, lead);
+        }
+        if constexpr (B_MN) {
+          tma_load_3d_pair_p(sb, &tmap_b, full_bar(stage), col0, k0, b, lead);
+          tma_load_3d_pair_p(sb + 8192, &tmap_b, full_bar(stage), col0 + 64, k0, b, lead);
+        } else {
+          tma_load_3d_pair_p(sb, &tmap_b, full_bar(stage), k0, col0, b, lead);
+        }
+        if (++stage == kNsStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (leader) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      constexpr uint32_t idesc = make_idesc(kNsTile, kNsTile, 0, 0, A_MN ? 1 : 0, B_MN ? 1 : 0);
+      const uint32_t a_lo0 = A_MN ? smem_desc_lo_mnmajor(smem_base, 8192u) : smem_desc_lo_kmajor(smem_base);
+      const uint32_t b_lo0 = B_MN ? smem_desc_lo_mnmajor(smem_base + kNsOperandBytes, 8192u) : smem_desc_lo_kmajor(smem_base + kNsOperandBytes);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.wait_budget_ns)) {
+          if (lane == 0) record_status(p.status, kStatusMbarTimeout, kNsKernelId, 0, acc, 20, tile);
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t tmem_d = tmem_base + acc * 256;
+        for (int kb = 0; kb < num_k; ++kb) {
+          if (!mbar_wait(full_bar(stage), phase, abort_flag, p.wait_budget_ns)) {
+            if (lane == 0) record_status(p.status, kStatusMbarTimeout, kNsKernelId, 0, stage, 21, tile);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t a_lo = a_lo0 + stage * (kNsStageBytes >> 4), b_lo = b_lo0 + stage * (kNsStageBytes >> 4);
+#pragma unroll
+          for (int k = 0; k < kGemmBlockK / 16; ++k)
+            umma_f16_ss_pair_p(tmem_d, smem_desc_join(a_lo + (A_MN ? 128u : 2u) * k), smem_desc_join(b_lo + (B_MN ? 128u : 2u) * k), idesc,
+                               (kb | k) != 0 ? 1u : 0u, lead);
+          umma_commit_pair_p(empty_bar(stage), 0x3, lead);
+          if (++stage == kNsStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        umma_commit_pair_p(tfull_bar(acc), 0x3, lead);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    const uint32_t leader_tempty0 = mapa_shared(tempty_bar(0), 0), leader_tempty1 = mapa_shared(tempty_bar(1), 0);
+    for (int tile = pair; tile < num_tiles; tile += num_pairs) {
+      const int b = tile / per_matrix;
+      int ti, tj;
+      ns_tile<kSym>(tile - b * per_matrix, num_m, num_n, ti, tj);
+      bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.wait_budget_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (lane == 0) record_status(p.status, kStatusMbarTimeout, kNsKernelId, 0, acc, 30, tile);
+        break;
+      }
+      tc_fence_after_sync();
+      const int row = ti * kNsTile + (int)cta_rank * 128 + q * 32 + lane;
+      const bool row_ok = row < p.rows;
+      const long long grow = (long long)b * p.rows + row;     // row of the stack of matrices
+#pragma unroll 1
+      for (int c = 0; c < kNsTile / 32; ++c) {
+        const int col0 = tj * kNsTile + c * 32;
+        if (col0 >= p.cols) break;
+        uint32_t r[32];
+        tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * 256 + c * 32), r);
+        tmem_ld_wait();
+        const int width = min(32, p.cols - col0), width8 = (width + 7) & ~7;     // rows of the scratch tensors are padded to eights
+        if constexpr (kSym) {
+          uint32_t w[16];
+          if constexpr (EPI == kNsPoly) {
+            // the padding of a row up to its pitch is readable, so groups of eight never leave the row
+            const __half* src = p.a16 + grow * p.pitch16 + col0;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              U4 u{0u, 0u, 0u, 0u};
+              if (row_ok && v * 8 < width) u = ld_global_v4(src + v * 8);
+              const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int h = 0; h < 4; ++h) {
+                const float2 f = unpack_half2(in[h]);
+                w[v * 4 + h] = pack_half2(fmaf(p.alpha, __uint_as_float(r[v * 8 + 2 * h]), p.beta * f.x),
+                                          fmaf(p.alpha, __uint_as_float(r[v * 8 + 2 * h + 1]), p.beta * f.y));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int h = 0; h < 16; ++h) w[h] = pack_half2(p.alpha * __uint_as_float(r[2 * h]), p.alpha * __uint_as_float(r[2 * h + 1]));
+          }
+          if (row_ok) {
+            __half* dst = p.out16 + grow * p.pitch16 + col0;
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (v * 8 < width) st_global_v4(dst + v * 8, U4{w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]});
+          }
+          if (ti != tj && row_ok) {
+            // the mirrored half: 32 lanes hold 32 consecutive columns of row col0 + j
+            __half* dst = p.out16 + ((long long)b * p.rows + col0) * p.pitch16 + row;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < width) {
+                const uint32_t h2 = w[j >> 1];
+                dst[(long long)j * p.pitch16] = __ushort_as_half((unsigned short)((j & 1) ? h2 >> 16 : h2 & 0xffffu));
+              }
+          }
+        } else if (row_ok) {
+          const float* mrow = p.master + grow * p.pitch_m + col0;
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            if (j < width8) {
+              const U4 u = ld_global_v4(mrow + j);
+              v[j] = fmaf(p.beta, __uint_as_float(u.x), __uint_as_float(r[j]));
+              v[j + 1] = fmaf(p.beta, __uint_as_float(u.y), __uint_as_float(r[j + 1]));
+              v[j + 2] = fmaf(p.beta, __uint_as_float(u.z), __uint_as_float(r[j + 2]));
+              v[j + 3] = fmaf(p.beta, __uint_as_float(u.w), __uint_as_float(r[j + 3]));
+            }
+          }
+          if constexpr (EPI == kNsUpdate) {
+            float* mdst = p.master + grow * p.pitch_m + col0;
+            __half* xdst = p.out16 + grow * p.pitch16 + col0;
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              if (j < width) {
+                st_global_v4(mdst + j, U4{__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3])});
+                st_global_v4(mdst + j + 4, U4{__float_as_uint(v[j + 4]), __float_as_uint(v[j + 5]), __float_as_uint(v[j + 6]), __float_as_uint(v[j + 7])});
+                st_global_v4(xdst + j, U4{pack_half2(v[j], v[j + 1]), pack_half2(v[j + 2], v[j + 3]), pack_half2(v[j + 4], v[j + 5]),
+                                          pack_half2(v[j + 6], v[j + 7])});
+              }
+            }
+          } else if constexpr (EPI == kNsResult) {
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.final_out) + grow * p.cols + col0;
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              if (j >= width) break;
+              if (p.vec_out) {
+                st_global_v4(dst + j, U4{pack_bf16x2(p.alpha * v[j], p.alpha * v[j + 1]), pack_bf16x2(p.alpha * v[j + 2], p.alpha * v[j + 3]),
+                                         pack_bf16x2(p.alpha * v[j + 4], p.alpha * v[j + 5]), pack_bf16x2(p.alpha * v[j + 6], p.alpha * v[j + 7])});
+              } else {
+#pragma unroll
+                for (int i = j; i < j + 8; ++i)
+                  if (i < width) dst[i] = __float2bfloat16_rn(p.alpha * v[i]);
+              }
+            }
+          } else {
+            float* dst = static_cast<float*>(p.final_out) + grow * p.cols + col0;
+            __nv_bfloat16* dst16 = p.p_bf16 != nullptr ? p.p_bf16 + grow * p.cols + col0 : nullptr;
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              if (j >= width) break;
+              if (p.vec_out) {
+                const U4 u0 = ld_global_v4(dst + j), u1 = ld_global_v4(dst + j + 4);
+                const uint32_t in[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[j + i] = fmaf(-p.alpha, v[j + i], p.decay * __uint_as_float(in[i]));
+                st_global_v4(dst + j, U4{__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3])});
+                st_global_v4(dst + j + 4, U4{__float_as_uint(v[j + 4]), __float_as_uint(v[j + 5]), __float_as_uint(v[j + 6]), __float_as_uint(v[j + 7])});
+                if (dst16 != nullptr)
+                  st_global_v4(dst16 + j, U4{pack_bf16x2(v[j], v[j + 1]), pack_bf16x2(v[j + 2], v[j + 3]), pack_bf16x2(v[j + 4], v[j + 5]),
+                                             pack_bf16x2(v[j + 6], v[j + 7])});
+              } else {
+#pragma unroll
+                for (int i = j; i < j + 8; ++i)
+                  if (i < width) {
+                    const float np = fmaf(-p.alpha, v[i], p.decay * dst[i]);
+                    dst[i] = np;
+                    if (dst16 != nullptr) dst16[i] = __float2bfloat16_rn(np);
+                  }
+              }
+            }
+          }
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc == 0 ? leader_tempty0 : leader_tempty1);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag) {      // copies and products in flight end before the memory that they use goes away
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ what goes before the products
+// m <- momentum m + g, u = g + momentum m (Nesterov) or m; without momentum (m null) u = g. The sums of u^2 are 64-bit: squares of fp32 values
+// neither overflow nor vanish there. part[matrix][block], added by every block of the next kernel in the same order.
+struct NsInput {
+  const void* g;
+  int g_f32;
+  float* m;
+  float momentum;
+  int nesterov;
+  __device__ __forceinline__ float grad(long long i) const {
+    return g_f32 ? static_cast<const float*>(g)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(g)[i]);
+  }
+  __device__ __forceinline__ float use(float gv, float mv) const { return m == nullptr ? gv : nesterov ? fmaf(momentum, mv, gv) : mv; }
+};
+
+constexpr int kNsPrepThreads = 256;
+constexpr int kNsMaxParts = 256;
+
+__device__ __forceinline__ double block_sum_double(double v, double* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double t = 0.0;
+#pragma unroll
+  for (int w = 0; w < kNsPrepThreads / 32; ++w) t += red[w];
+  __syncthreads();
+  return t;
+}
+
+__device__ __forceinline__ void load4(const NsInput& in, long long i, float (&g)[4]) {
+  if (in.g_f32) {
+    const U4 u = ld_global_v4(static_cast<const float*>(in.g) + i);
+    g[0] = __uint_as_float(u.x); g[1] = __uint_as_float(u.y); g[2] = __uint_as_float(u.z); g[3] = __uint_as_float(u.w);
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(in.g) + i);
+    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
+    g[0] = a.x; g[1] = a.y; g[2] = b.x; g[3] = b.y;
+  }
+}
+
+// VEC4: every matrix is a multiple of four values and its tensors start on 16 bytes (bf16: 8)
+template <bool VEC4>
+__global__ void __launch_bounds__(kNsPrepThreads)
+ns_norm_kernel(const NsInput in, long long numel, double* __restrict__ part) {
+  __shared__ double red[kNsPrepThreads / 32];
+  const long long base = (long long)blockIdx.y * numel;
+  constexpr int W = VEC4 ? 4 : 1;
+  double s = 0.0;
+  for (long long i = ((long long)blockIdx.x * kNsPrepThreads + threadIdx.x) * W; i < numel; i += (long long)gridDim.x * kNsPrepThreads * W) {
+    float g[W], u[W];
+    if constexpr (VEC4) load4(in, base + i, g);
+    else g[0] = in.grad(base + i);
+    if (in.m != nullptr) {
+      float m[W];
+      if constexpr (VEC4) {
+        const U4 v = ld_global_v4(in.m + base + i);
+        m[0] = __uint_as_float(v.x); m[1] = __uint_as_float(v.y); m[2] = __uint_as_float(v.z); m[3] = __uint_as_float(v.w);
+      } else {
+        m[0] = in.m[base + i];
+      }
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        m[j] = fmaf(in.momentum, m[j], g[j]);
+        u[j] = in.use(g[j], m[j]);
+      }
+      if constexpr (VEC4) st_global_v4(in.m + base + i, U4{__float_as_uint(m[0]), __float_as_uint(m[1]), __float_as_uint(m[2]), __float_as_uint(m[3])});
+      else in.m[base + i] = m[0];
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; ++j) u[j] = g[j];
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) s += (double)u[j] * (double)u[j];
+  }
+  s = block_sum_double(s, red);
+  if (threadIdx.x == 0) part[(long long)blockIdx.y * gridDim.x + blockIdx.x] = s;
+}
+
+// M = k u / (|u| + eps) and its fp16 copy, rows padded to their pitch with zeros
+__global__ void __launch_bounds__(kNsPrepThreads)
+ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* __restrict__ part, int parts, double eps, double k,
+                float* __restrict__ master, __half* __restrict__ x16) {
+  __shared__ double red[kNsPrepThreads / 32];
+  const long long b = blockIdx.y;
+  const double sum = block_sum_double((int)threadIdx.x < parts ? part[b * parts + threadIdx.x] : 0.0, red);
+  const double inv = k / (sqrt(sum) + eps);
+  const int vecs = pitch / 4;
+  const long long total = (long long)rows * vecs, base = b * rows * cols;
+  const bool vec4 = cols % 4 == 0 && (reinterpret_cast<uintptr_t>(in.g) & 15) == 0 && (reinterpret_cast<uintptr_t>(in.m) & 15) == 0;
+  for (long long i = (long long)blockIdx.x * kNsPrepThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kNsPrepThreads) {
+    const long long r = i / vecs;
+    const int c = (int)(i - r * vecs) * 4;
+    float u[4];
+    const long long at = base + r * cols + c;
+    if (vec4 && c < cols) {
+      float g[4];
+      load4(in, at, g);
+      U4 v{0u, 0u, 0u, 0u};
+      if (in.m != nullptr) v = ld_global_v4(in.m + at);
+      const uint32_t m[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = in.use(g[j], __uint_as_float(m[j]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = c + j < cols ? in.use(in.grad(at + j), in.m != nullptr ? in.m[at + j] : 0.f) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = (float)((double)u[j] * inv);
+    const long long dst = (b * rows + r) * pitch + c;
+    st_global_v4(master + dst, U4{__float_as_uint(u[0]), __float_as_uint(u[1]), __float_as_uint(u[2]), __float_as_uint(u[3])});
+    *reinterpret_cast<uint2*>(x16 + dst) = make_uint2(pack_half2(u[0], u[1]), pack_half2(u[2], u[3]));
+  }
+}
+
+template <bool A_MN, bool B_MN, int EPI>
+int ns_gemm(const CUtensorMap& ta, const CUtensorMap& tb, NsParams p, cudaStream_t s) {
+  const long long num_m = (p.rows + kNsTile - 1) / kNsTile, num_n = (p.cols + kNsTile - 1) / kNsTile;
+  const long long tiles = (EPI == kNsGram || EPI == kNsPoly ? num_m * (num_m + 1) / 2 : num_m * num_n) * p.batch;
+  PKB_CHECK_ARG(tiles < (1ll << 24), "too many tiles");
+  int ctas = sm_count() & ~1;
+  if (ctas > 2 * tiles) ctas = (int)(2 * tiles);
+  auto kern = ns_gemm_kernel<A_MN, B_MN, EPI>;
+  PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem));
+  kern<<<ctas, kGemmThreads, kNsSmem, s>>>(ta, tb, p);
+  PKB_CHECK_CUDA(cudaGetLastError());
+  return kApiOk;
+}
+
+long long pad8(long long n) { return (n + 7) / 8 * 8; }
+long long pad256(long long n) { return (n + 255) / 256 * 256; }
+
+// scratch: M [batch, rows, pitch] fp32, X twice the same in fp16, A and B [batch, m, pitch of m] in fp16, the norm's partial sums
+struct NsScratch {
+  long long master, x0, x1, a, b, part, total;
+  NsScratch(long long batch, long long rows, long long cols) {
+    const long long m = rows < cols ? rows : cols, x = batch * rows * pad8(cols), g = batch * m * pad8(m);
+    master = 0;
+    x0 = master + pad256(4 * x);
+    x1 = x0 + pad256(2 * x);
+    a = x1 + pad256(2 * x);
+    b = a + pad256(2 * g);
+    part = b + pad256(2 * g);
+    total = part + pad256(8 * batch * kNsMaxParts);
+  }
+};
+
+}  // namespace
+
+}  // namespace pkb
+
+using namespace pkb;
+
+extern "C" long long pkb_newton_schulz_scratch(long long batch, int rows, int cols) {
+  return batch > 0 && rows > 0 && cols > 0 ? NsScratch(batch, rows, cols).total : 0;
+}
+
+// Orthogonalises `batch` matrices [rows, cols] u (see NsInput: g bf16 or fp32, with the momentum m fp32 updated in place where it is not null).
+// coeff: HOST array of steps triples (a, b, c). Result, by p: null -> out bf16 [batch, rows, cols]; else p (fp32) <- decay p - scale o,
+// with a bf16 copy in p_bf16 where that is not null. scratch: pkb_newton_schulz_scratch bytes on a 256-byte boundary.
+extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float momentum, int nesterov, long long batch, int rows, int cols,
+                                 const float* coeff, int steps, double eps, void* out, void* p, float decay, float scale, void* p_bf16,
+                                 void* scratch, void* stream) {
+  PKB_CHECK_ARG(batch > 0 && batch <= 65535 && rows > 0 && cols > 0, "1 .. 65535 matrices of at least one row and column");
+  PKB_CHECK_ARG(steps >= 1 && coeff != nullptr, "at least one step");
+  PKB_CHECK_ARG(g != nullptr && scratch != nullptr && ((out != nullptr) != (p != nullptr)), "g, scratch and one of out and p");
+  PKB_CHECK_ARG((reinterpret_cast<uintptr_t>(scratch) & 255) == 0, "scratch must start on 256 bytes");
+  // the first call on a device allocates its status block: let that happen inside a graph capture, too
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  PKB_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  uint32_t* status = status_block_device_ptr();
+  PKB_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const NsScratch at(batch, rows, cols);
+  uint8_t* base = static_cast<uint8_t*>(scratch);
+  const bool tall = rows > cols;
+  const int side = tall ? cols : rows, longer = tall ? rows : cols;
+  const long long pitch = pad8(cols), pitch_a = pad8(side), numel = (long long)rows * cols;
+  const double k = ldexp(1.0, (int)lrint(log2((double)longer) / 2));
+  float* master = reinterpret_cast<float*>(base + at.master);
+  __half *x[2] = {reinterpret_cast<__half*>(base + at.x0), reinterpret_cast<__half*>(base + at.x1)};
+  __half *a16 = reinterpret_cast<__half*>(base + at.a), *b16 = reinterpret_cast<__half*>(base + at.b);
+  double* part = reinterpret_cast<double*>(base + at.part);
+
+  const NsInput in{g, g_f32, static_cast<float*>(m), momentum, nesterov};
+  const bool vec4 = numel % 4 == 0 && ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m)) & 15) == 0;
+  const long long most = ((long long)sm_count() * 8 + batch - 1) / batch;          // blocks per matrix that fill the GPU
+  auto blocks_for = [&](long long items, long long cap) {
+    long long n = (items + kNsPrepThreads - 1) / kNsPrepThreads;
+    if (n > most) n = most;
+    if (n > cap) n = cap;
+    return (int)(n < 1 ? 1 : n);
+  };
+  const int parts = blocks_for(vec4 ? numel / 4 : numel, kNsMaxParts);
+  if (vec4) ns_norm_kernel<true><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
+  else ns_norm_kernel<false><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
+  PKB_CHECK_CUDA(cudaGetLastError());
+  const int start_blocks = blocks_for((long long)rows * (pitch / 4), 1 << 20);
+  ns_start_kernel<<<dim3((unsigned)start_blocks, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, rows, cols, (int)pitch, part, parts, eps, k, master, x[0]);
+  PKB_CHECK_CUDA(cudaGetLastError());
+
+  // maps of X as an operand whose rows lie along K (boxes of 64 columns x 128 rows) and as one whose rows are K (64 x 64), and of A and B
+  CUtensorMap xk[2], xm[2], ak, bk;
+  int rc;
+  for (int i = 0; i < 2; ++i) {
+    rc = encode_tmap_3d(&xk[i], kTmapFp16, x[i], cols, rows, batch, pitch * 2, rows * pitch * 2, kGemmBlockK, 128, 1, kSwizzle128);
+    if (rc) return rc;
+    rc = encode_tmap_3d(&xm[i], kTmapFp16, x[i], cols, rows, batch, pitch * 2, rows * pitch * 2, 64, kGemmBlockK, 1, kSwizzle128);
+    if (rc) return rc;
+  }
+  rc = encode_tmap_3d(&ak, kTmapFp16, a16, side, side, batch, pitch_a * 2, side * pitch_a * 2, kGemmBlockK, 128, 1, kSwizzle128);
+  if (rc) return rc;
+  rc = encode_tmap_3d(&bk, kTmapFp16, b16, side, side, batch, pitch_a * 2, side * pitch_a * 2, kGemmBlockK, 128, 1, kSwizzle128);
+  if (rc) return rc;
+
+  NsParams q = {};
+  q.batch = (int)batch;
+  q.vec_out = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(p_bf16)) & 15) == 0;
+  q.status = status;
+  q.wait_budget_ns = kDefaultWaitBudgetNs;
+  for (int step = 0; step < steps; ++step) {
+    const float *co = coeff + 3 * step;
+    const int cur = step & 1;
+    NsParams e = q;
+    e.rows = e.cols = side;
+    e.pitch16 = pitch_a;
+    e.K = longer;
+    e.out16 = a16;
+    e.alpha = (float)(1.0 / (k * k));
+    rc = tall ? ns_gemm<true, true, kNsGram>(xm[cur], xm[cur], e, s) : ns_gemm<false, false, kNsGram>(xk[cur], xk[cur], e, s);
+    if (rc) return rc;
+    e.K = side;
+    e.a16 = a16;
+    e.out16 = b16;
+    e.alpha = co[2];
+    e.beta = co[1];
+    rc = ns_gemm<false, false, kNsPoly>(ak, ak, e, s);
+    if (rc) return rc;
+    NsParams u = q;
+    u.rows = rows;
+    u.cols = cols;
+    u.K = side;
+    u.out16 = x[cur ^ 1];
+    u.pitch16 = u.pitch_m = pitch;
+    u.master = master;
+    u.beta = co[0];
+    if (step + 1 < steps) {
+      rc = tall ? ns_gemm<false, false, kNsUpdate>(xk[cur], bk, u, s) : ns_gemm<false, true, kNsUpdate>(bk, xm[cur], u, s);
+    } else if (p == nullptr) {
+      u.final_out = out;
+      u.alpha = (float)(1.0 / k);
+      rc = tall ? ns_gemm<false, false, kNsResult>(xk[cur], bk, u, s) : ns_gemm<false, true, kNsResult>(bk, xm[cur], u, s);
+    } else {
+      u.final_out = p;
+      u.p_bf16 = static_cast<__nv_bfloat16*>(p_bf16);
+      u.alpha = (float)(scale / k);
+      u.decay = decay;
+      rc = tall ? ns_gemm<false, false, kNsStep>(xk[cur], bk, u, s) : ns_gemm<false, true, kNsStep>(bk, xm[cur], u, s);
+    }
+    if (rc) return rc;
+  }
+  return kApiOk;
+}

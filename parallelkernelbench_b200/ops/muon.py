@@ -1,0 +1,110 @@
+"""Orthogonalised updates (kernels: csrc/kernels/muon.cu): Newton-Schulz products on the tensor cores, and the optimiser step around them.
+
+The step stands beside :func:`~parallelkernelbench_b200.ops.elementwise.adam_step`: it is for the matrices of a model (embeddings, heads, gains
+and biases keep Adam).
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+import torch
+
+from .. import _native as nv
+
+_P, _I, _LL, _F, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_double
+_ARGS = [_P, _I, _P, _F, _I, _LL, _I, _I, _P, _I, _D, _P, _P, _F, _F, _P, _P, _P]
+_DT = {torch.bfloat16: 0, torch.float32: 1}
+
+#: Coefficients (a, b, c) of a step s -> a s + b s^3 + c s^5 that lift small singular values fast and leave them within about 0.7 .. 1.2.
+FAST = (3.4445, -4.7750, 2.0315)
+
+
+@functools.lru_cache(maxsize=64)
+def _coefficients(coefficients, steps: int, longer: int):
+    """The steps' coefficients as a C array. The products run in fp16: what the singular values (at most 1 at the start), the Gram matrix and
+    the polynomial can reach has to stay inside its range."""
+    per_step = coefficients if isinstance(coefficients[0], tuple) else (coefficients,) * steps
+    if len(per_step) != steps or any(len(c) != 3 for c in per_step):
+        raise ValueError("coefficients are one (a, b, c) or one per step")
+    top = 1.0
+    k = 2.0 ** round(math.log2(longer) / 2)
+    for a, b, c in per_step:
+        if not all(math.isfinite(v) for v in (a, b, c)):
+            raise ValueError("coefficients must be finite")
+        inner = abs(b) * top ** 2 + abs(c) * top ** 4
+        top = 1.01 * max(abs(a * s + b * s ** 3 + c * s ** 5) for s in (top * i / 512 for i in range(513)))
+        if not max(inner, top * top, top * k) <= 3e4:
+            raise ValueError("these coefficients can leave the range of fp16")
+    flat = [v for c in per_step for v in c]
+    return (ctypes.c_float * len(flat))(*flat)
+
+
+def _launch(g, m, momentum, nesterov, steps, coefficients, eps, out, p, decay, scale, p_bf16) -> None:
+    rows, cols = g.shape[-2:]
+    batch = g.numel() // (rows * cols)
+    if batch > 65535:
+        raise ValueError("at most 65535 matrices at once")
+    if max(rows, cols) >= 1 << 24:
+        raise ValueError("sides of at most 2^24 - 1")
+    if isinstance(coefficients, list) or (len(coefficients) and isinstance(coefficients[0], list)):
+        coefficients = tuple(tuple(c) if isinstance(c, list) else c for c in coefficients)
+    if not steps >= 1 or not eps >= 0:
+        raise ValueError("at least one step, and eps >= 0")
+    if not len(coefficients):
+        raise ValueError("coefficients are one (a, b, c) or one per step")
+    coeff = _coefficients(coefficients, int(steps), max(rows, cols))
+    g = g.contiguous()
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    with nv.on_device(g):
+        scratch = torch.empty(nv.bound("pkb_newton_schulz_scratch", [_LL, _I, _I], _LL)(batch, rows, cols), dtype=torch.uint8, device=g.device)
+        nv.check(nv.bound("pkb_newton_schulz", _ARGS)(
+            g.data_ptr(), _DT[g.dtype], ptr(m), momentum, int(nesterov), batch, rows, cols, coeff, steps, eps, ptr(out), ptr(p), decay, scale,
+            ptr(p_bf16), scratch.data_ptr(), nv.raw_stream(g)), "pkb_newton_schulz")
+    nv.count_launch(2 + 3 * steps)
+
+
+def newton_schulz(g: torch.Tensor, *, steps: int = 5, coefficients=FAST, eps: float = 1e-7) -> torch.Tensor:
+    """Orthogonalises the matrices ``g`` (bf16 or fp32 ``[..., rows, cols]``, any sides): ``X = g / (|g|_F + eps)``, then ``steps`` times
+    ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``. ``coefficients`` is one ``(a, b, c)`` or a sequence of one per step. Returns bf16 of the
+    same shape. The iterate is held in fp32 and multiplied in fp16 with fp32 sums. A matrix of zeros stays zero; one with a value that is not
+    finite comes back as NaN, alone."""
+    if g.dtype not in _DT:
+        raise TypeError(f"newton_schulz takes bf16 or fp32, got {g.dtype}")
+    if g.dim() < 2:
+        raise ValueError("newton_schulz takes matrices [..., rows, cols]")
+    nv.same_cuda_device(g)
+    out = torch.empty(g.shape, dtype=torch.bfloat16, device=g.device)
+    if g.numel():
+        _launch(g, None, 0.0, False, steps, coefficients, eps, out, None, 0.0, 0.0, None)
+    return out
+
+
+def muon_step(p: torch.Tensor, m: torch.Tensor, g: torch.Tensor, *, lr: float, momentum: float = 0.95, nesterov: bool = True,
+              weight_decay: float = 0.0, scale: float | None = None, steps: int = 5, coefficients=FAST, eps: float = 1e-7,
+              p_bf16: torch.Tensor | None = None) -> None:
+    """One step on fp32 matrices ``p [..., rows, cols]`` with the momentum ``m`` (fp32) and the gradient ``g`` (bf16 or fp32), in place::
+
+        m <- momentum * m + g;   u = g + momentum * m (nesterov) or m
+        p <- p * (1 - lr * weight_decay) - lr * scale * newton_schulz(u)
+
+    ``scale`` defaults to ``0.2 * sqrt(max(rows, cols))``: an update of about Adam's root mean square, so that its learning rate and decay carry
+    over. ``p_bf16`` receives a bf16 copy. Leading dimensions are matrices of their own (the experts of a MoE layer)."""
+    for name, t in (("p", p), ("m", m)):
+        if t.dtype != torch.float32 or not t.is_contiguous():
+            raise TypeError(f"{name} must be contiguous fp32")
+    if g.dtype not in _DT:
+        raise TypeError(f"g must be bf16 or fp32, got {g.dtype}")
+    if p.dim() < 2 or m.shape != p.shape or g.shape != p.shape:
+        raise ValueError("p, m and g must be matrices [..., rows, cols] of one shape")
+    if p_bf16 is not None and (p_bf16.dtype != torch.bfloat16 or p_bf16.shape != p.shape or not p_bf16.is_contiguous()):
+        raise ValueError("p_bf16 must be contiguous bf16 of the shape of p")
+    nv.same_cuda_device(p, m=m, g=g, p_bf16=p_bf16)
+    if not p.numel():
+        return
+    if m.data_ptr() == p.data_ptr():
+        raise ValueError("p and m must be different tensors")
+    if scale is None:
+        scale = 0.2 * math.sqrt(max(p.shape[-2:]))
+    _launch(g, m, momentum, nesterov, steps, coefficients, eps, None, p, 1.0 - lr * weight_decay, lr * scale, p_bf16)
