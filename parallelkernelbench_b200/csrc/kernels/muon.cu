@@ -26,7 +26,9 @@ constexpr int kNsTile = 256;                                  // rows and column
 constexpr int kNsStages = 6;
 constexpr int kNsOperandBytes = 128 * kGemmBlockK * 2;        // a CTA's half of an operand
 constexpr int kNsStageBytes = 2 * kNsOperandBytes;
-constexpr int kNsSmem = kNsStages * kNsStageBytes + 256 + 1024;
+constexpr int kNsThreads = 64 + 256;                          // loader, issuer, eight epilogue warps
+constexpr int kNsStageOut = 8 * 4096;                         // a 32 x 32 fp32 chunk per epilogue warp
+constexpr int kNsSmem = kNsStages * kNsStageBytes + kNsStageOut + 256 + 1024;
 constexpr uint32_t kNsKernelId = 111;
 
 enum NsEpilogue : int {
@@ -104,21 +106,21 @@ __device__ __forceinline__ void ns_tile(int t, int num_m, int num_n, int& i, int
 }
 
 // Persistent GEMM on clusters of two CTAs, tiles of 256 x 256 (tcgen05.mma.cta_group::2, M = 256): warp 0 of both CTAs loads, warp 1 of
-// the leader issues the products into two accumulators in tensor memory, warps 2 to 5 of both CTAs turn the finished one into results
+// the leader issues the products into two accumulators in tensor memory, warps 2 to 9 of both CTAs turn the finished one into results
 // meanwhile. A_MN / B_MN: the operand is [K, rows] row-major and is described to the tensor core as MN-major.
 template <bool A_MN, bool B_MN, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNsThreads, 1)
 ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const NsParams p) {
   constexpr bool kSym = EPI == kNsGram || EPI == kNsPoly;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
-  const uint32_t bar_base = smem_base + kNsStages * kNsStageBytes;
+  const uint32_t bar_base = smem_base + kNsStages * kNsStageBytes + kNsStageOut;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (kNsStages + s); };
   auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * kNsStages + a); };
   auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * kNsStages + 2 + a); };
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem_gen + kNsStages * kNsStageBytes + 8 * (2 * kNsStages + 4));
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem_gen + kNsStages * kNsStageBytes + kNsStageOut + 8 * (2 * kNsStages + 4));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -138,7 +140,7 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), 8);
+      mbar_init(tempty_bar(a), 16);     // eight epilogue warps of each CTA
     }
     fence_mbar_init();
     tma_prefetch_desc(&tmap_a);
@@ -236,7 +238,13 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     }
     __syncwarp();
   } else {
-    const int q = warp & 3;
+    // Two warps per quarter of a CTA's 128 rows, each with half of the tile's columns, 32 x 32 values at a time. The accumulator comes with a
+    // row per lane; through 4 KB of shared memory (16-byte pieces swizzled by the row) it is turned so that eight lanes hold 128 bytes of a
+    // row, and every access to global memory covers whole sectors. What the step adds (M, or A) is fetched one chunk ahead, for the first
+    // chunk while the products still run. With a row per lane in global memory as well, 4096 x 4096 took 123 us per update, 62 per Gram matrix.
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t stg = smem_base + kNsStages * kNsStageBytes + static_cast<uint32_t>(warp - 2) * 4096u;
+    const int trow = lane >> 3, tcol = (lane & 7) * 4;       // place in the turned chunk: rows trow + 4 it, columns tcol .. tcol + 3
     int acc = 0;
     uint32_t acc_phase = 0;
     const uint32_t leader_tempty0 = mapa_shared(tempty_bar(0), 0), leader_tempty1 = mapa_shared(tempty_bar(1), 0);
@@ -244,6 +252,30 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       const int b = tile / per_matrix;
       int ti, tj;
       ns_tile<kSym>(tile - b * per_matrix, num_m, num_n, ti, tj);
+      const int row0 = ti * kNsTile + (int)cta_rank * 128 + q * 32;
+      const int colh = tj * kNsTile + half * 128;
+      const int rows_here = p.rows - row0;                     // may be <= 0
+      const long long grow = (long long)b * p.rows + row0;     // first row in the stack of matrices
+      // the next chunk's M (four floats) or A (four halves) per row of the turned chunk; rows of the scratch tensors are padded to eights
+      uint4 in[8];
+      auto fetch = [&](int c) {
+        const int col = colh + c * 32 + tcol;
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const int r = trow + it * 4;
+          if (c < 4 && col < p.cols && r < rows_here) {
+            if constexpr (EPI == kNsPoly) {
+              const uint2 u = *reinterpret_cast<const uint2*>(p.a16 + (grow + r) * p.pitch16 + col);
+              in[it].x = u.x;
+              in[it].y = u.y;
+            } else if constexpr (EPI != kNsGram) {
+              const U4 u = ld_global_v4(p.master + (grow + r) * p.pitch_m + col);
+              in[it] = make_uint4(u.x, u.y, u.z, u.w);
+            }
+          }
+        }
+      };
+      fetch(0);
       bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.wait_budget_ns);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
@@ -251,118 +283,116 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         break;
       }
       tc_fence_after_sync();
-      const int row = ti * kNsTile + (int)cta_rank * 128 + q * 32 + lane;
-      const bool row_ok = row < p.rows;
-      const long long grow = (long long)b * p.rows + row;     // row of the stack of matrices
 #pragma unroll 1
-      for (int c = 0; c < kNsTile / 32; ++c) {
-        const int col0 = tj * kNsTile + c * 32;
-        if (col0 >= p.cols) break;
+      for (int c = 0; c < 4; ++c) {
+        const int col0 = colh + c * 32;
+        if (col0 >= p.cols || rows_here <= 0) break;
         uint32_t r[32];
-        tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * 256 + c * 32), r);
+        __syncwarp();                                           // the last chunk was read
+        tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * 256 + half * 128 + c * 32), r);
         tmem_ld_wait();
-        const int width = min(32, p.cols - col0), width8 = (width + 7) & ~7;     // rows of the scratch tensors are padded to eights
+#pragma unroll
+        for (int f = 0; f < 8; ++f)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + lane * 128u + ((f ^ (lane & 7)) << 4)), "r"(r[4 * f]), "r"(r[4 * f + 1]),
+                       "r"(r[4 * f + 2]), "r"(r[4 * f + 3])
+                       : "memory");
+        __syncwarp();
+        float v[8][4];
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const int tr = trow + it * 4;
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[it][0]), "=f"(v[it][1]), "=f"(v[it][2]), "=f"(v[it][3])
+                       : "r"(stg + tr * 128u + (((lane & 7) ^ (tr & 7)) << 4))
+                       : "memory");
+          if constexpr (EPI == kNsGram) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[it][j] *= p.alpha;
+          } else if constexpr (EPI == kNsPoly) {
+            const float2 f0 = unpack_half2(in[it].x), f1 = unpack_half2(in[it].y);
+            v[it][0] = fmaf(p.alpha, v[it][0], p.beta * f0.x);
+            v[it][1] = fmaf(p.alpha, v[it][1], p.beta * f0.y);
+            v[it][2] = fmaf(p.alpha, v[it][2], p.beta * f1.x);
+            v[it][3] = fmaf(p.alpha, v[it][3], p.beta * f1.y);
+          } else {
+            v[it][0] = fmaf(p.beta, __uint_as_float(in[it].x), v[it][0]);
+            v[it][1] = fmaf(p.beta, __uint_as_float(in[it].y), v[it][1]);
+            v[it][2] = fmaf(p.beta, __uint_as_float(in[it].z), v[it][2]);
+            v[it][3] = fmaf(p.beta, __uint_as_float(in[it].w), v[it][3]);
+          }
+        }
+        fetch(c + 1);
+        const int col = col0 + tcol;
         if constexpr (kSym) {
-          uint32_t w[16];
-          if constexpr (EPI == kNsPoly) {
-            // the padding of a row up to its pitch is readable, so groups of eight never leave the row
-            const __half* src = p.a16 + grow * p.pitch16 + col0;
+          if (ti != tj) {
+            // the other triangle: turned back, a row per lane, 32 lanes write 32 consecutive columns of row col0 + j
+            uint32_t w[32];
+            if constexpr (EPI == kNsPoly) {
+              __syncwarp();
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              U4 u{0u, 0u, 0u, 0u};
-              if (row_ok && v * 8 < width) u = ld_global_v4(src + v * 8);
-              const uint32_t in[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-              for (int h = 0; h < 4; ++h) {
-                const float2 f = unpack_half2(in[h]);
-                w[v * 4 + h] = pack_half2(fmaf(p.alpha, __uint_as_float(r[v * 8 + 2 * h]), p.beta * f.x),
-                                          fmaf(p.alpha, __uint_as_float(r[v * 8 + 2 * h + 1]), p.beta * f.y));
+              for (int it = 0; it < 8; ++it) {
+                const int tr = trow + it * 4;
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(stg + tr * 128u + (((lane & 7) ^ (tr & 7)) << 4)), "f"(v[it][0]),
+                             "f"(v[it][1]), "f"(v[it][2]), "f"(v[it][3])
+                             : "memory");
               }
+              __syncwarp();
+#pragma unroll
+              for (int f = 0; f < 8; ++f)
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[4 * f]), "=r"(w[4 * f + 1]), "=r"(w[4 * f + 2]), "=r"(w[4 * f + 3])
+                             : "r"(stg + lane * 128u + ((f ^ (lane & 7)) << 4))
+                             : "memory");
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(p.alpha * __uint_as_float(r[j]));
             }
-          } else {
+            if (lane < rows_here) {
+              __half* dst = p.out16 + ((long long)b * p.rows + col0) * p.pitch16 + row0 + lane;
 #pragma unroll
-            for (int h = 0; h < 16; ++h) w[h] = pack_half2(p.alpha * __uint_as_float(r[2 * h]), p.alpha * __uint_as_float(r[2 * h + 1]));
-          }
-          if (row_ok) {
-            __half* dst = p.out16 + grow * p.pitch16 + col0;
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (v * 8 < width) st_global_v4(dst + v * 8, U4{w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]});
-          }
-          if (ti != tj && row_ok) {
-            // the mirrored half: 32 lanes hold 32 consecutive columns of row col0 + j
-            __half* dst = p.out16 + ((long long)b * p.rows + col0) * p.pitch16 + row;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < width) {
-                const uint32_t h2 = w[j >> 1];
-                dst[(long long)j * p.pitch16] = __ushort_as_half((unsigned short)((j & 1) ? h2 >> 16 : h2 & 0xffffu));
-              }
-          }
-        } else if (row_ok) {
-          const float* mrow = p.master + grow * p.pitch_m + col0;
-          float v[32];
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            if (j < width8) {
-              const U4 u = ld_global_v4(mrow + j);
-              v[j] = fmaf(p.beta, __uint_as_float(u.x), __uint_as_float(r[j]));
-              v[j + 1] = fmaf(p.beta, __uint_as_float(u.y), __uint_as_float(r[j + 1]));
-              v[j + 2] = fmaf(p.beta, __uint_as_float(u.z), __uint_as_float(r[j + 2]));
-              v[j + 3] = fmaf(p.beta, __uint_as_float(u.w), __uint_as_float(r[j + 3]));
+              for (int j = 0; j < 32; ++j)
+                if (col0 + j < p.cols) dst[(long long)j * p.pitch16] = __float2half_rn(__uint_as_float(w[j]));
             }
           }
-          if constexpr (EPI == kNsUpdate) {
-            float* mdst = p.master + grow * p.pitch_m + col0;
-            __half* xdst = p.out16 + grow * p.pitch16 + col0;
+        }
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              if (j < width) {
-                st_global_v4(mdst + j, U4{__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3])});
-                st_global_v4(mdst + j + 4, U4{__float_as_uint(v[j + 4]), __float_as_uint(v[j + 5]), __float_as_uint(v[j + 6]), __float_as_uint(v[j + 7])});
-                st_global_v4(xdst + j, U4{pack_half2(v[j], v[j + 1]), pack_half2(v[j + 2], v[j + 3]), pack_half2(v[j + 4], v[j + 5]),
-                                          pack_half2(v[j + 6], v[j + 7])});
-              }
+        for (int it = 0; it < 8; ++it) {
+          const int tr = trow + it * 4;
+          if (col >= p.cols || tr >= rows_here) continue;
+          if constexpr (EPI == kNsUpdate)
+            st_global_v4(p.master + (grow + tr) * p.pitch_m + col,
+                         U4{__float_as_uint(v[it][0]), __float_as_uint(v[it][1]), __float_as_uint(v[it][2]), __float_as_uint(v[it][3])});
+          if constexpr (EPI == kNsUpdate || kSym)
+            *reinterpret_cast<uint2*>(p.out16 + (grow + tr) * p.pitch16 + col) = make_uint2(pack_half2(v[it][0], v[it][1]), pack_half2(v[it][2], v[it][3]));
+          if constexpr (EPI == kNsResult) {
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.final_out) + (grow + tr) * p.cols + col;
+            if (p.vec_out) {
+              *reinterpret_cast<uint2*>(dst) =
+                  make_uint2(pack_bf16x2(p.alpha * v[it][0], p.alpha * v[it][1]), pack_bf16x2(p.alpha * v[it][2], p.alpha * v[it][3]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (col + j < p.cols) dst[j] = __float2bfloat16_rn(p.alpha * v[it][j]);
             }
-          } else if constexpr (EPI == kNsResult) {
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.final_out) + grow * p.cols + col0;
+          }
+          if constexpr (EPI == kNsStep) {
+            float* dst = static_cast<float*>(p.final_out) + (grow + tr) * p.cols + col;
+            __nv_bfloat16* dst16 = p.p_bf16 != nullptr ? p.p_bf16 + (grow + tr) * p.cols + col : nullptr;
+            if (p.vec_out) {
+              const U4 u = ld_global_v4(dst);
+              const uint32_t old[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              if (j >= width) break;
-              if (p.vec_out) {
-                st_global_v4(dst + j, U4{pack_bf16x2(p.alpha * v[j], p.alpha * v[j + 1]), pack_bf16x2(p.alpha * v[j + 2], p.alpha * v[j + 3]),
-                                         pack_bf16x2(p.alpha * v[j + 4], p.alpha * v[j + 5]), pack_bf16x2(p.alpha * v[j + 6], p.alpha * v[j + 7])});
-              } else {
+              for (int j = 0; j < 4; ++j) v[it][j] = fmaf(-p.alpha, v[it][j], p.decay * __uint_as_float(old[j]));
+              st_global_v4(dst, U4{__float_as_uint(v[it][0]), __float_as_uint(v[it][1]), __float_as_uint(v[it][2]), __float_as_uint(v[it][3])});
+              if (dst16 != nullptr) *reinterpret_cast<uint2*>(dst16) = make_uint2(pack_bf16x2(v[it][0], v[it][1]), pack_bf16x2(v[it][2], v[it][3]));
+            } else {
 #pragma unroll
-                for (int i = j; i < j + 8; ++i)
-                  if (i < width) dst[i] = __float2bfloat16_rn(p.alpha * v[i]);
-              }
-            }
-          } else {
-            float* dst = static_cast<float*>(p.final_out) + grow * p.cols + col0;
-            __nv_bfloat16* dst16 = p.p_bf16 != nullptr ? p.p_bf16 + grow * p.cols + col0 : nullptr;
-#pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              if (j >= width) break;
-              if (p.vec_out) {
-                const U4 u0 = ld_global_v4(dst + j), u1 = ld_global_v4(dst + j + 4);
-                const uint32_t in[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[j + i] = fmaf(-p.alpha, v[j + i], p.decay * __uint_as_float(in[i]));
-                st_global_v4(dst + j, U4{__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3])});
-                st_global_v4(dst + j + 4, U4{__float_as_uint(v[j + 4]), __float_as_uint(v[j + 5]), __float_as_uint(v[j + 6]), __float_as_uint(v[j + 7])});
-                if (dst16 != nullptr)
-                  st_global_v4(dst16 + j, U4{pack_bf16x2(v[j], v[j + 1]), pack_bf16x2(v[j + 2], v[j + 3]), pack_bf16x2(v[j + 4], v[j + 5]),
-                                             pack_bf16x2(v[j + 6], v[j + 7])});
-              } else {
-#pragma unroll
-                for (int i = j; i < j + 8; ++i)
-                  if (i < width) {
-                    const float np = fmaf(-p.alpha, v[i], p.decay * dst[i]);
-                    dst[i] = np;
-                    if (dst16 != nullptr) dst16[i] = __float2bfloat16_rn(np);
-                  }
-              }
+              for (int j = 0; j < 4; ++j)
+                if (col + j < p.cols) {
+                  const float np = fmaf(-p.alpha, v[it][j], p.decay * dst[j]);
+                  dst[j] = np;
+                  if (dst16 != nullptr) dst16[j] = __float2bfloat16_rn(np);
+                }
             }
           }
         }
@@ -407,7 +437,7 @@ struct NsInput {
 };
 
 constexpr int kNsPrepThreads = 256;
-constexpr int kNsMaxParts = 256;
+constexpr int kNsMaxParts = 1024;
 
 __device__ __forceinline__ double block_sum_double(double v, double* red) {
 #pragma unroll
@@ -421,50 +451,74 @@ __device__ __forceinline__ double block_sum_double(double v, double* red) {
   return t;
 }
 
-__device__ __forceinline__ void load4(const NsInput& in, long long i, float (&g)[4]) {
+// eight gradient values from i on (16 or 32 bytes, aligned)
+__device__ __forceinline__ void load8(const NsInput& in, long long i, float (&g)[8]) {
   if (in.g_f32) {
-    const U4 u = ld_global_v4(static_cast<const float*>(in.g) + i);
-    g[0] = __uint_as_float(u.x); g[1] = __uint_as_float(u.y); g[2] = __uint_as_float(u.z); g[3] = __uint_as_float(u.w);
+    const U4 u = ld_global_nc_v4(static_cast<const float*>(in.g) + i), v = ld_global_nc_v4(static_cast<const float*>(in.g) + i + 4);
+    const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = __uint_as_float(w[j]);
   } else {
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(in.g) + i);
-    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
-    g[0] = a.x; g[1] = a.y; g[2] = b.x; g[3] = b.y;
+    const U4 u = ld_global_nc_v4(static_cast<const __nv_bfloat16*>(in.g) + i);
+    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
+    g[0] = a.x; g[1] = a.y; g[2] = b.x; g[3] = b.y; g[4] = c.x; g[5] = c.y; g[6] = d.x; g[7] = d.y;
   }
 }
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+  const U4 u = ld_global_v4(p), v = ld_global_v4(p + 4);
+  const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
+}
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+  st_global_v4(p, U4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])});
+  st_global_v4(p + 4, U4{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])});
+}
 
-// VEC4: every matrix is a multiple of four values and its tensors start on 16 bytes (bf16: 8)
-template <bool VEC4>
+// VEC: a matrix is a multiple of eight values and the tensors start on 16 bytes. Two accesses of eight values in flight per thread.
+template <bool VEC>
 __global__ void __launch_bounds__(kNsPrepThreads)
 ns_norm_kernel(const NsInput in, long long numel, double* __restrict__ part) {
   __shared__ double red[kNsPrepThreads / 32];
   const long long base = (long long)blockIdx.y * numel;
-  constexpr int W = VEC4 ? 4 : 1;
   double s = 0.0;
-  for (long long i = ((long long)blockIdx.x * kNsPrepThreads + threadIdx.x) * W; i < numel; i += (long long)gridDim.x * kNsPrepThreads * W) {
-    float g[W], u[W];
-    if constexpr (VEC4) load4(in, base + i, g);
-    else g[0] = in.grad(base + i);
-    if (in.m != nullptr) {
-      float m[W];
-      if constexpr (VEC4) {
-        const U4 v = ld_global_v4(in.m + base + i);
-        m[0] = __uint_as_float(v.x); m[1] = __uint_as_float(v.y); m[2] = __uint_as_float(v.z); m[3] = __uint_as_float(v.w);
-      } else {
-        m[0] = in.m[base + i];
+  if constexpr (VEC) {
+    const long long step = (long long)gridDim.x * kNsPrepThreads * 8;
+    for (long long i = ((long long)blockIdx.x * kNsPrepThreads + threadIdx.x) * 8; i < numel; i += 2 * step) {
+      float g[2][8], m[2][8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (i + h * step < numel) {
+          load8(in, base + i + h * step, g[h]);
+          if (in.m != nullptr) load8(in.m + base + i + h * step, m[h]);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        m[j] = fmaf(in.momentum, m[j], g[j]);
-        u[j] = in.use(g[j], m[j]);
-      }
-      if constexpr (VEC4) st_global_v4(in.m + base + i, U4{__float_as_uint(m[0]), __float_as_uint(m[1]), __float_as_uint(m[2]), __float_as_uint(m[3])});
-      else in.m[base + i] = m[0];
-    } else {
+      for (int h = 0; h < 2; ++h) {
+        if (i + h * step >= numel) break;
+        if (in.m != nullptr) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) u[j] = g[j];
+          for (int j = 0; j < 8; ++j) m[h][j] = fmaf(in.momentum, m[h][j], g[h][j]);
+          store8(in.m + base + i + h * step, m[h]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const double u = in.use(g[h][j], m[h][j]);
+          s += u * u;
+        }
+      }
     }
-#pragma unroll
-    for (int j = 0; j < W; ++j) s += (double)u[j] * (double)u[j];
+  } else {
+    for (long long i = (long long)blockIdx.x * kNsPrepThreads + threadIdx.x; i < numel; i += (long long)gridDim.x * kNsPrepThreads) {
+      const float g = in.grad(base + i);
+      float m = 0.f;
+      if (in.m != nullptr) {
+        m = fmaf(in.momentum, in.m[base + i], g);
+        in.m[base + i] = m;
+      }
+      const double u = in.use(g, m);
+      s += u * u;
+    }
   }
   s = block_sum_double(s, red);
   if (threadIdx.x == 0) part[(long long)blockIdx.y * gridDim.x + blockIdx.x] = s;
@@ -472,37 +526,36 @@ ns_norm_kernel(const NsInput in, long long numel, double* __restrict__ part) {
 
 // M = k u / (|u| + eps) and its fp16 copy, rows padded to their pitch with zeros
 __global__ void __launch_bounds__(kNsPrepThreads)
-ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* __restrict__ part, int parts, double eps, double k,
+ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* __restrict__ part, int parts, double eps, double k, int vec,
                 float* __restrict__ master, __half* __restrict__ x16) {
   __shared__ double red[kNsPrepThreads / 32];
   const long long b = blockIdx.y;
-  const double sum = block_sum_double((int)threadIdx.x < parts ? part[b * parts + threadIdx.x] : 0.0, red);
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kNsPrepThreads) sum += part[b * parts + i];
+  sum = block_sum_double(sum, red);
   const double inv = k / (sqrt(sum) + eps);
-  const int vecs = pitch / 4;
+  const int vecs = pitch / 8;
   const long long total = (long long)rows * vecs, base = b * rows * cols;
-  const bool vec4 = cols % 4 == 0 && (reinterpret_cast<uintptr_t>(in.g) & 15) == 0 && (reinterpret_cast<uintptr_t>(in.m) & 15) == 0;
   for (long long i = (long long)blockIdx.x * kNsPrepThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kNsPrepThreads) {
     const long long r = i / vecs;
-    const int c = (int)(i - r * vecs) * 4;
-    float u[4];
+    const int c = (int)(i - r * vecs) * 8;
+    float u[8];
     const long long at = base + r * cols + c;
-    if (vec4 && c < cols) {
-      float g[4];
-      load4(in, at, g);
-      U4 v{0u, 0u, 0u, 0u};
-      if (in.m != nullptr) v = ld_global_v4(in.m + at);
-      const uint32_t m[4] = {v.x, v.y, v.z, v.w};
+    if (vec) {
+      float g[8], m[8];
+      load8(in, at, g);
+      if (in.m != nullptr) load8(in.m + at, m);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = in.use(g[j], __uint_as_float(m[j]));
+      for (int j = 0; j < 8; ++j) u[j] = in.use(g[j], m[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = c + j < cols ? in.use(in.grad(at + j), in.m != nullptr ? in.m[at + j] : 0.f) : 0.f;
+      for (int j = 0; j < 8; ++j) u[j] = c + j < cols ? in.use(in.grad(at + j), in.m != nullptr ? in.m[at + j] : 0.f) : 0.f;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) u[j] = (float)((double)u[j] * inv);
+    for (int j = 0; j < 8; ++j) u[j] = (float)((double)u[j] * inv);
     const long long dst = (b * rows + r) * pitch + c;
-    st_global_v4(master + dst, U4{__float_as_uint(u[0]), __float_as_uint(u[1]), __float_as_uint(u[2]), __float_as_uint(u[3])});
-    *reinterpret_cast<uint2*>(x16 + dst) = make_uint2(pack_half2(u[0], u[1]), pack_half2(u[2], u[3]));
+    store8(master + dst, u);
+    st_global_v4(x16 + dst, U4{pack_half2(u[0], u[1]), pack_half2(u[2], u[3]), pack_half2(u[4], u[5]), pack_half2(u[6], u[7])});
   }
 }
 
@@ -515,7 +568,7 @@ int ns_gemm(const CUtensorMap& ta, const CUtensorMap& tb, NsParams p, cudaStream
   if (ctas > 2 * tiles) ctas = (int)(2 * tiles);
   auto kern = ns_gemm_kernel<A_MN, B_MN, EPI>;
   PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem));
-  kern<<<ctas, kGemmThreads, kNsSmem, s>>>(ta, tb, p);
+  kern<<<ctas, kNsThreads, kNsSmem, s>>>(ta, tb, p);
   PKB_CHECK_CUDA(cudaGetLastError());
   return kApiOk;
 }
@@ -576,7 +629,7 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
   double* part = reinterpret_cast<double*>(base + at.part);
 
   const NsInput in{g, g_f32, static_cast<float*>(m), momentum, nesterov};
-  const bool vec4 = numel % 4 == 0 && ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m)) & 15) == 0;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m)) & 15) == 0, vec = aligned && numel % 8 == 0;
   const long long most = ((long long)sm_count() * 8 + batch - 1) / batch;          // blocks per matrix that fill the GPU
   auto blocks_for = [&](long long items, long long cap) {
     long long n = (items + kNsPrepThreads - 1) / kNsPrepThreads;
@@ -584,12 +637,13 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
     if (n > cap) n = cap;
     return (int)(n < 1 ? 1 : n);
   };
-  const int parts = blocks_for(vec4 ? numel / 4 : numel, kNsMaxParts);
-  if (vec4) ns_norm_kernel<true><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
+  const int parts = blocks_for(vec ? numel / 16 : numel, kNsMaxParts);
+  if (vec) ns_norm_kernel<true><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
   else ns_norm_kernel<false><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
   PKB_CHECK_CUDA(cudaGetLastError());
-  const int start_blocks = blocks_for((long long)rows * (pitch / 4), 1 << 20);
-  ns_start_kernel<<<dim3((unsigned)start_blocks, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, rows, cols, (int)pitch, part, parts, eps, k, master, x[0]);
+  const int start_blocks = blocks_for((long long)rows * (pitch / 8), 1 << 20);
+  ns_start_kernel<<<dim3((unsigned)start_blocks, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, rows, cols, (int)pitch, part, parts, eps, k,
+                                                                                         aligned && cols % 8 == 0, master, x[0]);
   PKB_CHECK_CUDA(cudaGetLastError());
 
   // maps of X as an operand whose rows lie along K (boxes of 64 columns x 128 rows) and as one whose rows are K (64 x 64), and of A and B
@@ -608,7 +662,7 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
 
   NsParams q = {};
   q.batch = (int)batch;
-  q.vec_out = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(p_bf16)) & 15) == 0;
+  q.vec_out = cols % 4 == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(p_bf16)) & 15) == 0;
   q.status = status;
   q.wait_budget_ns = kDefaultWaitBudgetNs;
   for (int step = 0; step < steps; ++step) {
