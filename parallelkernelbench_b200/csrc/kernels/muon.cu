@@ -71,6 +71,12 @@ __device__ __forceinline__ void tma_load_3d_pair_p(uint32_t smem_dst, const CUte
       : "memory");
 }
 
+// The launches of a call depend on one another and are short where the matrices are: each one is launched while the one before it still
+// runs (programmatic dependent launch), sets up its barriers and tensor memory, and waits here until everything before it has finished and is
+// visible. Every thread waits before its first access to global memory.
+__device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_successor_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // the row of the triangle's t-th element (rows of 1, 2, 3, ... elements)
 __host__ __device__ inline int tri_row(int t) {
   int r = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
@@ -155,6 +161,8 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   cluster_sync_all();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_holder;
+  let_successor_launch();
+  wait_for_predecessor();
 
   if (warp == 0) {
     const uint32_t lead = elect_one() ? 1u : 0u;
@@ -481,6 +489,7 @@ __global__ void __launch_bounds__(kNsPrepThreads)
 ns_norm_kernel(const NsInput in, long long numel, double* __restrict__ part) {
   __shared__ double red[kNsPrepThreads / 32];
   const long long base = (long long)blockIdx.y * numel;
+  let_successor_launch();
   double s = 0.0;
   if constexpr (VEC) {
     const long long step = (long long)gridDim.x * kNsPrepThreads * 8;
@@ -530,6 +539,8 @@ ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* _
                 float* __restrict__ master, __half* __restrict__ x16) {
   __shared__ double red[kNsPrepThreads / 32];
   const long long b = blockIdx.y;
+  let_successor_launch();
+  wait_for_predecessor();
   double sum = 0.0;
   for (int i = threadIdx.x; i < parts; i += kNsPrepThreads) sum += part[b * parts + i];
   sum = block_sum_double(sum, red);
@@ -559,6 +570,21 @@ ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* _
   }
 }
 
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kern)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 template <bool A_MN, bool B_MN, int EPI>
 int ns_gemm(const CUtensorMap& ta, const CUtensorMap& tb, NsParams p, cudaStream_t s) {
   const long long num_m = (p.rows + kNsTile - 1) / kNsTile, num_n = (p.cols + kNsTile - 1) / kNsTile;
@@ -568,8 +594,7 @@ int ns_gemm(const CUtensorMap& ta, const CUtensorMap& tb, NsParams p, cudaStream
   if (ctas > 2 * tiles) ctas = (int)(2 * tiles);
   auto kern = ns_gemm_kernel<A_MN, B_MN, EPI>;
   PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem));
-  kern<<<ctas, kNsThreads, kNsSmem, s>>>(ta, tb, p);
-  PKB_CHECK_CUDA(cudaGetLastError());
+  PKB_CHECK_CUDA(launch_dependent(kern, dim3((unsigned)ctas), kNsThreads, kNsSmem, s, ta, tb, p));
   return kApiOk;
 }
 
@@ -642,9 +667,8 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
   else ns_norm_kernel<false><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
   PKB_CHECK_CUDA(cudaGetLastError());
   const int start_blocks = blocks_for((long long)rows * (pitch / 8), 1 << 20);
-  ns_start_kernel<<<dim3((unsigned)start_blocks, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, rows, cols, (int)pitch, part, parts, eps, k,
-                                                                                         aligned && cols % 8 == 0, master, x[0]);
-  PKB_CHECK_CUDA(cudaGetLastError());
+  PKB_CHECK_CUDA(launch_dependent(ns_start_kernel, dim3((unsigned)start_blocks, (unsigned)batch), kNsPrepThreads, 0, s, in, rows, cols, (int)pitch,
+                                  part, parts, eps, k, (int)(aligned && cols % 8 == 0), master, x[0]));
 
   // maps of X as an operand whose rows lie along K (boxes of 64 columns x 128 rows) and as one whose rows are K (64 x 64), and of A and B
   CUtensorMap xk[2], xm[2], ak, bk;
