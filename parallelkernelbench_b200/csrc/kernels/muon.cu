@@ -570,6 +570,369 @@ ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* _
   }
 }
 
+// ------------------------------------------------------------------------------------------------ a short side: one launch
+// Matrices whose smaller side is at most 128 stay on the chip for the whole call: a cluster owns a matrix, each of its CTAs a slice of
+// S <= 256 along the longer side. The iterate is in tensor memory in fp32, its fp16 copy in shared memory, where the same bytes serve the
+// Gram product (K-major, over the slice) and the update (MN-major, the slice as columns). Only the Gram matrix crosses CTAs: each adds its
+// rows' share of all partial sums, in the order of the CTAs, and hands the rounded rows to all (distributed shared memory); the polynomial is
+// computed by every CTA for itself. What bounds it is latency: five rounds of three short products with two cluster barriers each.
+constexpr int kSmallSide = 128;
+constexpr int kSmallSlice = 256;
+constexpr int kSmallCluster = 16;
+constexpr int kSmallThreads = 256;
+constexpr int kSmallX = kSmallSlice / 64 * 16384;              // X16: atoms of 64 columns, 128 rows of 128 bytes
+constexpr int kSmallGram = kSmallSide * kSmallSide * 4;        // partial Gram sums, fp32
+constexpr int kSmallA = kSmallSide * kSmallSide * 2;           // A and B, fp16
+constexpr int kSmallSmem = kSmallX + kSmallGram + 2 * kSmallA + 1024;
+static_assert(kSmallGram + 2 * kSmallA >= kSmallSide * kSmallSlice * 4, "u is staged where the Gram matrices come later");
+
+constexpr int kSmallMaxSteps = 16;
+
+struct NsSmallParams {
+  NsInput in;
+  long long matrix;          // values of one matrix
+  int side, longer, tall, slice, steps;
+  double eps, k;
+  float co[3 * kSmallMaxSteps];
+  int vec_in, vec_out;
+  void* out;                 // bf16 result, or null
+  float* p;
+  __nv_bfloat16* p_bf16;
+  float decay, scale;
+  uint32_t* status;
+  uint64_t wait_budget_ns;
+};
+
+// byte of value (row, col) in atoms of 64 columns with the 128-byte swizzle
+__device__ __forceinline__ uint32_t sw128_at(int row, int col) {
+  return (uint32_t)(col >> 6) * 16384u + (uint32_t)row * 128u + ((((uint32_t)(col & 63) >> 3) ^ ((uint32_t)row & 7u)) << 4) + ((uint32_t)col & 7u) * 2u;
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ U4 ld_shared_v4(uint32_t a) {
+  U4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+// eight values of row `row` from column `col` on (a multiple of eight) as fp16
+__device__ __forceinline__ void put8(uint32_t base, int row, int col, const float* v) {
+  st_shared_v4(base + sw128_at(row, col), pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]), pack_half2(v[6], v[7]));
+}
+
+__global__ void __launch_bounds__(kSmallThreads, 1)
+ns_small_kernel(const __grid_constant__ NsSmallParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ double red[kNsPrepThreads / 32];
+  __shared__ double norm_part;
+  __shared__ __align__(8) uint64_t bar_storage;
+  __shared__ uint32_t tmem_holder;
+  __shared__ int abort_storage;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t x16 = smem_base, gram = x16 + kSmallX, a16 = gram + kSmallGram, b16 = a16 + kSmallA;
+  float* u_stage = reinterpret_cast<float*>(smem_raw + (gram - smem_u32(smem_raw)));
+  volatile int* abort_flag = &abort_storage;
+  const uint32_t bar = smem_u32(&bar_storage);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ctas = p.longer > p.slice ? (int)cluster_nctaid() : 1;
+  const int rank = (int)cluster_ctarank();
+  const long long matrix = blockIdx.x / cluster_nctaid();
+  const int c0 = rank * p.slice;                                  // first column of the slice (along the longer side)
+  const int width = max(0, min(p.slice, p.longer - c0));
+  const long long base = matrix * p.matrix;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    mbar_init(bar, 1);
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&tmem_holder), 512);
+    tmem_relinquish();
+  }
+
+  // ---- u of this slice into shared memory (u_stage[c][r], columns of the staging swizzled so that neither side conflicts), its squares' sum
+  auto swz = [](int c) { return (c ^ (c >> 3)) & 31; };
+  double sum = 0.0;
+  auto take = [&](int r, int c, float g, float m) {
+    const float u = p.in.use(g, m);
+    u_stage[c * kSmallSide + (r ^ swz(c))] = u;
+    sum += (double)u * (double)u;
+  };
+  if (!p.tall && p.vec_in) {
+    const int per_row = (width + 7) / 8, items = p.side * per_row;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < items; i += kSmallThreads) {
+      const int r = i / per_row, c = (i - r * per_row) * 8;
+      const long long at = base + (long long)r * p.longer + c0 + c;
+      float g[8], m[8] = {};
+      load8(p.in, at, g);
+      if (p.in.m != nullptr) {
+        load8(p.in.m + at, m);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m[j] = fmaf(p.in.momentum, m[j], g[j]);
+        store8(p.in.m + at, m);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) take(r, c + j, g[j], m[j]);
+    }
+  } else {
+    // a row of the slice is contiguous where the matrix is tall (its columns are the side), else the columns of a row
+    const int inner = p.tall ? p.side : width, items = p.side * width;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < items; i += kSmallThreads) {
+      const int o = i / inner, w = i - o * inner;
+      const int r = p.tall ? w : o, c = p.tall ? o : w;
+      const long long at = base + (p.tall ? (long long)(c0 + c) * p.side + r : (long long)r * p.longer + c0 + c);
+      const float g = p.in.grad(at);
+      float m = 0.f;
+      if (p.in.m != nullptr) {
+        m = fmaf(p.in.momentum, p.in.m[at], g);
+        p.in.m[at] = m;
+      }
+      take(r, c, g, m);
+    }
+  }
+  sum = block_sum_double(sum, red);
+  if (ctas > 1) {
+    if (threadIdx.x == 0) norm_part = sum;
+    cluster_sync_all();
+    sum = 0.0;
+    for (int c = 0; c < ctas; ++c) {
+      double v;
+      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(mapa_shared(smem_u32(&norm_part), (uint32_t)c)) : "memory");
+      sum += v;
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const double inv = p.k / (sqrt(sum) + p.eps);
+  const uint32_t tmem = tmem_holder, tm_acc = tmem + 256;
+  // a warp's place in tensor memory: 32 rows, and half of the columns of what it walks
+  const int q = warp & 3, half = warp >> 2, row = q * 32 + lane;
+  const uint32_t lanes = (uint32_t)(q * 32) << 16;
+  const int cols_half = p.slice / 2;
+  for (int c = half * cols_half; c < (half + 1) * cols_half; c += 32) {
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const bool in = row < p.side && c + j < width;
+      v[j] = in ? (float)((double)u_stage[(c + j) * kSmallSide + (row ^ swz(c + j))] * inv) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) put8(x16, row, c + j, v + j);
+    uint32_t w[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(v[j]);
+    tmem_st_32x32(tmem + lanes + c, w);
+  }
+  tmem_st_wait();
+  fence_proxy_async_smem();
+  tc_fence_before_sync();
+  __syncthreads();
+
+  uint32_t phase = 0;
+  bool ok = true;
+  auto wait_products = [&](int site) {
+    if (ok && !mbar_wait(bar, phase, abort_flag, p.wait_budget_ns)) {
+      if (threadIdx.x == 0) record_status(p.status, kStatusMbarTimeout, kNsKernelId + 1, 0, 0, site, (uint32_t)matrix);
+      ok = false;
+    }
+    phase ^= 1u;
+    __syncwarp();
+    tc_fence_after_sync();
+  };
+  const float alpha = (float)(1.0 / (p.k * p.k));
+  constexpr uint32_t kSquare = make_idesc(kSmallSide, kSmallSide, 0, 0, 0, 0);
+  const uint32_t idesc_update = make_idesc(kSmallSide, (uint32_t)p.slice, 0, 0, 0, 1);
+#pragma unroll 1
+  for (int step = 0; step < p.steps; ++step) {
+    const float a = p.co[3 * step], b = p.co[3 * step + 1], cc = p.co[3 * step + 2];
+    // ---- the slice's share of X X^T
+    if (warp == 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      tc_fence_after_sync();
+      for (int kk = 0; kk < p.slice / 16; ++kk) {
+        const uint32_t lo = smem_desc_lo_kmajor(x16 + (kk >> 2) * 16384u) + (kk & 3) * 2u;
+        umma_f16_ss_p(tm_acc, smem_desc_join(lo), smem_desc_join(lo), kSquare, kk != 0 ? 1u : 0u, lead);
+      }
+      umma_commit_p(bar, lead);
+    }
+    wait_products(1);
+#pragma unroll 1
+    for (int c = half * 64; c < half * 64 + 64; c += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32(tm_acc + lanes + c, r);
+      tmem_ld_wait();
+      if (ctas > 1) {
+#pragma unroll
+        for (int f = 0; f < 8; ++f)
+          st_shared_v4(gram + row * 512u + ((((uint32_t)(c >> 2) + f) ^ (row & 7)) << 4), r[4 * f], r[4 * f + 1], r[4 * f + 2], r[4 * f + 3]);
+      } else {
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = alpha * __uint_as_float(r[j]);
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) put8(a16, row, c + j, v + j);
+      }
+    }
+    if (ctas > 1) {
+      cluster_sync_all();
+      // this CTA's share of the rows: four columns per thread, from every CTA, to every CTA
+      for (int i = (int)threadIdx.x; i < 4096 / ctas; i += kSmallThreads) {
+        const int r = rank * (kSmallSide / ctas) + (i >> 5), f = i & 31;
+        const uint32_t src = gram + r * 512u + ((uint32_t)(f ^ (r & 7)) << 4);
+        float4 part[kSmallCluster];
+#pragma unroll
+        for (int c = 0; c < kSmallCluster; ++c)
+          if (c < ctas) part[c] = ld_shared_cluster_v4(mapa_shared(src, (uint32_t)c));
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < kSmallCluster; ++c) {
+          if (c < ctas) {
+            t.x += part[c].x; t.y += part[c].y; t.z += part[c].z; t.w += part[c].w;
+          }
+        }
+        const uint32_t lo = pack_half2(alpha * t.x, alpha * t.y), hi = pack_half2(alpha * t.z, alpha * t.w);
+        const uint32_t dst = a16 + sw128_at(r, f * 4);
+        for (int c = 0; c < ctas; ++c)
+          asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(mapa_shared(dst, (uint32_t)c)), "r"(lo), "r"(hi) : "memory");
+      }
+      fence_proxy_async_all();
+      tc_fence_before_sync();
+      cluster_sync_all();
+    } else {
+      fence_proxy_async_smem();
+      tc_fence_before_sync();
+      __syncthreads();
+    }
+    // ---- A A, and B = b A + c A A
+    if (warp == 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      fence_proxy_async_all();
+      tc_fence_after_sync();
+#pragma unroll
+      for (int kk = 0; kk < kSmallSide / 16; ++kk) {
+        const uint32_t lo = smem_desc_lo_kmajor(a16 + (kk >> 2) * 16384u) + (kk & 3) * 2u;
+        umma_f16_ss_p(tm_acc, smem_desc_join(lo), smem_desc_join(lo), kSquare, kk != 0 ? 1u : 0u, lead);
+      }
+      umma_commit_p(bar, lead);
+    }
+    wait_products(2);
+#pragma unroll 1
+    for (int c = half * 64; c < half * 64 + 64; c += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32(tm_acc + lanes + c, r);
+      tmem_ld_wait();
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 32; j += 8) {
+        const U4 u = ld_shared_v4(a16 + sw128_at(row, c + j));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const float2 f = unpack_half2(w[h]);
+          v[j + 2 * h] = fmaf(cc, __uint_as_float(r[j + 2 * h]), b * f.x);
+          v[j + 2 * h + 1] = fmaf(cc, __uint_as_float(r[j + 2 * h + 1]), b * f.y);
+        }
+        put8(b16, row, c + j, v + j);
+      }
+    }
+    fence_proxy_async_smem();
+    tc_fence_before_sync();
+    __syncthreads();
+    // ---- X <- a X + B X
+    if (warp == 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      tc_fence_after_sync();
+#pragma unroll
+      for (int kk = 0; kk < kSmallSide / 16; ++kk) {
+        const uint32_t alo = smem_desc_lo_kmajor(b16 + (kk >> 2) * 16384u) + (kk & 3) * 2u;
+        const uint32_t blo = smem_desc_lo_mnmajor(x16, 16384u) + kk * 128u;
+        umma_f16_ss_p(tm_acc, smem_desc_join(alo), smem_desc_join(blo), idesc_update, kk != 0 ? 1u : 0u, lead);
+      }
+      umma_commit_p(bar, lead);
+    }
+    wait_products(3);
+    const bool last = step + 1 == p.steps;
+#pragma unroll 1
+    for (int c = half * cols_half; c < (half + 1) * cols_half; c += 32) {
+      uint32_t r[32], m[32];
+      tmem_ld_32x32(tm_acc + lanes + c, r);
+      tmem_ld_32x32(tmem + lanes + c, m);
+      tmem_ld_wait();
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = fmaf(a, __uint_as_float(m[j]), __uint_as_float(r[j]));
+      if (!last) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) m[j] = __float_as_uint(v[j]);
+        tmem_st_32x32(tmem + lanes + c, m);
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) put8(x16, row, c + j, v + j);
+      } else if (row < p.side) {
+        const long long stride = p.tall ? p.side : 1;
+        const long long at = base + (p.tall ? (long long)(c0 + c) * p.side + row : (long long)row * p.longer + c0 + c);
+        if (p.out != nullptr) {
+          __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + at;
+          if (p.vec_out) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              if (c + j < width)
+                st_global_v4(dst + j, U4{pack_bf16x2(p.scale * v[j], p.scale * v[j + 1]), pack_bf16x2(p.scale * v[j + 2], p.scale * v[j + 3]),
+                                         pack_bf16x2(p.scale * v[j + 4], p.scale * v[j + 5]), pack_bf16x2(p.scale * v[j + 6], p.scale * v[j + 7])});
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j < width) dst[j * stride] = __float2bfloat16_rn(p.scale * v[j]);
+          }
+        } else if (p.vec_out) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            if (c + j < width) {
+              float o[8];
+              load8(p.p + at + j, o);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o[i] = fmaf(-p.scale, v[j + i], p.decay * o[i]);
+              store8(p.p + at + j, o);
+              if (p.p_bf16 != nullptr)
+                st_global_v4(p.p_bf16 + at + j, U4{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7])});
+            }
+          }
+        } else {
+          float o[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < width) o[j] = p.p[at + j * stride];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (c + j < width) {
+              const float np = fmaf(-p.scale, v[j], p.decay * o[j]);
+              p.p[at + j * stride] = np;
+              if (p.p_bf16 != nullptr) p.p_bf16[at + j * stride] = __float2bfloat16_rn(np);
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+    tmem_st_wait();
+    fence_proxy_async_smem();
+    tc_fence_before_sync();
+    __syncthreads();
+  }
+  if (*abort_flag) {      // products in flight end before their memory goes away
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 template <typename... Params, typename... Args>
 cudaError_t launch_dependent(void (*kern)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
   cudaLaunchConfig_t cfg = {};
@@ -598,6 +961,35 @@ int ns_gemm(const CUtensorMap& ta, const CUtensorMap& tb, NsParams p, cudaStream
   return kApiOk;
 }
 
+// CTAs per matrix: as few as hold it, then more (down to slices of 64) while all matrices together leave SMs idle. A cluster stays inside a
+// group of 16 to 20 SMs, so seven or more clusters of 16 are resident at once.
+int small_cluster(long long batch, int longer) {
+  int c = 1;
+  while (c * kSmallSlice < longer) c *= 2;
+  while (c < kSmallCluster && c * 64 < longer && batch * c * 2 <= 112) c *= 2;
+  return c;
+}
+
+bool small_fits(int side, int longer, int steps) { return side <= kSmallSide && longer <= kSmallCluster * kSmallSlice && steps <= kSmallMaxSteps; }
+
+int launch_small(const NsSmallParams& p, int cluster, long long batch, cudaStream_t s) {
+  PKB_CHECK_CUDA(cudaFuncSetAttribute(ns_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallSmem));
+  PKB_CHECK_CUDA(cudaFuncSetAttribute(ns_small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(batch * cluster));
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.dynamicSmemBytes = kSmallSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, ns_small_kernel, p));
+  return kApiOk;
+}
+
 long long pad8(long long n) { return (n + 7) / 8 * 8; }
 long long pad256(long long n) { return (n + 255) / 256 * 256; }
 
@@ -622,8 +1014,12 @@ struct NsScratch {
 
 using namespace pkb;
 
-extern "C" long long pkb_newton_schulz_scratch(long long batch, int rows, int cols) {
-  return batch > 0 && rows > 0 && cols > 0 ? NsScratch(batch, rows, cols).total : 0;
+// bytes of scratch that pkb_newton_schulz wants (0: none) and, in *launches, the kernels that it launches
+extern "C" long long pkb_newton_schulz_scratch(long long batch, int rows, int cols, int steps, int* launches) {
+  if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+  const bool small = small_fits(rows < cols ? rows : cols, rows < cols ? cols : rows, steps);
+  if (launches != nullptr) *launches = small ? 1 : 2 + 3 * steps;
+  return small ? 0 : NsScratch(batch, rows, cols).total;
 }
 
 // Orthogonalises `batch` matrices [rows, cols] u (see NsInput: g bf16 or fp32, with the momentum m fp32 updated in place where it is not null).
@@ -634,27 +1030,52 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
                                  void* scratch, void* stream) {
   PKB_CHECK_ARG(batch > 0 && batch <= 65535 && rows > 0 && cols > 0, "1 .. 65535 matrices of at least one row and column");
   PKB_CHECK_ARG(steps >= 1 && coeff != nullptr, "at least one step");
-  PKB_CHECK_ARG(g != nullptr && scratch != nullptr && ((out != nullptr) != (p != nullptr)), "g, scratch and one of out and p");
-  PKB_CHECK_ARG((reinterpret_cast<uintptr_t>(scratch) & 255) == 0, "scratch must start on 256 bytes");
+  PKB_CHECK_ARG(g != nullptr && ((out != nullptr) != (p != nullptr)), "g, scratch and one of out and p");
   // the first call on a device allocates its status block: let that happen inside a graph capture, too
   cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
   PKB_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
   uint32_t* status = status_block_device_ptr();
   PKB_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const NsScratch at(batch, rows, cols);
-  uint8_t* base = static_cast<uint8_t*>(scratch);
   const bool tall = rows > cols;
   const int side = tall ? cols : rows, longer = tall ? rows : cols;
   const long long pitch = pad8(cols), pitch_a = pad8(side), numel = (long long)rows * cols;
   const double k = ldexp(1.0, (int)lrint(log2((double)longer) / 2));
+  const NsInput in{g, g_f32, static_cast<float*>(m), momentum, nesterov};
+  const bool aligned_out = ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(p_bf16)) & 15) == 0;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m)) & 15) == 0, vec = aligned && numel % 8 == 0;
+  if (small_fits(side, longer, steps)) {
+    NsSmallParams q = {};
+    q.in = in;
+    q.matrix = numel;
+    q.side = side;
+    q.longer = longer;
+    q.tall = tall;
+    const int cluster = small_cluster(batch, longer);
+    q.slice = ((longer + cluster - 1) / cluster + 63) / 64 * 64;
+    q.steps = steps;
+    q.eps = eps;
+    q.k = k;
+    for (int i = 0; i < 3 * steps; ++i) q.co[i] = coeff[i];
+    q.vec_in = aligned && cols % 8 == 0;
+    q.vec_out = !tall && aligned_out && cols % 8 == 0;
+    q.out = out;
+    q.p = static_cast<float*>(p);
+    q.p_bf16 = static_cast<__nv_bfloat16*>(p_bf16);
+    q.decay = decay;
+    q.scale = (float)((p == nullptr ? 1.0 : (double)scale) / k);
+    q.status = status;
+    q.wait_budget_ns = kDefaultWaitBudgetNs;
+    return launch_small(q, cluster, batch, s);
+  }
+
+  PKB_CHECK_ARG(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 255) == 0, "scratch must start on 256 bytes");
+  const NsScratch at(batch, rows, cols);
+  uint8_t* base = static_cast<uint8_t*>(scratch);
   float* master = reinterpret_cast<float*>(base + at.master);
   __half *x[2] = {reinterpret_cast<__half*>(base + at.x0), reinterpret_cast<__half*>(base + at.x1)};
   __half *a16 = reinterpret_cast<__half*>(base + at.a), *b16 = reinterpret_cast<__half*>(base + at.b);
   double* part = reinterpret_cast<double*>(base + at.part);
-
-  const NsInput in{g, g_f32, static_cast<float*>(m), momentum, nesterov};
-  const bool aligned = ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m)) & 15) == 0, vec = aligned && numel % 8 == 0;
   const long long most = ((long long)sm_count() * 8 + batch - 1) / batch;          // blocks per matrix that fill the GPU
   auto blocks_for = [&](long long items, long long cap) {
     long long n = (items + kNsPrepThreads - 1) / kNsPrepThreads;
@@ -686,7 +1107,7 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
 
   NsParams q = {};
   q.batch = (int)batch;
-  q.vec_out = cols % 4 == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(p_bf16)) & 15) == 0;
+  q.vec_out = cols % 4 == 0 && aligned_out;
   q.status = status;
   q.wait_budget_ns = kDefaultWaitBudgetNs;
   for (int step = 0; step < steps; ++step) {

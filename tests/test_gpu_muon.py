@@ -63,8 +63,10 @@ def _check(out, u, **kw):
     return diff / max(want.norm().item(), 1e-30)
 
 
-# one value, rows and columns of one, the edges of tiles (256) and of a CTA's half (128), odd sides, wide and tall, a long inner extent
-SHAPES = [(1, 1), (1, 5), (5, 1), (7, 3), (16, 16), (3, 2000), (64, 2048), (2048, 40), (128, 128), (129, 127), (256, 256), (257, 255), (333, 1000), (1000, 333),
+# one value, rows and columns of one, slices of the one-launch form (a side of up to 128, the longer up to 4096) that end anywhere, the first
+# sizes beyond it, the edges of tiles (256) and of a CTA's half (128), odd sides, wide and tall, a long inner extent
+SHAPES = [(1, 1), (1, 5), (5, 1), (7, 3), (16, 16), (3, 2000), (64, 2048), (2048, 40), (128, 128), (129, 127), (33, 65), (128, 4096), (3001, 96), (70, 4097),
+          (4100, 128), (129, 300), (256, 256), (257, 255), (333, 1000), (1000, 333),
           (512, 1024), (640, 512), (1025, 513)]
 
 
@@ -107,6 +109,25 @@ def test_batches_are_matrices_of_their_own(shape):
         else:
             assert torch.equal(out[i], newton_schulz(flat[i]))
     assert torch.equal(out[1], torch.zeros_like(out[1]))
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(7, 64, 512), (40, 100, 72), (70, 12, 1000), (3, 1500, 90)])
+def test_many_small_matrices(batch, rows, cols):
+    """However many CTAs share a matrix, and whether or not all matrices are resident at once."""
+    from parallelkernelbench_b200.ops import newton_schulz
+
+    u = _matrix((batch, rows, cols), "noise").to(torch.bfloat16)
+    out = newton_schulz(u)
+    for i in (0, 1, batch // 2, batch - 1):
+        _check(out[i], u[i])
+
+
+def test_more_steps_than_one_launch_takes():
+    from parallelkernelbench_b200.ops import newton_schulz
+
+    u = _matrix((24, 40), "noise")
+    for steps in (16, 17):
+        _check(newton_schulz(u, steps=steps, coefficients=CUBIC), u, steps=steps, coefficients=CUBIC)
 
 
 @pytest.mark.parametrize("factor", [1e-30, 1e-12, 1e25])
