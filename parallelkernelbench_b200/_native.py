@@ -133,13 +133,20 @@ def bound(name: str, argtypes: list, restype=ctypes.c_int):
     return f
 
 
-def on_device(t):
-    """Context in which the device of ``t`` is the current one: launches go to the device of their tensors."""
-    import contextlib
-
+def launch(name: str, argtypes: list, t, *args, launches: int = 1) -> None:
+    """Call the entry point ``name`` with ``args`` and, last, the current stream of the device of ``t``, with that device as the current one."""
     import torch
 
-    return contextlib.nullcontext() if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+    f = _bound.get(name) or bound(name, argtypes)
+    device = t.device.index
+    if device == torch._C._cuda_getDevice():
+        rc = f(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = f(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        check(rc, name)
+    count_launch(launches)
 
 
 def same_cuda_device(first, **tensors) -> None:

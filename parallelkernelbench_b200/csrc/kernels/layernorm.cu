@@ -5,6 +5,7 @@
 // A row belongs to a team of TPR threads that holds VEC * CH of its values each: 16-byte accesses where base, row pitch and width
 // allow them (VEC = 8 bf16 or 4 fp32), single values otherwise. All sums are fp32.
 #include "pkb/api.h"
+#include "pkb/bulk_copy.cuh"
 #include "pkb/host.h"
 #include "pkb/ptx.cuh"
 
@@ -308,23 +309,276 @@ ln_bwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ dy, 
   }
 }
 
-// dgamma, dbeta [2][cols] = sum over the blocks of part[block][2][cols]: 32 columns and 8 strands of blocks per thread block
-__global__ void __launch_bounds__(256)
+// ---- many wide rows: a ring of rows in shared memory --------------------------------------------
+// A block of NT threads walks its rows with the next ones already on their way: thread 0 keeps bulk copies of up to kLnStages rows in flight
+// (192 KB per SM over all blocks), so the memory system does not wait for a row's sums. With the loads in registers and one row ahead,
+// 8192 x 4096 bf16 took 36 us forward and 59 backward, 16384 x 8192 took 142 and 237. A stage is free again once the block has passed the
+// first barrier of its row: by then every thread holds its part in registers.
+constexpr int kLnStages = 8;
+constexpr int kLnRingBytes = 192 * 1024;                  // per SM
+constexpr uint32_t kLnKernelId = 112;
+
+struct LnRing {
+  uint32_t base, bars, stage_bytes;
+  int stages;
+};
+
+// 16 bytes as VEC fp32 values
+template <int VEC>
+__device__ __forceinline__ void ln_unpack(const U4& u, float (&f)[VEC]) {
+  if constexpr (VEC == 8) {
+    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+  } else {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  }
+}
+__device__ __forceinline__ U4 ln_shared(uint32_t a) {
+  U4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ LnRing ln_ring_init(uint8_t* smem, int stages, uint32_t stage_bytes, int* abort_flag) {
+  const LnRing r{smem_u32(smem) + 128, smem_u32(smem), stage_bytes, stages};
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < stages; ++i) mbar_init(r.bars + 8 * i, 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  return r;
+}
+
+// false once a row did not come within the budget: the caller leaves, after what is in flight
+__device__ __forceinline__ bool ln_ring_wait(const LnRing& r, int stage, uint32_t parity, volatile int* abort_flag, uint32_t* status, long long row) {
+  if (mbar_wait(r.bars + 8 * stage, parity, abort_flag)) return true;
+  if (threadIdx.x == 0) record_status(status, kStatusMbarTimeout, kLnKernelId, 0, stage, 1, (uint32_t)row);
+  return false;
+}
+__device__ __forceinline__ void ln_ring_abandon() {
+  const uint64_t t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+}
+
+// PER: values per thread; with 16 the gain and bias are held in registers, with 32 they are read again for every row. (Read for every row, from
+// an L1 that the ring leaves little of, fp32 gains are twice the traffic of the rows: 8192 x 4096 took 40 us.)
+template <typename T, int NT, int PER>
+__global__ void __launch_bounds__(NT, 512 / NT)
+ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, const LnParam beta, T* __restrict__ y,
+                   float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, int cols, float eps, int stages, uint32_t* status) {
+  constexpr int VEC = 16 / sizeof(T), CH = PER / VEC;
+  constexpr bool kHoldGain = PER <= 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float red[2][NT / 32];
+  __shared__ int abort_flag;
+  const uint32_t bytes = (uint32_t)cols * sizeof(T);
+  const LnRing ring = ln_ring_init(smem, stages, bytes, &abort_flag);
+  const int t = threadIdx.x;
+  const float inv = 1.f / (float)cols;
+  auto issue = [&](long long row, int stage) {
+    mbar_expect_tx(ring.bars + 8 * stage, bytes);
+    bulk_load(ring.base + stage * bytes, x + row * ldx, bytes, ring.bars + 8 * stage);
+  };
+  if (t == 0)
+    for (int i = 0; i < stages; ++i)
+      if (blockIdx.x + (long long)i * gridDim.x < rows) issue(blockIdx.x + (long long)i * gridDim.x, i);
+  float g[kHoldGain ? CH : 1][VEC], b[kHoldGain ? CH : 1][VEC];
+  if constexpr (kHoldGain) {
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      const int c = (ch * NT + t) * VEC;
+      if (c < cols) {
+        gamma.template load<VEC>(c, g[ch]);
+        beta.template load<VEC>(c, b[ch]);
+      }
+    }
+  }
+  int stage = 0;
+  uint32_t parity = 0;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    if (!ln_ring_wait(ring, stage, parity, &abort_flag, status, row)) {
+      ln_ring_abandon();
+      return;
+    }
+    float v[CH][VEC];
+    float s[1] = {0.f}, q[1] = {0.f};
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      const int c = (ch * NT + t) * VEC;
+      if (c < cols) {
+        ln_unpack<VEC>(ln_shared(ring.base + stage * bytes + c * (int)sizeof(T)), v[ch]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s[0] += v[ch][j];
+      }
+    }
+    team_sum<1, NT, NT>(s, red[0], 0);
+    if (t == 0 && row + (long long)stages * gridDim.x < rows) {
+      fence_proxy_async_smem();
+      issue(row + (long long)stages * gridDim.x, stage);
+    }
+    const float mean = s[0] * inv;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      if ((ch * NT + t) * VEC < cols) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) q[0] += (v[ch][j] - mean) * (v[ch][j] - mean);
+      }
+    }
+    team_sum<1, NT, NT>(q, red[1], 0);
+    const float rstd = rsqrtf(q[0] * inv + eps);
+    if (t == 0 && mean_out != nullptr) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      const int c = (ch * NT + t) * VEC;
+      if (c < cols) {
+        constexpr int kAt = kHoldGain ? 1 : 0;
+        if constexpr (!kHoldGain) {
+          gamma.template load<VEC>(c, g[0]);
+          beta.template load<VEC>(c, b[0]);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[ch][j] = (v[ch][j] - mean) * rstd * g[kAt * ch][j] + b[kAt * ch][j];
+        ln_store<T, VEC>(y + row * cols + c, v[ch]);
+      }
+    }
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+}
+
+// A stage holds a row of x and the same row of dy. PER: values per thread; with 32 the gain is read again for every row (16 KB from L1 and
+// L2) instead of being held in registers.
+template <typename T, int NT, int PER>
+__global__ void __launch_bounds__(NT, 512 / NT)
+ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ dy, long long lddy, const LnParam gamma,
+                   const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part,
+                   long long rows, int cols, int stages, uint32_t* status) {
+  constexpr int VEC = 16 / sizeof(T), CH = PER / VEC;
+  constexpr bool kHoldGain = PER <= 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float red[2][2 * (NT / 32)];
+  __shared__ int abort_flag;
+  const uint32_t bytes = (uint32_t)cols * sizeof(T);
+  const LnRing ring = ln_ring_init(smem, stages, 2 * bytes, &abort_flag);
+  const int t = threadIdx.x;
+  const float inv = 1.f / (float)cols;
+  auto issue = [&](long long row, int stage) {
+    const uint32_t dst = ring.base + stage * 2 * bytes, bar = ring.bars + 8 * stage;
+    mbar_expect_tx(bar, 2 * bytes);
+    bulk_load(dst, x + row * ldx, bytes, bar);
+    bulk_load(dst + bytes, dy + row * lddy, bytes, bar);
+  };
+  if (t == 0)
+    for (int i = 0; i < stages; ++i)
+      if (blockIdx.x + (long long)i * gridDim.x < rows) issue(blockIdx.x + (long long)i * gridDim.x, i);
+  float ag[CH][VEC] = {}, ab[CH][VEC] = {};
+  float g[kHoldGain ? CH : 1][VEC];
+  if constexpr (kHoldGain) {
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      const int c = (ch * NT + t) * VEC;
+      if (c < cols) gamma.template load<VEC>(c, g[ch]);
+    }
+  }
+  int stage = 0, it = 0;
+  uint32_t parity = 0;
+  float mean_n = blockIdx.x < rows ? mean_in[blockIdx.x] : 0.f, rstd_n = blockIdx.x < rows ? rstd_in[blockIdx.x] : 0.f;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x, it ^= 1) {
+    const float mean = mean_n, rstd = rstd_n;
+    if (row + gridDim.x < rows) {        // the next row's, a row ahead of their use
+      mean_n = mean_in[row + gridDim.x];
+      rstd_n = rstd_in[row + gridDim.x];
+    }
+    if (!ln_ring_wait(ring, stage, parity, &abort_flag, status, row)) {
+      ln_ring_abandon();
+      return;
+    }
+    U4 xr[CH], dr[CH];
+    float s[2] = {0.f, 0.f};
+    const uint32_t at = ring.base + stage * 2 * bytes;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      const int c = (ch * NT + t) * VEC;
+      if (c < cols) {
+        xr[ch] = ln_shared(at + c * (int)sizeof(T));
+        dr[ch] = ln_shared(at + bytes + c * (int)sizeof(T));
+        float xv[VEC], dv[VEC];
+        ln_unpack<VEC>(xr[ch], xv);
+        ln_unpack<VEC>(dr[ch], dv);
+        if constexpr (!kHoldGain) gamma.template load<VEC>(c, g[0]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float xh = (xv[j] - mean) * rstd, gd = dv[j] * g[kHoldGain ? ch : 0][j];
+          ag[ch][j] += dv[j] * xh;
+          ab[ch][j] += dv[j];
+          s[0] += gd;
+          s[1] += gd * xh;
+        }
+      }
+    }
+    team_sum<2, NT, NT>(s, red[it], 0);
+    if (t == 0 && row + (long long)stages * gridDim.x < rows) {
+      fence_proxy_async_smem();
+      issue(row + (long long)stages * gridDim.x, stage);
+    }
+    const float c1 = s[0] * inv, c2 = s[1] * inv;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      const int c = (ch * NT + t) * VEC;
+      if (c < cols) {
+        float xv[VEC], dv[VEC];
+        ln_unpack<VEC>(xr[ch], xv);
+        ln_unpack<VEC>(dr[ch], dv);
+        if constexpr (!kHoldGain) gamma.template load<VEC>(c, g[0]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) dv[j] = rstd * (dv[j] * g[kHoldGain ? ch : 0][j] - c1 - (xv[j] - mean) * rstd * c2);
+        ln_store<T, VEC>(dx + row * cols + c, dv);
+      }
+    }
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+  float* out = part + (long long)blockIdx.x * 2 * cols;
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch) {
+    const int c = (ch * NT + t) * VEC;
+    if (c < cols) {
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4) {
+        st_global_v4(out + c + j, U4{__float_as_uint(ag[ch][j]), __float_as_uint(ag[ch][j + 1]), __float_as_uint(ag[ch][j + 2]), __float_as_uint(ag[ch][j + 3])});
+        st_global_v4(out + cols + c + j,
+                     U4{__float_as_uint(ab[ch][j]), __float_as_uint(ab[ch][j + 1]), __float_as_uint(ab[ch][j + 2]), __float_as_uint(ab[ch][j + 3])});
+      }
+    }
+  }
+}
+
+// dgamma, dbeta [2][cols] = sum over the blocks of part[block][2][cols]: 32 columns and 32 strands of blocks per thread block
+__global__ void __launch_bounds__(1024)
 ln_bwd_params_kernel(const float* __restrict__ part, int blocks, long long width, float* __restrict__ dgamma, float* __restrict__ dbeta, int cols) {
-  __shared__ float s[8][33];
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5;
   const long long i = (long long)blockIdx.x * 32 + lane;
   float a = 0.f;
-  if (i < width)
-    for (int b = strand; b < blocks; b += 8) a += part[b * width + i];
+  if (i < width) {
+#pragma unroll 8
+    for (int b = strand; b < blocks; b += 32) a += part[b * width + i];
+  }
   s[strand][lane] = a;
   __syncthreads();
-  if (strand == 0 && i < width) {
-    a = s[0][lane];
-#pragma unroll
-    for (int k = 1; k < 8; ++k) a += s[k][lane];
-    if (i < cols) dgamma[i] = a;
-    else dbeta[i - cols] = a;
+  a = warp_sum(s[lane][strand]);           // warp w adds the strands of column w
+  const long long o = (long long)blockIdx.x * 32 + strand;
+  if (lane == 0 && o < width) {
+    if (o < cols) dgamma[o] = a;
+    else dbeta[o - cols] = a;
   }
 }
 
@@ -412,18 +666,71 @@ int ln_fwd_team(const T* x, long long ldx, LnParam g, LnParam b, T* y, float* me
   return ln_by_width<decltype(go)&, T, VEC>(cols, go);
 }
 
+// The ring takes over from 1025 columns on (a warp per row, as below, has enough rows in flight) where every block has more than two rows; its
+// rows must be whole multiples of 16 bytes, start on 16 bytes and fit 16384 columns (backward in fp32: 8192).
+struct LnRingPlan {
+  int threads, per, blocks, stages, smem;
+};
+bool ln_ring_plan(LnRingPlan& r, long long rows, int cols, int esize, bool backward) {
+  const int most = backward && esize == 4 ? 8192 : 16384;
+  if (cols <= 1024 || cols > most || cols * esize % 16 != 0) return false;
+  r.per = cols > 8192 ? 32 : 16;
+  r.threads = cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
+  const int per_sm = 512 / r.threads;
+  r.blocks = sm_count() * per_sm;
+  const int stage = cols * esize * (backward ? 2 : 1);
+  r.stages = kLnRingBytes / per_sm / stage;
+  if (r.stages > kLnStages) r.stages = kLnStages;
+  r.smem = 128 + r.stages * stage;
+  return r.stages >= 2 && rows > 2ll * r.blocks;
+}
+
+template <typename T>
+int ln_fwd_ring(const LnRingPlan& r, const T* x, long long ldx, LnParam g, LnParam b, T* y, float* mean, float* rstd, long long rows, int cols,
+                float eps, cudaStream_t s) {
+  auto go = [&](auto kern) -> int {
+    PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, r.smem));
+    kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, r.stages, status_block_device_ptr());
+    PKB_CHECK_CUDA(cudaGetLastError());
+    return kApiOk;
+  };
+  if (r.threads == 128) return go(ln_fwd_ring_kernel<T, 128, 16>);
+  if (r.threads == 256) return go(ln_fwd_ring_kernel<T, 256, 16>);
+  if (r.per == 16) return go(ln_fwd_ring_kernel<T, 512, 16>);
+  return go(ln_fwd_ring_kernel<T, 512, 32>);
+}
+
+template <typename T>
+int ln_bwd_ring(const LnRingPlan& r, const T* x, long long ldx, const T* dy, long long lddy, LnParam g, const float* mean, const float* rstd,
+                T* dx, float* part, long long rows, int cols, cudaStream_t s) {
+  auto go = [&](auto kern) -> int {
+    PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, r.smem));
+    kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, r.stages, status_block_device_ptr());
+    PKB_CHECK_CUDA(cudaGetLastError());
+    return kApiOk;
+  };
+  if (r.threads == 128) return go(ln_bwd_ring_kernel<T, 128, 16>);
+  if (r.threads == 256) return go(ln_bwd_ring_kernel<T, 256, 16>);
+  if constexpr (sizeof(T) == 2) {
+    if (r.per == 32) return go(ln_bwd_ring_kernel<T, 512, 32>);
+  }
+  return go(ln_bwd_ring_kernel<T, 512, 16>);
+}
+
 template <typename T, int VEC16>
 int ln_fwd_any(const void* xv, long long ldx, LnParam g, LnParam b, void* yv, float* mean, float* rstd, long long rows, int cols, float eps,
                cudaStream_t s) {
   const T* x = static_cast<const T*>(xv);
   T* y = static_cast<T*>(yv);
+  const bool vec = cols % VEC16 == 0 && ln_aligned(x, ldx * (long long)sizeof(T)) && ln_aligned(y, 0) && ln_aligned(g.p, 0) && ln_aligned(b.p, 0);
+  LnRingPlan ring;
+  if (vec && ln_ring_plan(ring, rows, cols, sizeof(T), false)) return ln_fwd_ring<T>(ring, x, ldx, g, b, y, mean, rstd, rows, cols, eps, s);
   if (cols > kLnTeamCols) {
     const long long most = (long long)sm_count() * 4;
     ln_fwd_long_kernel<T><<<(unsigned)(rows < most ? rows : most), kLnLongThreads, 0, s>>>(x, ldx, g, b, y, mean, rstd, rows, cols, eps);
     PKB_CHECK_CUDA(cudaGetLastError());
     return kApiOk;
   }
-  const bool vec = cols % VEC16 == 0 && ln_aligned(x, ldx * (long long)sizeof(T)) && ln_aligned(y, 0) && ln_aligned(g.p, 0) && ln_aligned(b.p, 0);
   return vec ? ln_fwd_team<T, VEC16>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, s) : ln_fwd_team<T, 1>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, s);
 }
 
@@ -439,7 +746,7 @@ int ln_bwd_team(const T* x, long long ldx, const T* dy, long long lddy, LnParam 
   return ln_by_width<decltype(go)&, T, VEC>(cols, go);
 }
 
-// rows of a block at once and blocks per SM of the backward's team forms
+// blocks of the backward's team form (rows of a block at once, blocks per SM) or slices of its long form
 int ln_bwd_blocks(long long rows, int cols) {
   if (cols > kLnTeamCols) return (int)(rows < 4 * kLnLongSlices ? (rows + 3) / 4 : kLnLongSlices);
   const int tpr = cols <= 512 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
@@ -453,21 +760,26 @@ int ln_bwd_any(const void* xv, long long ldx, const void* dyv, long long lddy, L
                float* dgamma, float* dbeta, float* part, long long rows, int cols, cudaStream_t s) {
   const T *x = static_cast<const T*>(xv), *dy = static_cast<const T*>(dyv);
   T* dx = static_cast<T*>(dxv);
-  const int blocks = ln_bwd_blocks(rows, cols);
-  if (cols > kLnTeamCols) {
+  int blocks = ln_bwd_blocks(rows, cols);
+  const bool vec = cols % VEC16 == 0 && ln_aligned(x, ldx * (long long)sizeof(T)) && ln_aligned(dy, lddy * (long long)sizeof(T)) &&
+                   ln_aligned(dx, 0) && ln_aligned(g.p, 0) && ln_aligned(part, 0);
+  LnRingPlan ring;
+  if (vec && ln_ring_plan(ring, rows, cols, sizeof(T), true)) {
+    blocks = ring.blocks;
+    const int rc = ln_bwd_ring<T>(ring, x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, s);
+    if (rc) return rc;
+  } else if (cols > kLnTeamCols) {
     const long long most = (long long)sm_count() * 4;
     ln_bwd_long_dx_kernel<T><<<(unsigned)(rows < most ? rows : most), kLnLongThreads, 0, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, rows, cols);
     ln_bwd_long_params_kernel<T><<<dim3((unsigned)((cols + 63) / 64), (unsigned)blocks), 256, 0, s>>>(x, ldx, dy, lddy, mean, rstd, part, rows, cols);
     PKB_CHECK_CUDA(cudaGetLastError());
   } else {
-    const bool vec = cols % VEC16 == 0 && ln_aligned(x, ldx * (long long)sizeof(T)) && ln_aligned(dy, lddy * (long long)sizeof(T)) &&
-                     ln_aligned(dx, 0) && ln_aligned(g.p, 0);
     const int rc = vec ? ln_bwd_team<T, VEC16>(x, ldx, dy, lddy, g, mean, rstd, dx, part, blocks, rows, cols, s)
                        : ln_bwd_team<T, 1>(x, ldx, dy, lddy, g, mean, rstd, dx, part, blocks, rows, cols, s);
     if (rc) return rc;
   }
   const long long width = 2ll * cols;
-  ln_bwd_params_kernel<<<(unsigned)((width + 31) / 32), 256, 0, s>>>(part, blocks, width, dgamma, dbeta, cols);
+  ln_bwd_params_kernel<<<(unsigned)((width + 31) / 32), 1024, 0, s>>>(part, blocks, width, dgamma, dbeta, cols);
   PKB_CHECK_CUDA(cudaGetLastError());
   return kApiOk;
 }
@@ -492,7 +804,13 @@ extern "C" int pkb_layer_norm_fwd(const void* x, long long ldx, const void* gamm
 }
 
 // Blocks whose partial sums pkb_layer_norm_bwd writes: its scratch is [this][2][cols] fp32.
-extern "C" int pkb_layer_norm_bwd_partials(long long rows, int cols) { return rows > 0 && cols > 0 ? ln_bwd_blocks(rows, cols) : 0; }
+// (An upper bound over the forms that rows of this width may take: alignment decides between them.)
+extern "C" int pkb_layer_norm_bwd_partials(long long rows, int cols, int dtype) {
+  if (rows <= 0 || cols <= 0) return 0;
+  LnRingPlan ring;
+  const int blocks = ln_bwd_blocks(rows, cols), in_ring = ln_ring_plan(ring, rows, cols, dtype ? 4 : 2, true) ? ring.blocks : 0;
+  return blocks > in_ring ? blocks : in_ring;
+}
 
 // dx [rows, cols] (contiguous, the type of x and dy), dgamma and dbeta fp32 [cols] from the saved statistics.
 extern "C" int pkb_layer_norm_bwd(const void* x, long long ldx, const void* dy, long long lddy, const void* gamma, int param_f32, const void* mean,

@@ -28,45 +28,65 @@ constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortMaxExperts = 1024;
 constexpr int kSortCluster = 8;
 
+constexpr int kSortHeld = 8;       // rounds whose experts are held in registers between the passes
+
 __global__ void __launch_bounds__(kSortThreads)
 moe_sort_kernel(const int* __restrict__ idx, int n, int experts, int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ slots) {
-  extern __shared__ int table[];                        // [kSortWarps][experts]
-  __shared__ int total[kSortMaxExperts], base[kSortMaxExperts], warp_sums[kSortWarps + 1];
+  extern __shared__ int table[];                        // [warps in use][experts]
+  __shared__ int total[kSortMaxExperts], base[kSortMaxExperts], warp_sums[kSortWarps];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long rounds = ((long long)n + 32 * kSortWarps * ctas - 1) / (32 * kSortWarps * ctas);
+  const int all_rounds = (int)(((long long)n + 31) / 32);
+  const int rounds = (all_rounds + kSortWarps * ctas - 1) / (kSortWarps * ctas);                // per warp
+  const int warps = min(kSortWarps, (all_rounds + rounds - 1) / rounds);                        // that have any, in the first CTA
   const long long first = ((long long)rank * kSortWarps + warp) * rounds * 32;
   int* mine = table + warp * experts;
-  for (int e = threadIdx.x; e < kSortWarps * experts; e += kSortThreads) table[e] = 0;
-  __syncthreads();
-  for (long long r = 0; r < rounds && first + r * 32 < n; ++r) {
+  // the experts of the first rounds, all loads in flight at once
+  int held[kSortHeld];
+#pragma unroll
+  for (int r = 0; r < kSortHeld; ++r) {
     const long long i = first + r * 32 + lane;
-    const int e = i < n ? idx[i] : -1;
+    held[r] = r < rounds && i < n ? idx[i] : -1;
+  }
+  for (int e = threadIdx.x; e < warps * experts; e += kSortThreads) table[e] = 0;
+  __syncthreads();
+  auto count = [&](int e) {
     const bool ok = (unsigned)e < (unsigned)experts;
     const unsigned peers = __match_any_sync(0xffffffffu, ok ? e : -1);
     if (ok && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
     __syncwarp();
+  };
+#pragma unroll
+  for (int r = 0; r < kSortHeld; ++r)
+    if (r < rounds && first + r * 32 < n) count(held[r]);
+  for (int r = kSortHeld; r < rounds && first + r * 32ll < n; ++r) {
+    const long long i = first + r * 32ll + lane;
+    count(i < n ? idx[i] : -1);
   }
   __syncthreads();
   const int e = threadIdx.x;
   if (e < experts) {
     int run = 0;
-    for (int w = 0; w < kSortWarps; ++w) {
+    for (int w = 0; w < warps; ++w) {
       const int c = table[w * experts + e];
       table[w * experts + e] = run;
       run += c;
     }
     total[e] = run;
   }
-  cluster.sync();
   int before = 0, all = 0;
-  if (e < experts) {
-    for (int c = 0; c < ctas; ++c) {
-      const int v = cluster.map_shared_rank(total, c)[e];
-      if (c < rank) before += v;
-      all += v;
+  if (ctas > 1) {
+    cluster.sync();
+    if (e < experts) {
+      for (int c = 0; c < ctas; ++c) {
+        const int v = cluster.map_shared_rank(total, c)[e];
+        if (c < rank) before += v;
+        all += v;
+      }
     }
+  } else if (e < experts) {
+    all = total[e];
   }
   // exclusive sum over the experts, one per thread
   int incl = all;
@@ -97,9 +117,7 @@ moe_sort_kernel(const int* __restrict__ idx, int n, int experts, int* __restrict
     }
   }
   __syncthreads();
-  for (long long r = 0; r < rounds && first + r * 32 < n; ++r) {
-    const long long i = first + r * 32 + lane;
-    const int x = i < n ? idx[i] : -1;
+  auto place = [&](long long i, int x) {
     const bool ok = (unsigned)x < (unsigned)experts;
     const unsigned peers = __match_any_sync(0xffffffffu, ok ? x : -1);
     const int slot = ok ? base[x] + mine[x] + __popc(peers & ((1u << lane) - 1u)) : -1;
@@ -108,9 +126,16 @@ moe_sort_kernel(const int* __restrict__ idx, int n, int experts, int* __restrict
     __syncwarp();
     if (i < n) slots[i] = slot;
     if (ok) order[slot] = (int)i;
+  };
+#pragma unroll
+  for (int r = 0; r < kSortHeld; ++r)
+    if (r < rounds && first + r * 32 < n) place(first + r * 32 + lane, held[r]);
+  for (int r = kSortHeld; r < rounds && first + r * 32ll < n; ++r) {
+    const long long i = first + r * 32ll + lane;
+    place(i, i < n ? idx[i] : -1);
   }
   for (long long i = kept + (long long)rank * kSortThreads + threadIdx.x; i < n; i += (long long)ctas * kSortThreads) order[i] = -1;
-  cluster.sync();      // nobody leaves while its totals may still be read
+  if (ctas > 1) cluster.sync();      // nobody leaves while its totals may still be read
 }
 
 // ------------------------------------------------------------------------------------------------ rows
@@ -206,7 +231,7 @@ moe_permute_kernel(const T* __restrict__ x, long long ldx, const int* __restrict
 }
 
 // out[t] = sum_j gate[t, j] y[slots[t, j]]; GATED = false: weights of one
-constexpr int kGatherAhead = 4;   // rows whose loads are issued before the first of them is added
+constexpr int kGatherAhead = 8;   // rows whose loads are issued before the first of them is added
 
 template <typename T, int VEC, bool GATED>
 __global__ void __launch_bounds__(kRowThreads)
@@ -221,24 +246,24 @@ moe_unpermute_kernel(const T* __restrict__ y, long long ldy, const int* __restri
   float acc[kRowUnroll][VEC] = {};
   for (int j0 = 0; j0 < top_k; j0 += kGatherAhead) {
     typename V::Raw v[kGatherAhead][kRowUnroll];
+    unsigned s[kGatherAhead];
     float g[kGatherAhead];
-    bool there[kGatherAhead];
 #pragma unroll
     for (int a = 0; a < kGatherAhead; ++a) {
-      const int j = j0 + a;
-      const unsigned s = j < top_k ? (unsigned)slots[t * top_k + j] : n;
-      there[a] = s < n;
-      g[a] = 1.f;
-      if (there[a]) {
-        if constexpr (GATED) g[a] = gates[t * top_k + j];
+      s[a] = j0 + a < top_k ? (unsigned)slots[t * top_k + j0 + a] : n;
+      g[a] = GATED && j0 + a < top_k ? gates[t * top_k + j0 + a] : 1.f;
+    }
+#pragma unroll
+    for (int a = 0; a < kGatherAhead; ++a) {
+      if (s[a] < n) {
 #pragma unroll
         for (int u = 0; u < kRowUnroll; ++u)
-          if (first + u * team < nvec) v[a][u] = V::load(y + (long long)s * ldy + (long long)(first + u * team) * VEC);
+          if (first + u * team < nvec) v[a][u] = V::load(y + (long long)s[a] * ldy + (long long)(first + u * team) * VEC);
       }
     }
 #pragma unroll
     for (int a = 0; a < kGatherAhead; ++a) {
-      if (there[a]) {
+      if (s[a] < n) {
 #pragma unroll
         for (int u = 0; u < kRowUnroll; ++u) {
           if (first + u * team < nvec) {
@@ -256,29 +281,32 @@ moe_unpermute_kernel(const T* __restrict__ y, long long ldy, const int* __restri
     if (first + u * team < nvec) V::store(out + (t * nvec + first + u * team) * VEC, V::pack(acc[u]));
 }
 
-// One block per token: dy rows and the dot products in one pass over dout and y.
+// A team of TEAM threads per token: dy rows and the dot products in one pass over dout and y.
 constexpr int kBwdExperts = 8;    // experts of a token that a pass over its row handles at once
 
-template <typename T, int VEC, int NT>
-__global__ void __launch_bounds__(NT)
+template <typename T, int VEC, int TEAM>
+__global__ void __launch_bounds__(kRowThreads)
 moe_unpermute_bwd_kernel(const T* __restrict__ dout, long long lddo, const T* __restrict__ y, long long ldy, const int* __restrict__ slots,
                          const float* __restrict__ gates, const int* __restrict__ kept, T* __restrict__ dy, float* __restrict__ dgates,
                          long long tokens, int top_k, int nvec) {
   using V = RowVec<T, VEC>;
-  __shared__ float red[NT / 32][kBwdExperts];
+  constexpr int kTeams = kRowThreads / TEAM, kWarps = TEAM / 32;
+  __shared__ float red[kRowThreads / 32][kBwdExperts];
   const unsigned n = (unsigned)(tokens * top_k);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long t = blockIdx.x;
-  for (int j0 = 0; j0 < top_k; j0 += kBwdExperts) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, in_team = threadIdx.x % TEAM;
+  const long long t = (long long)blockIdx.x * kTeams + threadIdx.x / TEAM;
+  // a team of one warp leaves when there is no token for it; larger teams are the whole block
+  static_assert(TEAM == 32 || TEAM == kRowThreads, "teams are a warp or the block");
+  for (int j0 = 0; j0 < top_k && t < tokens; j0 += kBwdExperts) {
     unsigned s[kBwdExperts];
     float g[kBwdExperts], dot[kBwdExperts] = {};
 #pragma unroll
     for (int a = 0; a < kBwdExperts; ++a) {
-      const int j = j0 + a;
-      s[a] = j < top_k ? (unsigned)slots[t * top_k + j] : n;
-      g[a] = s[a] < n ? gates[t * top_k + j] : 0.f;
+      const bool in = j0 + a < top_k;
+      s[a] = in ? (unsigned)slots[t * top_k + j0 + a] : n;
+      g[a] = in ? gates[t * top_k + j0 + a] : 0.f;
     }
-    for (int i = threadIdx.x; i < nvec; i += NT) {
+    for (int i = in_team; i < nvec; i += TEAM) {
       float d[VEC];
       V::unpack(V::load(dout + t * lddo + (long long)i * VEC), d);
       typename V::Raw v[kBwdExperts];
@@ -304,17 +332,19 @@ moe_unpermute_bwd_kernel(const T* __restrict__ dout, long long lddo, const T* __
       const float w = warp_sum(dot[a]);
       if (lane == 0) red[warp][a] = w;
     }
-    __syncthreads();
-    if (threadIdx.x < kBwdExperts && j0 + (int)threadIdx.x < top_k) {
+    if constexpr (TEAM > 32) __syncthreads();
+    else __syncwarp();
+    if (in_team < kBwdExperts && j0 + in_team < top_k) {
+      const int w0 = TEAM > 32 ? 0 : warp;
       float w = 0.f;
 #pragma unroll
-      for (int k = 0; k < NT / 32; ++k) w += red[k][threadIdx.x];
-      dgates[t * top_k + j0 + threadIdx.x] = w;
+      for (int k = 0; k < kWarps; ++k) w += red[w0 + k][in_team];
+      dgates[t * top_k + j0 + in_team] = w;
     }
-    __syncthreads();
+    if constexpr (TEAM > 32) __syncthreads();
+    else __syncwarp();
   }
-  const long long from = max(*kept, 0), count = ((long long)n - from) * nvec;
-  for (long long i = t * NT + threadIdx.x; i < count; i += tokens * NT) V::store(dy + (from * nvec + i) * VEC, V::zero());
+  zero_rows<T, VEC>(dy, tokens * top_k, nvec, kept);
 }
 
 bool rows_aligned(const void* p, long long pitch_bytes) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)pitch_bytes) & 15) == 0; }
@@ -355,8 +385,13 @@ int unpermute_rows(const void* y, long long ldy, const int* slots, const float* 
 template <typename T, int VEC>
 int unpermute_bwd_rows(const void* dout, long long lddo, const void* y, long long ldy, const int* slots, const float* gates, const int* kept,
                        void* dy, float* dgates, long long tokens, int top_k, int hidden, cudaStream_t s) {
-  moe_unpermute_bwd_kernel<T, VEC, 256><<<(unsigned)tokens, 256, 0, s>>>(static_cast<const T*>(dout), lddo, static_cast<const T*>(y), ldy, slots, gates,
+  // a warp per token up to four accesses per lane (no barrier, eight tokens per block), else the block
+  auto go = [&](auto kern, int teams) {
+    kern<<<(unsigned)((tokens + teams - 1) / teams), kRowThreads, 0, s>>>(static_cast<const T*>(dout), lddo, static_cast<const T*>(y), ldy, slots, gates,
                                                                          kept, static_cast<T*>(dy), dgates, tokens, top_k, hidden / VEC);
+  };
+  if (hidden / VEC <= 128) go(moe_unpermute_bwd_kernel<T, VEC, 32>, kRowThreads / 32);
+  else go(moe_unpermute_bwd_kernel<T, VEC, kRowThreads>, 1);
   PKB_CHECK_CUDA(cudaGetLastError());
   return kApiOk;
 }
@@ -377,7 +412,8 @@ using namespace pkb;
 extern "C" int pkb_moe_sort(const void* idx, long long n, int experts, void* offsets, void* order, void* slots, void* stream) {
   PKB_CHECK_ARG(n > 0 && n <= 0x7fffffffll, "1 .. 2^31 - 1 assignments");
   PKB_CHECK_ARG(experts >= 1 && experts <= kSortMaxExperts, "1 .. 1024 experts");
-  const int smem = kSortWarps * experts * (int)sizeof(int);
+  const long long rounds = (n + 31) / 32;
+  const int smem = (int)(rounds < kSortWarps ? rounds : kSortWarps) * experts * (int)sizeof(int);
   PKB_CHECK_CUDA(cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const int ctas = n > 8192 ? kSortCluster : 1;
   cudaLaunchConfig_t cfg = {};

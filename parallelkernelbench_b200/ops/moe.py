@@ -290,10 +290,7 @@ def sort_by_expert(expert_idx: torch.Tensor, num_experts: int) -> ExpertSort:
     offsets = (torch.empty if n else torch.zeros)(num_experts + 1, dtype=torch.int32, device=idx.device)
     order, slots = (torch.empty(n, dtype=torch.int32, device=idx.device) for _ in range(2))
     if n:
-        with nv.on_device(idx):
-            nv.check(nv.bound("pkb_moe_sort", _SORT)(idx.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(), slots.data_ptr(),
-                                                     nv.raw_stream(idx)), "pkb_moe_sort")
-        nv.count_launch()
+        nv.launch("pkb_moe_sort", _SORT, idx, idx.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(), slots.data_ptr())
     return ExpertSort(offsets, order, slots, T, k)
 
 
@@ -332,10 +329,8 @@ def permute_tokens(x: torch.Tensor, srt: ExpertSort) -> torch.Tensor:
     n = _sort_arg(srt, x)
     out = torch.empty((n, x.shape[1]), dtype=x.dtype, device=x.device)
     if n:
-        with nv.on_device(x):
-            nv.check(nv.bound("pkb_moe_permute", _PERMUTE)(x.data_ptr(), x.stride(0), srt.slots.data_ptr(), _kept_ptr(srt), out.data_ptr(),
-                                                           srt.tokens, srt.top_k, x.shape[1], _DT[x.dtype], nv.raw_stream(x)), "pkb_moe_permute")
-        nv.count_launch()
+        nv.launch("pkb_moe_permute", _PERMUTE, x, x.data_ptr(), x.stride(0), srt.slots.data_ptr(), _kept_ptr(srt), out.data_ptr(), srt.tokens,
+                  srt.top_k, x.shape[1], _DT[x.dtype])
     return out
 
 
@@ -347,11 +342,8 @@ def unpermute_tokens(y: torch.Tensor, srt: ExpertSort, gates: torch.Tensor | Non
     g = None if gates is None else _gates_arg(gates, srt, y)
     out = (torch.empty if n else torch.zeros)((srt.tokens, y.shape[1]), dtype=y.dtype, device=y.device)
     if n:
-        with nv.on_device(y):
-            nv.check(nv.bound("pkb_moe_unpermute", _UNPERMUTE)(y.data_ptr(), y.stride(0), srt.slots.data_ptr(), 0 if g is None else g.data_ptr(),
-                                                               out.data_ptr(), srt.tokens, srt.top_k, y.shape[1], _DT[y.dtype], nv.raw_stream(y)),
-                     "pkb_moe_unpermute")
-        nv.count_launch()
+        nv.launch("pkb_moe_unpermute", _UNPERMUTE, y, y.data_ptr(), y.stride(0), srt.slots.data_ptr(), 0 if g is None else g.data_ptr(),
+                  out.data_ptr(), srt.tokens, srt.top_k, y.shape[1], _DT[y.dtype])
     return out
 
 
@@ -373,9 +365,6 @@ def unpermute_tokens_bwd(dout: torch.Tensor, y: torch.Tensor, srt: ExpertSort, g
     dy = torch.empty((n, y.shape[1]), dtype=y.dtype, device=y.device)
     dgates = torch.empty((srt.tokens, srt.top_k), dtype=torch.float32, device=y.device)
     if n:
-        with nv.on_device(y):
-            nv.check(nv.bound("pkb_moe_unpermute_bwd", _UNPERMUTE_BWD)(
-                dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0), srt.slots.data_ptr(), g.data_ptr(), _kept_ptr(srt), dy.data_ptr(),
-                dgates.data_ptr(), srt.tokens, srt.top_k, y.shape[1], _DT[y.dtype], nv.raw_stream(y)), "pkb_moe_unpermute_bwd")
-        nv.count_launch()
+        nv.launch("pkb_moe_unpermute_bwd", _UNPERMUTE_BWD, y, dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0), srt.slots.data_ptr(),
+                  g.data_ptr(), _kept_ptr(srt), dy.data_ptr(), dgates.data_ptr(), srt.tokens, srt.top_k, y.shape[1], _DT[y.dtype])
     return dy, dgates

@@ -57,14 +57,11 @@ def _launch(g, m, momentum, nesterov, steps, coefficients, eps, out, p, decay, s
     coeff = _coefficients(coefficients, int(steps), max(rows, cols))
     g = g.contiguous()
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    with nv.on_device(g):
-        launches = _I()
-        nbytes = nv.bound("pkb_newton_schulz_scratch", [_LL, _I, _I, _I, _P], _LL)(batch, rows, cols, steps, ctypes.addressof(launches))
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
-        nv.check(nv.bound("pkb_newton_schulz", _ARGS)(
-            g.data_ptr(), _DT[g.dtype], ptr(m), momentum, int(nesterov), batch, rows, cols, coeff, steps, eps, ptr(out), ptr(p), decay, scale,
-            ptr(p_bf16), ptr(scratch), nv.raw_stream(g)), "pkb_newton_schulz")
-    nv.count_launch(launches.value)
+    launches = _I()
+    nbytes = nv.bound("pkb_newton_schulz_scratch", [_LL, _I, _I, _I, _P], _LL)(batch, rows, cols, steps, ctypes.addressof(launches))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
+    nv.launch("pkb_newton_schulz", _ARGS, g, g.data_ptr(), _DT[g.dtype], ptr(m), momentum, int(nesterov), batch, rows, cols, coeff, steps, eps, ptr(out),
+              ptr(p), decay, scale, ptr(p_bf16), ptr(scratch), launches=launches.value)
 
 
 def newton_schulz(g: torch.Tensor, *, steps: int = 5, coefficients=FAST, eps: float = 1e-7) -> torch.Tensor:

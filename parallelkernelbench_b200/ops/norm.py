@@ -78,12 +78,9 @@ def _ln_forward(x, gamma, beta, eps, stats: bool):
     rstd = torch.empty_like(mean) if stats else None
     if rows:
         param = gamma if gamma is not None else beta
-        with nv.on_device(x):
-            nv.check(nv.bound("pkb_layer_norm_fwd", _LN_FWD)(
-                x2.data_ptr(), x2.stride(0), 0 if gamma is None else gamma.data_ptr(), 0 if beta is None else beta.data_ptr(),
-                0 if param is None else _DT[param.dtype], y.data_ptr(), mean.data_ptr() if stats else 0, rstd.data_ptr() if stats else 0,
-                rows, cols, eps, _DT[x.dtype], nv.raw_stream(x)), "pkb_layer_norm_fwd")
-        nv.count_launch()
+        nv.launch("pkb_layer_norm_fwd", _LN_FWD, x, x2.data_ptr(), x2.stride(0), 0 if gamma is None else gamma.data_ptr(),
+                  0 if beta is None else beta.data_ptr(), 0 if param is None else _DT[param.dtype], y.data_ptr(),
+                  mean.data_ptr() if stats else 0, rstd.data_ptr() if stats else 0, rows, cols, eps, _DT[x.dtype])
     return y, mean, rstd
 
 
@@ -115,12 +112,9 @@ def layer_norm_bwd(x: torch.Tensor, gamma: torch.Tensor | None, dy: torch.Tensor
         zero = torch.zeros((2, cols), dtype=torch.float32, device=x.device)
         return dx, zero[0], zero[1]
     dgamma, dbeta = (torch.empty(cols, dtype=torch.float32, device=x.device) for _ in range(2))
-    with nv.on_device(x):
-        blocks = nv.bound("pkb_layer_norm_bwd_partials", [_LL, _I])(rows, cols)
-        part = torch.empty((blocks, 2, cols), dtype=torch.float32, device=x.device)
-        nv.check(nv.bound("pkb_layer_norm_bwd", _LN_BWD)(
-            x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), 0 if gamma is None else gamma.data_ptr(),
-            0 if gamma is None else _DT[gamma.dtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(),
-            part.data_ptr(), rows, cols, _DT[x.dtype], nv.raw_stream(x)), "pkb_layer_norm_bwd")
-    nv.count_launch(2)
+    blocks = nv.bound("pkb_layer_norm_bwd_partials", [_LL, _I, _I])(rows, cols, _DT[x.dtype])
+    part = torch.empty((blocks, 2, cols), dtype=torch.float32, device=x.device)
+    nv.launch("pkb_layer_norm_bwd", _LN_BWD, x, x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), 0 if gamma is None else gamma.data_ptr(),
+              0 if gamma is None else _DT[gamma.dtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(),
+              part.data_ptr(), rows, cols, _DT[x.dtype], launches=2)
     return dx, dgamma, dbeta

@@ -62,7 +62,9 @@ def _check(x, dy, gamma, beta, eps, got, stats=None, grads=None):
 # one column, one access, the ends of a team's reach (32, 64, 128, 256, 512 threads of 16 values) and one more, rows that start at odd
 # addresses, rows beyond the teams, more rows than the grid takes at a time
 SHAPES = [(1, 1), (3, 2), (1, 4096), (3, 7), (5, 8), (7, 512), (7, 513), (9, 520), (9, 1024), (2, 1032), (33, 2048), (3, 2056), (17, 4096), (5, 4097),
-          (5, 4104), (3, 8192), (2, 8193), (3, 8200), (2, 20001), (300, 8200), (2500, 64), (1333, 1001), (9001, 33)]
+          (5, 4104), (3, 8192), (2, 8193), (3, 8200), (2, 20001), (300, 8200), (2500, 64), (1333, 1001), (9001, 33),
+          # many wide rows (the ring): every width class, the last row of a round and one more, a row that is no multiple of a thread's access
+          (2400, 1032), (1185, 2048), (1400, 2056), (1184, 4096), (1185, 4096), (3000, 4104), (600, 8192), (700, 8200), (301, 16384), (400, 16392)]
 
 
 @pytest.mark.parametrize("dtype,param", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32),
@@ -129,31 +131,41 @@ def test_a_bad_row_stays_alone():
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("view", ["offset", "pitch", "odd_pitch", "dims", "transposed", "expanded"])
 def test_layouts(view, dtype):
+    _layouts(view, dtype, 24)
+
+
+@pytest.mark.parametrize("view", ["pitch", "odd_pitch", "expanded"])
+def test_layouts_of_many_wide_rows(view):
+    _layouts(view, torch.bfloat16, 1300, 4)
+
+
+def _layouts(view, dtype, rows, times=1):
     from parallelkernelbench_b200.ops import layer_norm_bwd, layer_norm_fwd
 
-    x, dy, gamma, beta = _inputs(24, 520, dtype, torch.float32)
+    n = 512 * times
+    x, dy, gamma, beta = _inputs(rows, n + 8, dtype, torch.float32)
 
     def lay(t):
         if view == "offset":
-            return t.reshape(-1)[1:1 + 23 * 512].view(23, 512)
+            return t.reshape(-1)[1:1 + 23 * n].view(23, n)
         if view == "pitch":
-            return t[:, :512]
+            return t[:, :n]
         if view == "odd_pitch":
-            return torch.nn.functional.pad(t, (0, 1))[:, :512]
+            return torch.nn.functional.pad(t, (0, 1))[:, :n]
         if view == "dims":
-            return t[:, :512].reshape(2, 3, 4, 512)
+            return t[:, :n].reshape(2, 3, 4, n)
         if view == "transposed":
-            return t[:, :512].t().contiguous().t()
-        return t[:1, :512].expand(24, 512)
+            return t[:, :n].t().contiguous().t()
+        return t[:1, :n].expand(rows, n)
 
-    xv, dyv, g, b = lay(x), lay(dy), gamma[:512], beta[:512]
+    xv, dyv, g, b = lay(x), lay(dy), gamma[:n], beta[:n]
     before = (x.clone(), dy.clone())
     y, mean, rstd = layer_norm_fwd(xv, g, b)
     assert y.shape == xv.shape and mean.shape == xv.shape[:-1]
     _check(xv, dyv, g, b, 1e-5, y, (mean, rstd), layer_norm_bwd(xv, g, dyv, mean, rstd))
     # gain and bias off the 16-byte boundary
-    y, mean, rstd = layer_norm_fwd(xv, gamma[1:513], beta[1:513])
-    _check(xv, dyv, gamma[1:513], beta[1:513], 1e-5, y, (mean, rstd), layer_norm_bwd(xv, gamma[1:513], dyv, mean, rstd))
+    y, mean, rstd = layer_norm_fwd(xv, gamma[1:n + 1], beta[1:n + 1])
+    _check(xv, dyv, gamma[1:n + 1], beta[1:n + 1], 1e-5, y, (mean, rstd), layer_norm_bwd(xv, gamma[1:n + 1], dyv, mean, rstd))
     assert torch.equal(x, before[0]) and torch.equal(dy, before[1])
 
 
