@@ -138,7 +138,7 @@ def launch(name: str, argtypes: list, t, *args, launches: int = 1) -> None:
     import torch
 
     f = _bound.get(name) or bound(name, argtypes)
-    device = t.device.index
+    device = t.get_device()
     if device == torch._C._cuda_getDevice():
         rc = f(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
@@ -153,9 +153,17 @@ def same_cuda_device(first, **tensors) -> None:
     """Every tensor (``None`` is passed over) lives on the CUDA device of ``first``."""
     if not first.is_cuda:
         raise ValueError("expected CUDA tensors")
+    device = first.get_device()
     for name, t in tensors.items():
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != device:
             raise ValueError(f"{name} is on {t.device}, not on {first.device}")
+
+
+def contiguous_like(t):
+    """An uninitialised contiguous tensor of the shape and type of ``t`` (``empty_like`` is the cheaper call, but keeps strides)."""
+    import torch
+
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def read_status() -> list[int]:

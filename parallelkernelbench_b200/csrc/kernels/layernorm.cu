@@ -97,12 +97,12 @@ __device__ __forceinline__ void team_sum(float (&v)[K], float* red, int team) {
       for (int k = 0; k < K; ++k) red[k * (NT / 32) + warp] = v[k];
     }
     team_sync<TPR, NT>(team);
+    // a lane takes one warp's sum and the lanes add them up: the same tree, and so the same bits, in every lane
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float t = 0.f;
+      v[k] = red[k * (NT / 32) + team * W + (threadIdx.x & (W - 1))];
 #pragma unroll
-      for (int w = 0; w < W; ++w) t += red[k * (NT / 32) + team * W + w];
-      v[k] = t;
+      for (int o = W / 2; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
     }
   }
 }
@@ -323,15 +323,69 @@ struct LnRing {
   int stages;
 };
 
-// 16 bytes as VEC fp32 values
+// Pairs of fp32 values in one register pair: Blackwell's packed adds, products and fused products halve the arithmetic, which with single
+// values had the schedulers of 16 warps busy for 55 % (forward) and 67 % (backward) of the time at half of the memory bandwidth.
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float both) { return f2(both, both); }
+__device__ __forceinline__ float2 f2_split(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ float f2_sum(F2 a) {
+  const float2 r = f2_split(a);
+  return r.x + r.y;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 16 bytes as VEC / 2 pairs, and back (rounded to nearest)
 template <int VEC>
-__device__ __forceinline__ void ln_unpack(const U4& u, float (&f)[VEC]) {
-  if constexpr (VEC == 8) {
-    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
-    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
-  } else {
-    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+__device__ __forceinline__ void ln_pairs(const U4& u, F2 (&f)[VEC / 2]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < VEC / 2; ++j)
+    f[j] = VEC == 8 ? f2(__uint_as_float(w[j & 3] << 16), __uint_as_float(w[j & 3] & 0xffff0000u)) : f2(__uint_as_float(w[(2 * j) & 3]), __uint_as_float(w[(2 * j + 1) & 3]));
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void ln_store_pairs(T* p, const F2 (&f)[VEC / 2]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < VEC / 2; ++j) {
+    const float2 v = f2_split(f[j]);
+    if constexpr (VEC == 8) {
+      w[j] = pack_bf16x2(v.x, v.y);
+    } else {
+      w[2 * j] = __float_as_uint(v.x);
+      w[2 * j + 1] = __float_as_uint(v.y);
+    }
   }
+  st_global_v4(p, U4{w[0], w[1], w[2], w[3]});
+}
+template <int VEC>
+__device__ __forceinline__ void ln_param_pairs(const LnParam& p, int c, F2 (&f)[VEC / 2]) {
+  float v[VEC];
+  p.template load<VEC>(c, v);
+#pragma unroll
+  for (int j = 0; j < VEC / 2; ++j) f[j] = f2(v[2 * j], v[2 * j + 1]);
 }
 __device__ __forceinline__ U4 ln_shared(uint32_t a) {
   U4 v;
@@ -367,7 +421,7 @@ template <typename T, int NT, int PER>
 __global__ void __launch_bounds__(NT, 512 / NT)
 ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, const LnParam beta, T* __restrict__ y,
                    float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, int cols, float eps, int stages, uint32_t* status) {
-  constexpr int VEC = 16 / sizeof(T), CH = PER / VEC;
+  constexpr int VEC = 16 / sizeof(T), CH = PER / VEC, P = VEC / 2;
   constexpr bool kHoldGain = PER <= 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[2][NT / 32];
@@ -383,14 +437,14 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
   if (t == 0)
     for (int i = 0; i < stages; ++i)
       if (blockIdx.x + (long long)i * gridDim.x < rows) issue(blockIdx.x + (long long)i * gridDim.x, i);
-  float g[kHoldGain ? CH : 1][VEC], b[kHoldGain ? CH : 1][VEC];
+  F2 g[kHoldGain ? CH : 1][P], b[kHoldGain ? CH : 1][P];
   if constexpr (kHoldGain) {
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (ch * NT + t) * VEC;
       if (c < cols) {
-        gamma.template load<VEC>(c, g[ch]);
-        beta.template load<VEC>(c, b[ch]);
+        ln_param_pairs<VEC>(gamma, c, g[ch]);
+        ln_param_pairs<VEC>(beta, c, b[ch]);
       }
     }
   }
@@ -401,48 +455,56 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
       ln_ring_abandon();
       return;
     }
-    float v[CH][VEC];
-    float s[1] = {0.f}, q[1] = {0.f};
+    F2 v[CH][P], acc = 0;
+    float s[1], q[1];
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (ch * NT + t) * VEC;
       if (c < cols) {
-        ln_unpack<VEC>(ln_shared(ring.base + stage * bytes + c * (int)sizeof(T)), v[ch]);
+        ln_pairs<VEC>(ln_shared(ring.base + stage * bytes + c * (int)sizeof(T)), v[ch]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s[0] += v[ch][j];
+        for (int j = 0; j < P; ++j) acc = add2(acc, v[ch][j]);
       }
     }
+    s[0] = f2_sum(acc);
     team_sum<1, NT, NT>(s, red[0], 0);
     if (t == 0 && row + (long long)stages * gridDim.x < rows) {
       fence_proxy_async_smem();
       issue(row + (long long)stages * gridDim.x, stage);
     }
     const float mean = s[0] * inv;
+    const F2 shift = f2(-mean);
+    acc = 0;
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       if ((ch * NT + t) * VEC < cols) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) q[0] += (v[ch][j] - mean) * (v[ch][j] - mean);
+        for (int j = 0; j < P; ++j) {
+          v[ch][j] = add2(v[ch][j], shift);
+          acc = fma2(v[ch][j], v[ch][j], acc);
+        }
       }
     }
+    q[0] = f2_sum(acc);
     team_sum<1, NT, NT>(q, red[1], 0);
     const float rstd = rsqrtf(q[0] * inv + eps);
     if (t == 0 && mean_out != nullptr) {
       mean_out[row] = mean;
       rstd_out[row] = rstd;
     }
+    const F2 r2 = f2(rstd);
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (ch * NT + t) * VEC;
       if (c < cols) {
         constexpr int kAt = kHoldGain ? 1 : 0;
         if constexpr (!kHoldGain) {
-          gamma.template load<VEC>(c, g[0]);
-          beta.template load<VEC>(c, b[0]);
+          ln_param_pairs<VEC>(gamma, c, g[0]);
+          ln_param_pairs<VEC>(beta, c, b[0]);
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[ch][j] = (v[ch][j] - mean) * rstd * g[kAt * ch][j] + b[kAt * ch][j];
-        ln_store<T, VEC>(y + row * cols + c, v[ch]);
+        for (int j = 0; j < P; ++j) v[ch][j] = fma2(mul2(v[ch][j], r2), g[kAt * ch][j], b[kAt * ch][j]);
+        ln_store_pairs<T, VEC>(y + row * cols + c, v[ch]);
       }
     }
     if (++stage == stages) {
@@ -452,14 +514,13 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
   }
 }
 
-// A stage holds a row of x and the same row of dy. PER: values per thread; with 32 the gain is read again for every row (16 KB from L1 and
-// L2) instead of being held in registers.
+// A stage holds a row of x and the same row of dy. PER as above; here only the gain is held.
 template <typename T, int NT, int PER>
 __global__ void __launch_bounds__(NT, 512 / NT)
 ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ dy, long long lddy, const LnParam gamma,
                    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part,
                    long long rows, int cols, int stages, uint32_t* status) {
-  constexpr int VEC = 16 / sizeof(T), CH = PER / VEC;
+  constexpr int VEC = 16 / sizeof(T), CH = PER / VEC, P = VEC / 2;
   constexpr bool kHoldGain = PER <= 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[2][2 * (NT / 32)];
@@ -477,13 +538,13 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
   if (t == 0)
     for (int i = 0; i < stages; ++i)
       if (blockIdx.x + (long long)i * gridDim.x < rows) issue(blockIdx.x + (long long)i * gridDim.x, i);
-  float ag[CH][VEC] = {}, ab[CH][VEC] = {};
-  float g[kHoldGain ? CH : 1][VEC];
+  F2 ag[CH][P] = {}, ab[CH][P] = {};
+  F2 g[kHoldGain ? CH : 1][P];
   if constexpr (kHoldGain) {
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (ch * NT + t) * VEC;
-      if (c < cols) gamma.template load<VEC>(c, g[ch]);
+      if (c < cols) ln_param_pairs<VEC>(gamma, c, g[ch]);
     }
   }
   int stage = 0, it = 0;
@@ -499,8 +560,9 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
       ln_ring_abandon();
       return;
     }
+    const F2 shift = f2(-mean), r2 = f2(rstd);
     U4 xr[CH], dr[CH];
-    float s[2] = {0.f, 0.f};
+    F2 s1 = 0, s2 = 0;
     const uint32_t at = ring.base + stage * 2 * bytes;
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
@@ -508,37 +570,42 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
       if (c < cols) {
         xr[ch] = ln_shared(at + c * (int)sizeof(T));
         dr[ch] = ln_shared(at + bytes + c * (int)sizeof(T));
-        float xv[VEC], dv[VEC];
-        ln_unpack<VEC>(xr[ch], xv);
-        ln_unpack<VEC>(dr[ch], dv);
-        if constexpr (!kHoldGain) gamma.template load<VEC>(c, g[0]);
+        F2 xv[P], dv[P];
+        ln_pairs<VEC>(xr[ch], xv);
+        ln_pairs<VEC>(dr[ch], dv);
+        if constexpr (!kHoldGain) ln_param_pairs<VEC>(gamma, c, g[0]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float xh = (xv[j] - mean) * rstd, gd = dv[j] * g[kHoldGain ? ch : 0][j];
-          ag[ch][j] += dv[j] * xh;
-          ab[ch][j] += dv[j];
-          s[0] += gd;
-          s[1] += gd * xh;
+        for (int j = 0; j < P; ++j) {
+          const F2 xh = mul2(add2(xv[j], shift), r2), gd = mul2(dv[j], g[kHoldGain ? ch : 0][j]);
+          ag[ch][j] = fma2(dv[j], xh, ag[ch][j]);
+          ab[ch][j] = add2(dv[j], ab[ch][j]);
+          s1 = add2(gd, s1);
+          s2 = fma2(gd, xh, s2);
         }
       }
     }
+    float s[2] = {f2_sum(s1), f2_sum(s2)};
     team_sum<2, NT, NT>(s, red[it], 0);
     if (t == 0 && row + (long long)stages * gridDim.x < rows) {
       fence_proxy_async_smem();
       issue(row + (long long)stages * gridDim.x, stage);
     }
-    const float c1 = s[0] * inv, c2 = s[1] * inv;
+    // rstd (g dy - c1 - xhat c2)
+    const F2 c1 = f2(-s[0] * inv * rstd), c2 = f2(-s[1] * inv * rstd);
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (ch * NT + t) * VEC;
       if (c < cols) {
-        float xv[VEC], dv[VEC];
-        ln_unpack<VEC>(xr[ch], xv);
-        ln_unpack<VEC>(dr[ch], dv);
-        if constexpr (!kHoldGain) gamma.template load<VEC>(c, g[0]);
+        F2 xv[P], dv[P];
+        ln_pairs<VEC>(xr[ch], xv);
+        ln_pairs<VEC>(dr[ch], dv);
+        if constexpr (!kHoldGain) ln_param_pairs<VEC>(gamma, c, g[0]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) dv[j] = rstd * (dv[j] * g[kHoldGain ? ch : 0][j] - c1 - (xv[j] - mean) * rstd * c2);
-        ln_store<T, VEC>(dx + row * cols + c, dv);
+        for (int j = 0; j < P; ++j) {
+          const F2 xh = mul2(add2(xv[j], shift), r2), gd = mul2(dv[j], g[kHoldGain ? ch : 0][j]);
+          dv[j] = fma2(xh, c2, fma2(gd, r2, c1));
+        }
+        ln_store_pairs<T, VEC>(dx + row * cols + c, dv);
       }
     }
     if (++stage == stages) {
@@ -552,10 +619,9 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
     const int c = (ch * NT + t) * VEC;
     if (c < cols) {
 #pragma unroll
-      for (int j = 0; j < VEC; j += 4) {
-        st_global_v4(out + c + j, U4{__float_as_uint(ag[ch][j]), __float_as_uint(ag[ch][j + 1]), __float_as_uint(ag[ch][j + 2]), __float_as_uint(ag[ch][j + 3])});
-        st_global_v4(out + cols + c + j,
-                     U4{__float_as_uint(ab[ch][j]), __float_as_uint(ab[ch][j + 1]), __float_as_uint(ab[ch][j + 2]), __float_as_uint(ab[ch][j + 3])});
+      for (int j = 0; j < P; j += 2) {
+        *reinterpret_cast<ulonglong2*>(out + c + 2 * j) = make_ulonglong2(ag[ch][j], ag[ch][j + 1]);
+        *reinterpret_cast<ulonglong2*>(out + cols + c + 2 * j) = make_ulonglong2(ab[ch][j], ab[ch][j + 1]);
       }
     }
   }

@@ -20,13 +20,14 @@ namespace cg = cooperative_groups;
 
 // ------------------------------------------------------------------------------------------------ sort
 // One cluster of CTAs, one launch. A warp owns a contiguous run of assignments, 32 at a time. Pass 1 counts its experts in its own row of
-// the CTA's table (lanes with the same expert find one another by match.any; one of them adds for all, so the table needs no atomics);
+// the CTA's table (lanes with the same expert find one another by votes; one of them adds for all, so the table needs no atomics);
 // the table is then summed over warps, over CTAs (distributed shared memory) and over experts; pass 2 walks the assignments again and
 // hands out the slots in order.
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortMaxExperts = 1024;
-constexpr int kSortCluster = 8;
+constexpr int kSortMaxBits = 10;
+constexpr int kSortCluster = 16;
 
 constexpr int kSortHeld = 8;       // rounds whose experts are held in registers between the passes
 
@@ -51,9 +52,22 @@ moe_sort_kernel(const int* __restrict__ idx, int n, int experts, int* __restrict
   }
   for (int e = threadIdx.x; e < warps * experts; e += kSortThreads) table[e] = 0;
   __syncthreads();
+  const int bits = 32 - __clz(experts - 1);
+  // lanes that name the same expert (of a lane that names one): a vote per bit of its number
+  auto peers_of = [&](int e, bool ok) {
+    unsigned peers = __ballot_sync(0xffffffffu, ok);
+#pragma unroll
+    for (int b = 0; b < kSortMaxBits; ++b) {
+      if (b < bits) {
+        const unsigned set = __ballot_sync(0xffffffffu, (e >> b) & 1);
+        peers &= (e >> b) & 1 ? set : ~set;
+      }
+    }
+    return peers;
+  };
   auto count = [&](int e) {
     const bool ok = (unsigned)e < (unsigned)experts;
-    const unsigned peers = __match_any_sync(0xffffffffu, ok ? e : -1);
+    const unsigned peers = peers_of(e, ok);
     if (ok && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
     __syncwarp();
   };
@@ -119,7 +133,7 @@ moe_sort_kernel(const int* __restrict__ idx, int n, int experts, int* __restrict
   __syncthreads();
   auto place = [&](long long i, int x) {
     const bool ok = (unsigned)x < (unsigned)experts;
-    const unsigned peers = __match_any_sync(0xffffffffu, ok ? x : -1);
+    const unsigned peers = peers_of(x, ok);
     const int slot = ok ? base[x] + mine[x] + __popc(peers & ((1u << lane) - 1u)) : -1;
     __syncwarp();
     if (ok && lane == __ffs(peers) - 1) mine[x] += __popc(peers);
@@ -183,7 +197,7 @@ constexpr int kRowThreads = 256;
 // team * unroll accesses of its row.
 struct RowGrid {
   int team_log2, pieces;
-  __device__ __forceinline__ bool place(long long tokens, long long& token, int& first, int unroll) const {
+  __device__ __forceinline__ bool place(long long tokens, long long& token, int& first, int unroll = 1) const {
     const int team = 1 << team_log2;
     const long long unit = (long long)blockIdx.x * (kRowThreads >> team_log2) + (threadIdx.x >> team_log2);
     token = unit / pieces;
@@ -230,22 +244,23 @@ moe_permute_kernel(const T* __restrict__ x, long long ldx, const int* __restrict
   zero_rows<T, VEC>(xp, tokens * top_k, nvec, kept);
 }
 
-// out[t] = sum_j gate[t, j] y[slots[t, j]]; GATED = false: weights of one
+// out[t] = sum_j gate[t, j] y[slots[t, j]]; GATED = false: weights of one. One access per row and thread, eight rows in flight: with two
+// accesses per row the registers left two blocks per SM, too few to cover the way from a slot to its row (8192 tokens x 7168, top-8: 210 us).
 constexpr int kGatherAhead = 8;   // rows whose loads are issued before the first of them is added
 
 template <typename T, int VEC, bool GATED>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 4)
 moe_unpermute_kernel(const T* __restrict__ y, long long ldy, const int* __restrict__ slots, const float* __restrict__ gates, T* __restrict__ out,
                      long long tokens, int top_k, int nvec, const RowGrid grid) {
   using V = RowVec<T, VEC>;
   long long t;
-  int first;
-  if (!grid.place(tokens, t, first, kRowUnroll)) return;
-  const int team = 1 << grid.team_log2;
+  int i;
+  if (!grid.place(tokens, t, i) || i >= nvec) return;
   const unsigned n = (unsigned)(tokens * top_k);
-  float acc[kRowUnroll][VEC] = {};
+  const T* col = y + (long long)i * VEC;
+  float acc[VEC] = {};
   for (int j0 = 0; j0 < top_k; j0 += kGatherAhead) {
-    typename V::Raw v[kGatherAhead][kRowUnroll];
+    typename V::Raw v[kGatherAhead];
     unsigned s[kGatherAhead];
     float g[kGatherAhead];
 #pragma unroll
@@ -254,31 +269,19 @@ moe_unpermute_kernel(const T* __restrict__ y, long long ldy, const int* __restri
       g[a] = GATED && j0 + a < top_k ? gates[t * top_k + j0 + a] : 1.f;
     }
 #pragma unroll
-    for (int a = 0; a < kGatherAhead; ++a) {
-      if (s[a] < n) {
-#pragma unroll
-        for (int u = 0; u < kRowUnroll; ++u)
-          if (first + u * team < nvec) v[a][u] = V::load(y + (long long)s[a] * ldy + (long long)(first + u * team) * VEC);
-      }
-    }
+    for (int a = 0; a < kGatherAhead; ++a)
+      if (s[a] < n) v[a] = V::load(col + (long long)s[a] * ldy);
 #pragma unroll
     for (int a = 0; a < kGatherAhead; ++a) {
       if (s[a] < n) {
+        float f[VEC];
+        V::unpack(v[a], f);
 #pragma unroll
-        for (int u = 0; u < kRowUnroll; ++u) {
-          if (first + u * team < nvec) {
-            float f[VEC];
-            V::unpack(v[a][u], f);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[u][i] += GATED ? g[a] * f[i] : f[i];
-          }
-        }
+        for (int c = 0; c < VEC; ++c) acc[c] += GATED ? g[a] * f[c] : f[c];
       }
     }
   }
-#pragma unroll
-  for (int u = 0; u < kRowUnroll; ++u)
-    if (first + u * team < nvec) V::store(out + (t * nvec + first + u * team) * VEC, V::pack(acc[u]));
+  V::store(out + (t * nvec + i) * VEC, V::pack(acc));
 }
 
 // A team of TEAM threads per token: dy rows and the dot products in one pass over dout and y.
@@ -349,11 +352,11 @@ moe_unpermute_bwd_kernel(const T* __restrict__ dout, long long lddo, const T* __
 
 bool rows_aligned(const void* p, long long pitch_bytes) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)pitch_bytes) & 15) == 0; }
 
-// teams of the smallest power of two that covers a row with kRowUnroll accesses per thread, up to the whole block
-RowGrid row_grid(long long tokens, int nvec, unsigned* blocks) {
+// teams of the smallest power of two that covers a row with `unroll` accesses per thread, up to the whole block
+RowGrid row_grid(long long tokens, int nvec, int unroll, unsigned* blocks) {
   RowGrid g{0, 1};
-  while (g.team_log2 < 8 && (kRowUnroll << g.team_log2) < nvec) ++g.team_log2;
-  const int per = kRowUnroll << g.team_log2;
+  while (g.team_log2 < 8 && (unroll << g.team_log2) < nvec) ++g.team_log2;
+  const int per = unroll << g.team_log2;
   g.pieces = (nvec + per - 1) / per;
   const long long teams = kRowThreads >> g.team_log2;
   *blocks = (unsigned)((tokens * g.pieces + teams - 1) / teams);
@@ -363,7 +366,7 @@ RowGrid row_grid(long long tokens, int nvec, unsigned* blocks) {
 template <typename T, int VEC>
 int permute_rows(const void* x, long long ldx, const int* slots, const int* kept, void* xp, long long tokens, int top_k, int hidden, cudaStream_t s) {
   unsigned blocks;
-  const RowGrid g = row_grid(tokens, hidden / VEC, &blocks);
+  const RowGrid g = row_grid(tokens, hidden / VEC, kRowUnroll, &blocks);
   moe_permute_kernel<T, VEC><<<blocks, kRowThreads, 0, s>>>(static_cast<const T*>(x), ldx, slots, kept, static_cast<T*>(xp), tokens, top_k, hidden / VEC, g);
   PKB_CHECK_CUDA(cudaGetLastError());
   return kApiOk;
@@ -373,7 +376,7 @@ template <typename T, int VEC>
 int unpermute_rows(const void* y, long long ldy, const int* slots, const float* gates, void* out, long long tokens, int top_k, int hidden,
                    cudaStream_t s) {
   unsigned blocks;
-  const RowGrid g = row_grid(tokens, hidden / VEC, &blocks);
+  const RowGrid g = row_grid(tokens, hidden / VEC, 1, &blocks);
   const T* yp = static_cast<const T*>(y);
   T* op = static_cast<T*>(out);
   if (gates != nullptr) moe_unpermute_kernel<T, VEC, true><<<blocks, kRowThreads, 0, s>>>(yp, ldy, slots, gates, op, tokens, top_k, hidden / VEC, g);
@@ -415,6 +418,7 @@ extern "C" int pkb_moe_sort(const void* idx, long long n, int experts, void* off
   const long long rounds = (n + 31) / 32;
   const int smem = (int)(rounds < kSortWarps ? rounds : kSortWarps) * experts * (int)sizeof(int);
   PKB_CHECK_CUDA(cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  PKB_CHECK_CUDA(cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   const int ctas = n > 8192 ? kSortCluster : 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);

@@ -287,8 +287,9 @@ def sort_by_expert(expert_idx: torch.Tensor, num_experts: int) -> ExpertSort:
         raise ValueError("at most 2^31 - 1 assignments")
     nv.same_cuda_device(expert_idx)
     idx = expert_idx.contiguous()
-    offsets = (torch.empty if n else torch.zeros)(num_experts + 1, dtype=torch.int32, device=idx.device)
-    order, slots = (torch.empty(n, dtype=torch.int32, device=idx.device) for _ in range(2))
+    offsets = (idx.new_empty if n else idx.new_zeros)(num_experts + 1)
+    order = idx.new_empty(n)
+    slots = torch.empty_like(order)
     if n:
         nv.launch("pkb_moe_sort", _SORT, idx, idx.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(), slots.data_ptr())
     return ExpertSort(offsets, order, slots, T, k)
@@ -304,10 +305,13 @@ def _rows_arg(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
 
 def _sort_arg(srt: ExpertSort, like: torch.Tensor) -> int:
     n = srt.tokens * srt.top_k
-    for name, t, numel in (("offsets", srt.offsets, None), ("slots", srt.slots, n)):
-        if t.dtype != torch.int32 or not t.is_contiguous() or (numel is not None and t.numel() != numel):
-            raise ValueError(f"{name} of the sort must be contiguous int32 as sort_by_expert makes it")
-    nv.same_cuda_device(like, offsets=srt.offsets, slots=srt.slots)
+    offsets, slots, device = srt.offsets, srt.slots, like.get_device()
+    if offsets.dtype != torch.int32 or slots.dtype != torch.int32 or not offsets.numel() or slots.numel() != n:
+        raise ValueError("offsets and slots of the sort must be int32 as sort_by_expert makes them")
+    if not (offsets.is_contiguous() and slots.is_contiguous()):
+        raise ValueError("offsets and slots of the sort must be contiguous as sort_by_expert makes them")
+    if device < 0 or offsets.get_device() != device or slots.get_device() != device:
+        raise ValueError("the rows and the sort must be on one CUDA device")
     return n
 
 
@@ -318,7 +322,8 @@ def _kept_ptr(srt: ExpertSort) -> int:
 def _gates_arg(gates: torch.Tensor, srt: ExpertSort, like: torch.Tensor) -> torch.Tensor:
     if gates.dtype != torch.float32 or gates.shape != (srt.tokens, srt.top_k):
         raise ValueError(f"gates must be fp32 [{srt.tokens}, {srt.top_k}]")
-    nv.same_cuda_device(like, gates=gates)
+    if gates.get_device() != like.get_device():
+        raise ValueError(f"gates is on {gates.device}, not on {like.device}")
     return gates.contiguous()
 
 
@@ -327,7 +332,7 @@ def permute_tokens(x: torch.Tensor, srt: ExpertSort) -> torch.Tensor:
     ``out[slots[t, j]] = x[t]``. Rows from ``offsets[E]`` on are zero."""
     x = _rows_arg(x, srt.tokens, "x")
     n = _sort_arg(srt, x)
-    out = torch.empty((n, x.shape[1]), dtype=x.dtype, device=x.device)
+    out = x.new_empty((n, x.shape[1]))
     if n:
         nv.launch("pkb_moe_permute", _PERMUTE, x, x.data_ptr(), x.stride(0), srt.slots.data_ptr(), _kept_ptr(srt), out.data_ptr(), srt.tokens,
                   srt.top_k, x.shape[1], _DT[x.dtype])
@@ -340,7 +345,7 @@ def unpermute_tokens(y: torch.Tensor, srt: ExpertSort, gates: torch.Tensor | Non
     y = _rows_arg(y, srt.tokens * srt.top_k, "y")
     n = _sort_arg(srt, y)
     g = None if gates is None else _gates_arg(gates, srt, y)
-    out = (torch.empty if n else torch.zeros)((srt.tokens, y.shape[1]), dtype=y.dtype, device=y.device)
+    out = (y.new_empty if n else y.new_zeros)((srt.tokens, y.shape[1]))
     if n:
         nv.launch("pkb_moe_unpermute", _UNPERMUTE, y, y.data_ptr(), y.stride(0), srt.slots.data_ptr(), 0 if g is None else g.data_ptr(),
                   out.data_ptr(), srt.tokens, srt.top_k, y.shape[1], _DT[y.dtype])
@@ -362,8 +367,8 @@ def unpermute_tokens_bwd(dout: torch.Tensor, y: torch.Tensor, srt: ExpertSort, g
         raise ValueError("dout and y must have the same dtype and width")
     nv.same_cuda_device(y, dout=dout)
     g = _gates_arg(gates, srt, y)
-    dy = torch.empty((n, y.shape[1]), dtype=y.dtype, device=y.device)
-    dgates = torch.empty((srt.tokens, srt.top_k), dtype=torch.float32, device=y.device)
+    dy = nv.contiguous_like(y)
+    dgates = torch.empty_like(g)
     if n:
         nv.launch("pkb_moe_unpermute_bwd", _UNPERMUTE_BWD, y, dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0), srt.slots.data_ptr(),
                   g.data_ptr(), _kept_ptr(srt), dy.data_ptr(), dgates.data_ptr(), srt.tokens, srt.top_k, y.shape[1], _DT[y.dtype])

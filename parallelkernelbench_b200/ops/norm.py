@@ -60,12 +60,16 @@ def _ln_check(x: torch.Tensor, gamma, beta=None) -> int:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("layer norm needs at least one column")
     cols = x.shape[-1]
+    if not x.is_cuda:
+        raise ValueError("expected CUDA tensors")
     for name, p in (("gamma", gamma), ("beta", beta)):
-        if p is not None and (p.dtype not in _DT or p.numel() != cols or not p.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous bf16 or fp32 with {cols} values")
+        if p is not None:
+            if p.dtype not in _DT or p.numel() != cols or not p.is_contiguous():
+                raise ValueError(f"{name} must be contiguous bf16 or fp32 with {cols} values")
+            if p.get_device() != x.get_device():
+                raise ValueError(f"{name} is on {p.device}, not on {x.device}")
     if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
         raise TypeError("gamma and beta must have the same dtype")
-    nv.same_cuda_device(x, gamma=gamma, beta=beta)
     return cols
 
 
@@ -73,8 +77,8 @@ def _ln_forward(x, gamma, beta, eps, stats: bool):
     cols = _ln_check(x, gamma, beta)
     x2 = _rows_of(x, cols)
     rows = x2.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if stats else None
+    y = nv.contiguous_like(x)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32) if stats else None
     rstd = torch.empty_like(mean) if stats else None
     if rows:
         param = gamma if gamma is not None else beta
@@ -107,13 +111,13 @@ def layer_norm_bwd(x: torch.Tensor, gamma: torch.Tensor | None, dy: torch.Tensor
     nv.same_cuda_device(x, dy=dy, mean=mean, rstd=rstd)
     x2, dy2 = _rows_of(x, cols), _rows_of(dy, cols)
     rows = x2.shape[0]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = nv.contiguous_like(x)
     if not rows:
-        zero = torch.zeros((2, cols), dtype=torch.float32, device=x.device)
-        return dx, zero[0], zero[1]
-    dgamma, dbeta = (torch.empty(cols, dtype=torch.float32, device=x.device) for _ in range(2))
+        return dx, x.new_zeros(cols, dtype=torch.float32), x.new_zeros(cols, dtype=torch.float32)
+    dgamma = x.new_empty(cols, dtype=torch.float32)
+    dbeta = torch.empty_like(dgamma)
     blocks = nv.bound("pkb_layer_norm_bwd_partials", [_LL, _I, _I])(rows, cols, _DT[x.dtype])
-    part = torch.empty((blocks, 2, cols), dtype=torch.float32, device=x.device)
+    part = x.new_empty((blocks, 2, cols), dtype=torch.float32)
     nv.launch("pkb_layer_norm_bwd", _LN_BWD, x, x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), 0 if gamma is None else gamma.data_ptr(),
               0 if gamma is None else _DT[gamma.dtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(),
               part.data_ptr(), rows, cols, _DT[x.dtype], launches=2)
