@@ -417,26 +417,31 @@ __device__ __forceinline__ void ln_ring_abandon() {
 
 // PER: values per thread; with 16 the gain and bias are held in registers, with 32 they are read again for every row. (Read for every row, from
 // an L1 that the ring leaves little of, fp32 gains are twice the traffic of the rows: 8192 x 4096 took 40 us.)
-template <typename T, int NT, int PER>
+// R rows at a time share the two barriers of their sums: with one, the latency of shuffles, shared memory and barriers left the schedulers idle
+// for 56 % of the time (16384 x 8192: 116 us).
+template <typename T, int NT, int PER, int R>
 __global__ void __launch_bounds__(NT, 512 / NT)
 ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, const LnParam beta, T* __restrict__ y,
                    float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, int cols, float eps, int stages, uint32_t* status) {
   constexpr int VEC = 16 / sizeof(T), CH = PER / VEC, P = VEC / 2;
   constexpr bool kHoldGain = PER <= 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float red[2][NT / 32];
+  __shared__ float red[2][R * (NT / 32)];
   __shared__ int abort_flag;
   const uint32_t bytes = (uint32_t)cols * sizeof(T);
-  const LnRing ring = ln_ring_init(smem, stages, bytes, &abort_flag);
+  const LnRing ring = ln_ring_init(smem, stages, R * bytes, &abort_flag);
   const int t = threadIdx.x;
   const float inv = 1.f / (float)cols;
-  auto issue = [&](long long row, int stage) {
-    mbar_expect_tx(ring.bars + 8 * stage, bytes);
-    bulk_load(ring.base + stage * bytes, x + row * ldx, bytes, ring.bars + 8 * stage);
+  const long long groups = (rows + R - 1) / R;        // of R rows, the last one maybe with fewer
+  auto issue = [&](long long grp, int stage) {
+    const uint32_t bar = ring.bars + 8 * stage;
+    const int here = (int)min((long long)R, rows - grp * R);
+    mbar_expect_tx(bar, here * bytes);
+    for (int i = 0; i < here; ++i) bulk_load(ring.base + (stage * R + i) * bytes, x + (grp * R + i) * ldx, bytes, bar);
   };
   if (t == 0)
     for (int i = 0; i < stages; ++i)
-      if (blockIdx.x + (long long)i * gridDim.x < rows) issue(blockIdx.x + (long long)i * gridDim.x, i);
+      if (blockIdx.x + (long long)i * gridDim.x < groups) issue(blockIdx.x + (long long)i * gridDim.x, i);
   F2 g[kHoldGain ? CH : 1][P], b[kHoldGain ? CH : 1][P];
   if constexpr (kHoldGain) {
 #pragma unroll
@@ -450,49 +455,59 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
   }
   int stage = 0;
   uint32_t parity = 0;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    if (!ln_ring_wait(ring, stage, parity, &abort_flag, status, row)) {
+  for (long long grp = blockIdx.x; grp < groups; grp += gridDim.x) {
+    if (!ln_ring_wait(ring, stage, parity, &abort_flag, status, grp)) {
       ln_ring_abandon();
       return;
     }
-    F2 v[CH][P], acc = 0;
-    float s[1], q[1];
+    const int here = R == 1 ? 1 : (int)min((long long)R, rows - grp * R);
+    F2 v[R][CH][P];
+    float s[R], q[R], rstd[R];
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch) {
-      const int c = (ch * NT + t) * VEC;
-      if (c < cols) {
-        ln_pairs<VEC>(ln_shared(ring.base + stage * bytes + c * (int)sizeof(T)), v[ch]);
+    for (int i = 0; i < R; ++i) {
+      F2 acc = 0;
 #pragma unroll
-        for (int j = 0; j < P; ++j) acc = add2(acc, v[ch][j]);
-      }
-    }
-    s[0] = f2_sum(acc);
-    team_sum<1, NT, NT>(s, red[0], 0);
-    if (t == 0 && row + (long long)stages * gridDim.x < rows) {
-      fence_proxy_async_smem();
-      issue(row + (long long)stages * gridDim.x, stage);
-    }
-    const float mean = s[0] * inv;
-    const F2 shift = f2(-mean);
-    acc = 0;
+      for (int ch = 0; ch < CH; ++ch) {
+        const int c = (ch * NT + t) * VEC;
+        if (c < cols) {       // (a row that is not there reads the stage's old bytes: they are not used)
+          ln_pairs<VEC>(ln_shared(ring.base + (stage * R + i) * bytes + c * (int)sizeof(T)), v[i][ch]);
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch) {
-      if ((ch * NT + t) * VEC < cols) {
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-          v[ch][j] = add2(v[ch][j], shift);
-          acc = fma2(v[ch][j], v[ch][j], acc);
+          for (int j = 0; j < P; ++j) acc = add2(acc, v[i][ch][j]);
         }
       }
+      s[i] = f2_sum(acc);
     }
-    q[0] = f2_sum(acc);
-    team_sum<1, NT, NT>(q, red[1], 0);
-    const float rstd = rsqrtf(q[0] * inv + eps);
-    if (t == 0 && mean_out != nullptr) {
-      mean_out[row] = mean;
-      rstd_out[row] = rstd;
+    team_sum<R, NT, NT>(s, red[0], 0);
+    if (t == 0 && grp + (long long)stages * gridDim.x < groups) {
+      fence_proxy_async_smem();
+      issue(grp + (long long)stages * gridDim.x, stage);
     }
-    const F2 r2 = f2(rstd);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      s[i] *= inv;
+      const F2 shift = f2(-s[i]);
+      F2 acc = 0;
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) {
+        if ((ch * NT + t) * VEC < cols) {
+#pragma unroll
+          for (int j = 0; j < P; ++j) {
+            v[i][ch][j] = add2(v[i][ch][j], shift);
+            acc = fma2(v[i][ch][j], v[i][ch][j], acc);
+          }
+        }
+      }
+      q[i] = f2_sum(acc);
+    }
+    team_sum<R, NT, NT>(q, red[1], 0);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      rstd[i] = rsqrtf(q[i] * inv + eps);
+      if (t == 0 && i < here && mean_out != nullptr) {
+        mean_out[grp * R + i] = s[i];
+        rstd_out[grp * R + i] = rstd[i];
+      }
+    }
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (ch * NT + t) * VEC;
@@ -503,8 +518,14 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
           ln_param_pairs<VEC>(beta, c, b[0]);
         }
 #pragma unroll
-        for (int j = 0; j < P; ++j) v[ch][j] = fma2(mul2(v[ch][j], r2), g[kAt * ch][j], b[kAt * ch][j]);
-        ln_store_pairs<T, VEC>(y + row * cols + c, v[ch]);
+        for (int i = 0; i < R; ++i) {
+          if (i < here) {
+            const F2 r2 = f2(rstd[i]);
+#pragma unroll
+            for (int j = 0; j < P; ++j) v[i][ch][j] = fma2(mul2(v[i][ch][j], r2), g[kAt * ch][j], b[kAt * ch][j]);
+            ln_store_pairs<T, VEC>(y + (grp * R + i) * cols + c, v[i][ch]);
+          }
+        }
       }
     }
     if (++stage == stages) {
@@ -735,7 +756,7 @@ int ln_fwd_team(const T* x, long long ldx, LnParam g, LnParam b, T* y, float* me
 // The ring takes over from 1025 columns on (a warp per row, as below, has enough rows in flight) where every block has more than two rows; its
 // rows must be whole multiples of 16 bytes, start on 16 bytes and fit 16384 columns (backward in fp32: 8192).
 struct LnRingPlan {
-  int threads, per, blocks, stages, smem;
+  int threads, per, together, blocks, stages, smem;
 };
 bool ln_ring_plan(LnRingPlan& r, long long rows, int cols, int esize, bool backward) {
   const int most = backward && esize == 4 ? 8192 : 16384;
@@ -744,11 +765,12 @@ bool ln_ring_plan(LnRingPlan& r, long long rows, int cols, int esize, bool backw
   r.threads = cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
   const int per_sm = 512 / r.threads;
   r.blocks = sm_count() * per_sm;
-  const int stage = cols * esize * (backward ? 2 : 1);
+  r.together = !backward && r.per == 16 ? 2 : 1;
+  const int stage = cols * esize * (backward ? 2 : r.together);
   r.stages = kLnRingBytes / per_sm / stage;
   if (r.stages > kLnStages) r.stages = kLnStages;
   r.smem = 128 + r.stages * stage;
-  return r.stages >= 2 && rows > 2ll * r.blocks;
+  return r.stages >= 2 && rows > 2ll * r.blocks * r.together;
 }
 
 template <typename T>
@@ -760,10 +782,10 @@ int ln_fwd_ring(const LnRingPlan& r, const T* x, long long ldx, LnParam g, LnPar
     PKB_CHECK_CUDA(cudaGetLastError());
     return kApiOk;
   };
-  if (r.threads == 128) return go(ln_fwd_ring_kernel<T, 128, 16>);
-  if (r.threads == 256) return go(ln_fwd_ring_kernel<T, 256, 16>);
-  if (r.per == 16) return go(ln_fwd_ring_kernel<T, 512, 16>);
-  return go(ln_fwd_ring_kernel<T, 512, 32>);
+  if (r.threads == 128) return go(ln_fwd_ring_kernel<T, 128, 16, 2>);
+  if (r.threads == 256) return go(ln_fwd_ring_kernel<T, 256, 16, 2>);
+  if (r.per == 16) return go(ln_fwd_ring_kernel<T, 512, 16, 2>);
+  return go(ln_fwd_ring_kernel<T, 512, 32, 1>);
 }
 
 template <typename T>

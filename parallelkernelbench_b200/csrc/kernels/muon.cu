@@ -111,6 +111,88 @@ __device__ __forceinline__ void ns_tile(int t, int num_m, int num_n, int& i, int
   }
 }
 
+// ---- four columns of a result row: what the step adds to the product, and where the sum goes ----
+// `at`: row in the stack of matrices, col: first of the four columns (a multiple of four, < p.cols). Rows of the scratch tensors are padded to
+// eights, so there four columns never leave a row.
+template <int EPI>
+__device__ __forceinline__ uint4 ns_fetch4(const NsParams& p, long long at, int col) {
+  if constexpr (EPI == kNsPoly) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p.a16 + at * p.pitch16 + col);
+    return make_uint4(u.x, u.y, 0u, 0u);
+  } else if constexpr (EPI != kNsGram) {
+    const U4 u = ld_global_v4(p.master + at * p.pitch_m + col);
+    return make_uint4(u.x, u.y, u.z, u.w);
+  } else {
+    return make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+template <int EPI>
+__device__ __forceinline__ void ns_apply4(const NsParams& p, const uint4& in, float (&v)[4]) {
+  if constexpr (EPI == kNsGram) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= p.alpha;
+  } else if constexpr (EPI == kNsPoly) {
+    const float2 f0 = unpack_half2(in.x), f1 = unpack_half2(in.y);
+    v[0] = fmaf(p.alpha, v[0], p.beta * f0.x);
+    v[1] = fmaf(p.alpha, v[1], p.beta * f0.y);
+    v[2] = fmaf(p.alpha, v[2], p.beta * f1.x);
+    v[3] = fmaf(p.alpha, v[3], p.beta * f1.y);
+  } else {
+    v[0] = fmaf(p.beta, __uint_as_float(in.x), v[0]);
+    v[1] = fmaf(p.beta, __uint_as_float(in.y), v[1]);
+    v[2] = fmaf(p.beta, __uint_as_float(in.z), v[2]);
+    v[3] = fmaf(p.beta, __uint_as_float(in.w), v[3]);
+  }
+}
+
+template <int EPI>
+__device__ __forceinline__ void ns_put4(const NsParams& p, long long at, int col, float (&v)[4]) {
+  if constexpr (EPI == kNsUpdate)
+    st_global_v4(p.master + at * p.pitch_m + col, U4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
+  if constexpr (EPI == kNsUpdate || EPI == kNsGram || EPI == kNsPoly)
+    *reinterpret_cast<uint2*>(p.out16 + at * p.pitch16 + col) = make_uint2(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]));
+  if constexpr (EPI == kNsResult) {
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.final_out) + at * p.cols + col;
+    if (p.vec_out) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(p.alpha * v[0], p.alpha * v[1]), pack_bf16x2(p.alpha * v[2], p.alpha * v[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < p.cols) dst[j] = __float2bfloat16_rn(p.alpha * v[j]);
+    }
+  }
+  if constexpr (EPI == kNsStep) {
+    float* dst = static_cast<float*>(p.final_out) + at * p.cols + col;
+    __nv_bfloat16* dst16 = p.p_bf16 != nullptr ? p.p_bf16 + at * p.cols + col : nullptr;
+    if (p.vec_out) {
+      const U4 u = ld_global_v4(dst);
+      const uint32_t old[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = fmaf(-p.alpha, v[j], p.decay * __uint_as_float(old[j]));
+      st_global_v4(dst, U4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
+      if (dst16 != nullptr) *reinterpret_cast<uint2*>(dst16) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < p.cols) {
+          const float np = fmaf(-p.alpha, v[j], p.decay * dst[j]);
+          dst[j] = np;
+          if (dst16 != nullptr) dst16[j] = __float2bfloat16_rn(np);
+        }
+    }
+  }
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ U4 ld_shared_v4(uint32_t a) {
+  U4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
 // Persistent GEMM on clusters of two CTAs, tiles of 256 x 256 (tcgen05.mma.cta_group::2, M = 256): warp 0 of both CTAs loads, warp 1 of
 // the leader issues the products into two accumulators in tensor memory, warps 2 to 9 of both CTAs turn the finished one into results
 // meanwhile. A_MN / B_MN: the operand is [K, rows] row-major and is described to the tensor core as MN-major.
@@ -264,24 +346,13 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       const int colh = tj * kNsTile + half * 128;
       const int rows_here = p.rows - row0;                     // may be <= 0
       const long long grow = (long long)b * p.rows + row0;     // first row in the stack of matrices
-      // the next chunk's M (four floats) or A (four halves) per row of the turned chunk; rows of the scratch tensors are padded to eights
+      // the next chunk's M (four floats) or A (four halves) per row of the turned chunk
       uint4 in[8];
       auto fetch = [&](int c) {
         const int col = colh + c * 32 + tcol;
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int r = trow + it * 4;
-          if (c < 4 && col < p.cols && r < rows_here) {
-            if constexpr (EPI == kNsPoly) {
-              const uint2 u = *reinterpret_cast<const uint2*>(p.a16 + (grow + r) * p.pitch16 + col);
-              in[it].x = u.x;
-              in[it].y = u.y;
-            } else if constexpr (EPI != kNsGram) {
-              const U4 u = ld_global_v4(p.master + (grow + r) * p.pitch_m + col);
-              in[it] = make_uint4(u.x, u.y, u.z, u.w);
-            }
-          }
-        }
+        for (int it = 0; it < 8; ++it)
+          if (c < 4 && col < p.cols && trow + it * 4 < rows_here) in[it] = ns_fetch4<EPI>(p, grow + trow + it * 4, col);
       };
       fetch(0);
       bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.wait_budget_ns);
@@ -300,34 +371,15 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * 256 + half * 128 + c * 32), r);
         tmem_ld_wait();
 #pragma unroll
-        for (int f = 0; f < 8; ++f)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + lane * 128u + ((f ^ (lane & 7)) << 4)), "r"(r[4 * f]), "r"(r[4 * f + 1]),
-                       "r"(r[4 * f + 2]), "r"(r[4 * f + 3])
-                       : "memory");
+        for (int f = 0; f < 8; ++f) st_shared_v4(stg + lane * 128u + ((f ^ (lane & 7)) << 4), r[4 * f], r[4 * f + 1], r[4 * f + 2], r[4 * f + 3]);
         __syncwarp();
         float v[8][4];
 #pragma unroll
         for (int it = 0; it < 8; ++it) {
           const int tr = trow + it * 4;
-          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(v[it][0]), "=f"(v[it][1]), "=f"(v[it][2]), "=f"(v[it][3])
-                       : "r"(stg + tr * 128u + (((lane & 7) ^ (tr & 7)) << 4))
-                       : "memory");
-          if constexpr (EPI == kNsGram) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[it][j] *= p.alpha;
-          } else if constexpr (EPI == kNsPoly) {
-            const float2 f0 = unpack_half2(in[it].x), f1 = unpack_half2(in[it].y);
-            v[it][0] = fmaf(p.alpha, v[it][0], p.beta * f0.x);
-            v[it][1] = fmaf(p.alpha, v[it][1], p.beta * f0.y);
-            v[it][2] = fmaf(p.alpha, v[it][2], p.beta * f1.x);
-            v[it][3] = fmaf(p.alpha, v[it][3], p.beta * f1.y);
-          } else {
-            v[it][0] = fmaf(p.beta, __uint_as_float(in[it].x), v[it][0]);
-            v[it][1] = fmaf(p.beta, __uint_as_float(in[it].y), v[it][1]);
-            v[it][2] = fmaf(p.beta, __uint_as_float(in[it].z), v[it][2]);
-            v[it][3] = fmaf(p.beta, __uint_as_float(in[it].w), v[it][3]);
-          }
+          const U4 u = ld_shared_v4(stg + tr * 128u + (((lane & 7) ^ (tr & 7)) << 4));
+          v[it][0] = __uint_as_float(u.x); v[it][1] = __uint_as_float(u.y); v[it][2] = __uint_as_float(u.z); v[it][3] = __uint_as_float(u.w);
+          ns_apply4<EPI>(p, in[it], v[it]);
         }
         fetch(c + 1);
         const int col = col0 + tcol;
@@ -340,17 +392,15 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 #pragma unroll
               for (int it = 0; it < 8; ++it) {
                 const int tr = trow + it * 4;
-                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(stg + tr * 128u + (((lane & 7) ^ (tr & 7)) << 4)), "f"(v[it][0]),
-                             "f"(v[it][1]), "f"(v[it][2]), "f"(v[it][3])
-                             : "memory");
+                st_shared_v4(stg + tr * 128u + (((lane & 7) ^ (tr & 7)) << 4), __float_as_uint(v[it][0]), __float_as_uint(v[it][1]),
+                             __float_as_uint(v[it][2]), __float_as_uint(v[it][3]));
               }
               __syncwarp();
 #pragma unroll
-              for (int f = 0; f < 8; ++f)
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(w[4 * f]), "=r"(w[4 * f + 1]), "=r"(w[4 * f + 2]), "=r"(w[4 * f + 3])
-                             : "r"(stg + lane * 128u + ((f ^ (lane & 7)) << 4))
-                             : "memory");
+              for (int f = 0; f < 8; ++f) {
+                const U4 u = ld_shared_v4(stg + lane * 128u + ((f ^ (lane & 7)) << 4));
+                w[4 * f] = u.x; w[4 * f + 1] = u.y; w[4 * f + 2] = u.z; w[4 * f + 3] = u.w;
+              }
             } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(p.alpha * __uint_as_float(r[j]));
@@ -364,46 +414,8 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           }
         }
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int tr = trow + it * 4;
-          if (col >= p.cols || tr >= rows_here) continue;
-          if constexpr (EPI == kNsUpdate)
-            st_global_v4(p.master + (grow + tr) * p.pitch_m + col,
-                         U4{__float_as_uint(v[it][0]), __float_as_uint(v[it][1]), __float_as_uint(v[it][2]), __float_as_uint(v[it][3])});
-          if constexpr (EPI == kNsUpdate || kSym)
-            *reinterpret_cast<uint2*>(p.out16 + (grow + tr) * p.pitch16 + col) = make_uint2(pack_half2(v[it][0], v[it][1]), pack_half2(v[it][2], v[it][3]));
-          if constexpr (EPI == kNsResult) {
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.final_out) + (grow + tr) * p.cols + col;
-            if (p.vec_out) {
-              *reinterpret_cast<uint2*>(dst) =
-                  make_uint2(pack_bf16x2(p.alpha * v[it][0], p.alpha * v[it][1]), pack_bf16x2(p.alpha * v[it][2], p.alpha * v[it][3]));
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (col + j < p.cols) dst[j] = __float2bfloat16_rn(p.alpha * v[it][j]);
-            }
-          }
-          if constexpr (EPI == kNsStep) {
-            float* dst = static_cast<float*>(p.final_out) + (grow + tr) * p.cols + col;
-            __nv_bfloat16* dst16 = p.p_bf16 != nullptr ? p.p_bf16 + (grow + tr) * p.cols + col : nullptr;
-            if (p.vec_out) {
-              const U4 u = ld_global_v4(dst);
-              const uint32_t old[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-              for (int j = 0; j < 4; ++j) v[it][j] = fmaf(-p.alpha, v[it][j], p.decay * __uint_as_float(old[j]));
-              st_global_v4(dst, U4{__float_as_uint(v[it][0]), __float_as_uint(v[it][1]), __float_as_uint(v[it][2]), __float_as_uint(v[it][3])});
-              if (dst16 != nullptr) *reinterpret_cast<uint2*>(dst16) = make_uint2(pack_bf16x2(v[it][0], v[it][1]), pack_bf16x2(v[it][2], v[it][3]));
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (col + j < p.cols) {
-                  const float np = fmaf(-p.alpha, v[it][j], p.decay * dst[j]);
-                  dst[j] = np;
-                  if (dst16 != nullptr) dst16[j] = __float2bfloat16_rn(np);
-                }
-            }
-          }
-        }
+        for (int it = 0; it < 8; ++it)
+          if (col < p.cols && trow + it * 4 < rows_here) ns_put4<EPI>(p, grow + trow + it * 4, col, v[it]);
       }
       tc_fence_before_sync();
       __syncwarp();
@@ -426,6 +438,201 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   if (warp == 1) {
     tc_fence_after_sync();
     tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ few tiles: one per cluster, K split over its CTAs
+// Where a product has too few 256 x 256 tiles to occupy the GPU, its time is the way through K on the few SMs that have work: a CTA takes
+// its 32 KB per 64 of K from L2 at about 0.27 us. Here a tile is 128 x 128 and belongs to a cluster of up to 16 CTAs that share its K range;
+// each puts its partial sums into its shared memory, and after a cluster barrier sums its share of the rows over all of them (distributed
+// shared memory, in the order of the CTAs) and finishes those rows. 333 x 1000, us per launch: Gram 9 -> 5, update 10 -> 6.
+constexpr int kSplitTile = 128;
+constexpr int kSplitStages = 4;
+constexpr int kSplitStageBytes = 2 * kNsOperandBytes;         // 128 rows of A, 128 of B
+constexpr int kSplitPartial = kSplitTile * kSplitTile * 4;
+constexpr int kSplitSmem = kSplitStages * kSplitStageBytes + kSplitPartial + 256 + 1024;
+constexpr int kSplitCluster = 16;
+
+template <bool A_MN, bool B_MN, int EPI>
+__global__ void __launch_bounds__(kNsThreads, 1)
+ns_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const NsParams p) {
+  constexpr bool kSym = EPI == kNsGram || EPI == kNsPoly;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t partial = smem_base + kSplitStages * kSplitStageBytes;
+  const uint32_t bar_base = partial + kSplitPartial;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (kSplitStages + s); };
+  const uint32_t done_bar = bar_base + 8u * 2 * kSplitStages;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem_gen + kSplitStages * kSplitStageBytes + kSplitPartial + 8 * (2 * kSplitStages + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ctas = (int)cluster_nctaid(), rank = (int)cluster_ctarank();
+  const int tile = (int)(blockIdx.x / ctas);
+  const int num_m = (p.rows + kSplitTile - 1) / kSplitTile, num_n = (p.cols + kSplitTile - 1) / kSplitTile;
+  const int per_matrix = kSym ? num_m * (num_m + 1) / 2 : num_m * num_n;
+  const int b = tile / per_matrix;
+  int ti, tj;
+  ns_tile<kSym>(tile - b * per_matrix, num_m, num_n, ti, tj);
+  const int row0 = ti * kSplitTile, col0 = tj * kSplitTile;
+  const int num_k = (p.K + kGemmBlockK - 1) / kGemmBlockK, share_k = (num_k + ctas - 1) / ctas;
+  const int kb0 = min(num_k, rank * share_k), kb1 = min(num_k, kb0 + share_k);     // may be empty
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < kSplitStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(done_bar, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_holder), 128);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_holder;
+  let_successor_launch();
+  wait_for_predecessor();
+
+  const int et = (int)threadIdx.x - 64;             // thread of the epilogue, < 0: not one
+  const int share = kSplitTile / ctas;              // rows that this CTA finishes: four columns of a row per thread and turn
+  uint4 in[16];
+  if (warp == 0) {
+    const uint32_t lead = elect_one() ? 1u : 0u;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_budget_ns)) {
+        if (lane == 0) record_status(p.status, kStatusMbarTimeout, kNsKernelId + 2, 0, stage, 11, tile);
+        break;
+      }
+      mbar_expect_tx_p(full_bar(stage), kSplitStageBytes, lead);
+      const uint32_t sa = smem_base + stage * kSplitStageBytes, sb = sa + kNsOperandBytes;
+      const int k0 = kb * kGemmBlockK;
+      if constexpr (A_MN) {
+        tma_load_3d_p(sa, &tmap_a, full_bar(stage), row0, k0, b, lead);
+        tma_load_3d_p(sa + 8192, &tmap_a, full_bar(stage), row0 + 64, k0, b, lead);
+      } else {
+        tma_load_3d_p(sa, &tmap_a, full_bar(stage), k0, row0, b, lead);
+      }
+      if constexpr (B_MN) {
+        tma_load_3d_p(sb, &tmap_b, full_bar(stage), col0, k0, b, lead);
+        tma_load_3d_p(sb + 8192, &tmap_b, full_bar(stage), col0 + 64, k0, b, lead);
+      } else {
+        tma_load_3d_p(sb, &tmap_b, full_bar(stage), k0, col0, b, lead);
+      }
+      if (++stage == kSplitStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t lead = elect_one() ? 1u : 0u;
+    constexpr uint32_t idesc = make_idesc(kSplitTile, kSplitTile, 0, 0, A_MN ? 1 : 0, B_MN ? 1 : 0);
+    const uint32_t a_lo0 = A_MN ? smem_desc_lo_mnmajor(smem_base, 8192u) : smem_desc_lo_kmajor(smem_base);
+    const uint32_t b_lo0 = B_MN ? smem_desc_lo_mnmajor(smem_base + kNsOperandBytes, 8192u) : smem_desc_lo_kmajor(smem_base + kNsOperandBytes);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait(full_bar(stage), phase, abort_flag, p.wait_budget_ns)) {
+        if (lane == 0) record_status(p.status, kStatusMbarTimeout, kNsKernelId + 2, 0, stage, 21, tile);
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t a_lo = a_lo0 + stage * (kSplitStageBytes >> 4), b_lo = b_lo0 + stage * (kSplitStageBytes >> 4);
+#pragma unroll
+      for (int k = 0; k < kGemmBlockK / 16; ++k)
+        umma_f16_ss_p(tmem, smem_desc_join(a_lo + (A_MN ? 128u : 2u) * k), smem_desc_join(b_lo + (B_MN ? 128u : 2u) * k), idesc,
+                      (kb != kb0 || k != 0) ? 1u : 0u, lead);
+      umma_commit_p(empty_bar(stage), lead);
+      if (++stage == kSplitStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (ok) umma_commit_p(done_bar, lead);
+  } else {
+    // what the step adds to this CTA's rows, fetched while the products run
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = rank * share + (et >> 5) + i * 8, col = col0 + lane * 4;
+      if (i * 8 + (et >> 5) < share && row0 + row < p.rows && col < p.cols) in[i] = ns_fetch4<EPI>(p, (long long)b * p.rows + row0 + row, col);
+    }
+    const int q = warp & 3, half = (warp - 2) >> 2, prow = q * 32 + lane;
+    if (kb0 < kb1) {
+      const bool ok = mbar_wait(done_bar, 0, abort_flag, p.wait_budget_ns);
+      if (!__all_sync(0xffffffffu, ok) && lane == 0) record_status(p.status, kStatusMbarTimeout, kNsKernelId + 2, 0, 0, 30, tile);
+      tc_fence_after_sync();
+    }
+#pragma unroll 1
+    for (int c = half * 64; c < half * 64 + 64; c += 32) {
+      uint32_t r[32];
+      if (kb0 < kb1) {
+        tmem_ld_32x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, r);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = 0u;
+      }
+#pragma unroll
+      for (int f = 0; f < 8; ++f)
+        st_shared_v4(partial + prow * 512u + ((((uint32_t)(c >> 2) + f) ^ (prow & 7)) << 4), r[4 * f], r[4 * f + 1], r[4 * f + 2], r[4 * f + 3]);
+    }
+    tc_fence_before_sync();
+  }
+  __syncwarp();
+  cluster_sync_all();
+  if (et >= 0) {
+    auto place = [&](int row, int f) { return partial + row * 512u + ((uint32_t)(f ^ (row & 7)) << 4); };
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i * 8 + (et >> 5) >= share) break;
+      const int row = rank * share + (et >> 5) + i * 8, col = col0 + lane * 4;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      float4 part[kSplitCluster];
+#pragma unroll
+      for (int c = 0; c < kSplitCluster; ++c)
+        if (c < ctas) part[c] = ld_shared_cluster_v4(mapa_shared(place(row, lane), (uint32_t)c));
+#pragma unroll
+      for (int c = 0; c < kSplitCluster; ++c) {
+        if (c < ctas) {
+          v[0] += part[c].x; v[1] += part[c].y; v[2] += part[c].z; v[3] += part[c].w;
+        }
+      }
+      ns_apply4<EPI>(p, in[i], v);
+      if (kSym && ti != tj)      // kept for the other triangle: nobody else reads this CTA's copy of its own rows
+        st_shared_v4(place(row, lane), __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      if (row0 + row < p.rows && col < p.cols) ns_put4<EPI>(p, (long long)b * p.rows + row0 + row, col, v);
+    }
+    if (kSym && ti != tj) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      for (int i = et; i < share * kSplitTile; i += 256) {
+        const int r = i % share, j = i / share, row = rank * share + r;
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(place(row, j >> 2) + (j & 3) * 4u) : "memory");
+        if (row0 + row < p.rows && col0 + j < p.cols) p.out16[((long long)b * p.rows + col0 + j) * p.pitch16 + row0 + row] = __float2half_rn(v);
+      }
+    }
+  }
+  if (*abort_flag) {      // copies and products in flight end before the memory that they use goes away
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  __syncwarp();
+  cluster_sync_all();     // nobody leaves while its partial sums may still be read
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 128);
   }
 }
 
@@ -606,14 +813,6 @@ struct NsSmallParams {
 // byte of value (row, col) in atoms of 64 columns with the 128-byte swizzle
 __device__ __forceinline__ uint32_t sw128_at(int row, int col) {
   return (uint32_t)(col >> 6) * 16384u + (uint32_t)row * 128u + ((((uint32_t)(col & 63) >> 3) ^ ((uint32_t)row & 7u)) << 4) + ((uint32_t)col & 7u) * 2u;
-}
-__device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-__device__ __forceinline__ U4 ld_shared_v4(uint32_t a) {
-  U4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
 }
 // eight values of row `row` from column `col` on (a multiple of eight) as fp16
 __device__ __forceinline__ void put8(uint32_t base, int row, int col, const float* v) {
@@ -933,31 +1132,57 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
   }
 }
 
+// cluster: CTAs of a cluster where the kernel does not fix them itself, else 0
 template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kern)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
+cudaError_t launch_dependent(void (*kern)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, int cluster, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// CTAs that share a tile of the split form, 0 where the pairs' form is taken: that one's tiles are four times as large, so it needs the GPU
+// filled, which 128 x 128 tiles in one wave say it is not.
+int split_ctas(long long tiles, int num_k) {
+  if (tiles > sm_count()) return 0;
+  // clusters of 16, 8, 4, 2 that are resident at once (a cluster stays inside a group of 16 to 20 SMs), and at least two blocks of K each
+  const struct { int ctas, resident; } sizes[] = {{16, 7}, {8, 15}, {4, 33}, {2, 74}};
+  for (const auto& z : sizes)
+    if (tiles <= z.resident && num_k >= 2 * z.ctas) return z.ctas;
+  return 1;
 }
 
 template <bool A_MN, bool B_MN, int EPI>
 int ns_gemm(const CUtensorMap& ta, const CUtensorMap& tb, NsParams p, cudaStream_t s) {
-  const long long num_m = (p.rows + kNsTile - 1) / kNsTile, num_n = (p.cols + kNsTile - 1) / kNsTile;
-  const long long tiles = (EPI == kNsGram || EPI == kNsPoly ? num_m * (num_m + 1) / 2 : num_m * num_n) * p.batch;
+  constexpr bool kSym = EPI == kNsGram || EPI == kNsPoly;
+  auto tiles_of = [&](int size) {
+    const long long num_m = (p.rows + size - 1) / size, num_n = (p.cols + size - 1) / size;
+    return (kSym ? num_m * (num_m + 1) / 2 : num_m * num_n) * p.batch;
+  };
+  const long long small_tiles = tiles_of(kSplitTile), tiles = tiles_of(kNsTile);
   PKB_CHECK_ARG(tiles < (1ll << 24), "too many tiles");
+  if (const int ctas = split_ctas(small_tiles, (p.K + kGemmBlockK - 1) / kGemmBlockK)) {
+    auto kern = ns_split_kernel<A_MN, B_MN, EPI>;
+    PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem));
+    PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    PKB_CHECK_CUDA(launch_dependent(kern, dim3((unsigned)(small_tiles * ctas)), kNsThreads, kSplitSmem, s, ctas, ta, tb, p));
+    return kApiOk;
+  }
   int ctas = sm_count() & ~1;
   if (ctas > 2 * tiles) ctas = (int)(2 * tiles);
   auto kern = ns_gemm_kernel<A_MN, B_MN, EPI>;
   PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem));
-  PKB_CHECK_CUDA(launch_dependent(kern, dim3((unsigned)ctas), kNsThreads, kNsSmem, s, ta, tb, p));
+  PKB_CHECK_CUDA(launch_dependent(kern, dim3((unsigned)ctas), kNsThreads, kNsSmem, s, 0, ta, tb, p));
   return kApiOk;
 }
 
@@ -1088,7 +1313,7 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
   else ns_norm_kernel<false><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
   PKB_CHECK_CUDA(cudaGetLastError());
   const int start_blocks = blocks_for((long long)rows * (pitch / 8), 1 << 20);
-  PKB_CHECK_CUDA(launch_dependent(ns_start_kernel, dim3((unsigned)start_blocks, (unsigned)batch), kNsPrepThreads, 0, s, in, rows, cols, (int)pitch,
+  PKB_CHECK_CUDA(launch_dependent(ns_start_kernel, dim3((unsigned)start_blocks, (unsigned)batch), kNsPrepThreads, 0, s, 0, in, rows, cols, (int)pitch,
                                   part, parts, eps, k, (int)(aligned && cols % 8 == 0), master, x[0]));
 
   // maps of X as an operand whose rows lie along K (boxes of 64 columns x 128 rows) and as one whose rows are K (64 x 64), and of A and B
