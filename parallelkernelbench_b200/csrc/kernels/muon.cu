@@ -453,6 +453,46 @@ constexpr int kSplitPartial = kSplitTile * kSplitTile * 4;
 constexpr int kSplitSmem = kSplitStages * kSplitStageBytes + kSplitPartial + 256 + 1024;
 constexpr int kSplitCluster = 16;
 
+constexpr int kSplitRows = kSplitTile / 8;        // rows of a tile per epilogue warp, over all CTAs of its cluster
+
+// The end of a tile on a cluster of S CTAs: this CTA's kSplitTile / S rows, a warp per row at a time, four columns per lane. All 16 reads of a
+// thread (its rows times S CTAs) are in flight before the first sum: one row after the other took 3.6 us.
+template <int EPI, int S>
+__device__ __forceinline__ void split_finish(const NsParams& p, uint32_t partial, int rank, int et, int b, int row0, int col0, bool mirror,
+                                             const uint4 (&in)[kSplitRows]) {
+  constexpr int kShare = kSplitTile / S, kTurns = kSplitRows / S;
+  const int lane = et & 31, col = col0 + lane * 4;
+  auto place = [&](int row, int f) { return partial + row * 512u + ((uint32_t)(f ^ (row & 7)) << 4); };
+  float4 part[kTurns][S];
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i)
+#pragma unroll
+    for (int c = 0; c < S; ++c) part[i][c] = ld_shared_cluster_v4(mapa_shared(place(rank * kShare + (et >> 5) + i * 8, lane), (uint32_t)c));
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int row = rank * kShare + (et >> 5) + i * 8;
+    float v[4] = {part[i][0].x, part[i][0].y, part[i][0].z, part[i][0].w};
+#pragma unroll
+    for (int c = 1; c < S; ++c) {
+      v[0] += part[i][c].x; v[1] += part[i][c].y; v[2] += part[i][c].z; v[3] += part[i][c].w;
+    }
+    ns_apply4<EPI>(p, in[i], v);
+    if (mirror)      // kept for the other triangle: nobody else reads this CTA's copy of its own rows
+      st_shared_v4(place(row, lane), __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    if (row0 + row < p.rows && col < p.cols) ns_put4<EPI>(p, (long long)b * p.rows + row0 + row, col, v);
+  }
+  if (mirror) {
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll 8
+    for (int i = et; i < kShare * kSplitTile; i += 256) {
+      const int r = i % kShare, j = i / kShare, row = rank * kShare + r;
+      float v;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(place(row, j >> 2) + (j & 3) * 4u) : "memory");
+      if (row0 + row < p.rows && col0 + j < p.cols) p.out16[((long long)b * p.rows + col0 + j) * p.pitch16 + row0 + row] = __float2half_rn(v);
+    }
+  }
+}
+
 template <bool A_MN, bool B_MN, int EPI>
 __global__ void __launch_bounds__(kNsThreads, 1)
 ns_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const NsParams p) {
@@ -499,12 +539,11 @@ ns_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_holder;
-  let_successor_launch();
   wait_for_predecessor();
 
   const int et = (int)threadIdx.x - 64;             // thread of the epilogue, < 0: not one
   const int share = kSplitTile / ctas;              // rows that this CTA finishes: four columns of a row per thread and turn
-  uint4 in[16];
+  uint4 in[kSplitRows];
   if (warp == 0) {
     const uint32_t lead = elect_one() ? 1u : 0u;
     int stage = 0;
@@ -564,7 +603,7 @@ ns_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   } else {
     // what the step adds to this CTA's rows, fetched while the products run
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < kSplitRows; ++i) {
       const int row = rank * share + (et >> 5) + i * 8, col = col0 + lane * 4;
       if (i * 8 + (et >> 5) < share && row0 + row < p.rows && col < p.cols) in[i] = ns_fetch4<EPI>(p, (long long)b * p.rows + row0 + row, col);
     }
@@ -593,37 +632,18 @@ ns_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   __syncwarp();
   cluster_sync_all();
   if (et >= 0) {
-    auto place = [&](int row, int f) { return partial + row * 512u + ((uint32_t)(f ^ (row & 7)) << 4); };
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (i * 8 + (et >> 5) >= share) break;
-      const int row = rank * share + (et >> 5) + i * 8, col = col0 + lane * 4;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      float4 part[kSplitCluster];
-#pragma unroll
-      for (int c = 0; c < kSplitCluster; ++c)
-        if (c < ctas) part[c] = ld_shared_cluster_v4(mapa_shared(place(row, lane), (uint32_t)c));
-#pragma unroll
-      for (int c = 0; c < kSplitCluster; ++c) {
-        if (c < ctas) {
-          v[0] += part[c].x; v[1] += part[c].y; v[2] += part[c].z; v[3] += part[c].w;
-        }
-      }
-      ns_apply4<EPI>(p, in[i], v);
-      if (kSym && ti != tj)      // kept for the other triangle: nobody else reads this CTA's copy of its own rows
-        st_shared_v4(place(row, lane), __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-      if (row0 + row < p.rows && col < p.cols) ns_put4<EPI>(p, (long long)b * p.rows + row0 + row, col, v);
-    }
-    if (kSym && ti != tj) {
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      for (int i = et; i < share * kSplitTile; i += 256) {
-        const int r = i % share, j = i / share, row = rank * share + r;
-        float v;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(place(row, j >> 2) + (j & 3) * 4u) : "memory");
-        if (row0 + row < p.rows && col0 + j < p.cols) p.out16[((long long)b * p.rows + col0 + j) * p.pitch16 + row0 + row] = __float2half_rn(v);
-      }
+    const bool mirror = kSym && ti != tj;
+    switch (ctas) {
+      case 1: split_finish<EPI, 1>(p, partial, rank, et, b, row0, col0, mirror, in); break;
+      case 2: split_finish<EPI, 2>(p, partial, rank, et, b, row0, col0, mirror, in); break;
+      case 4: split_finish<EPI, 4>(p, partial, rank, et, b, row0, col0, mirror, in); break;
+      case 8: split_finish<EPI, 8>(p, partial, rank, et, b, row0, col0, mirror, in); break;
+      default: split_finish<EPI, 16>(p, partial, rank, et, b, row0, col0, mirror, in); break;
     }
   }
+  // Only now: CTAs that wait for their predecessor from its first microsecond on slow its reads of shared memory across the cluster (1024 x 1024:
+  // 209 us a call against 180 with none).
+  let_successor_launch();
   if (*abort_flag) {      // copies and products in flight end before the memory that they use goes away
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
@@ -696,7 +716,6 @@ __global__ void __launch_bounds__(kNsPrepThreads)
 ns_norm_kernel(const NsInput in, long long numel, double* __restrict__ part) {
   __shared__ double red[kNsPrepThreads / 32];
   const long long base = (long long)blockIdx.y * numel;
-  let_successor_launch();
   double s = 0.0;
   if constexpr (VEC) {
     const long long step = (long long)gridDim.x * kNsPrepThreads * 8;
@@ -738,6 +757,7 @@ ns_norm_kernel(const NsInput in, long long numel, double* __restrict__ part) {
   }
   s = block_sum_double(s, red);
   if (threadIdx.x == 0) part[(long long)blockIdx.y * gridDim.x + blockIdx.x] = s;
+  let_successor_launch();
 }
 
 // M = k u / (|u| + eps) and its fp16 copy, rows padded to their pitch with zeros
@@ -746,7 +766,6 @@ ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* _
                 float* __restrict__ master, __half* __restrict__ x16) {
   __shared__ double red[kNsPrepThreads / 32];
   const long long b = blockIdx.y;
-  let_successor_launch();
   wait_for_predecessor();
   double sum = 0.0;
   for (int i = threadIdx.x; i < parts; i += kNsPrepThreads) sum += part[b * parts + i];
@@ -775,6 +794,7 @@ ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* _
     store8(master + dst, u);
     st_global_v4(x16 + dst, U4{pack_half2(u[0], u[1]), pack_half2(u[2], u[3]), pack_half2(u[4], u[5]), pack_half2(u[6], u[7])});
   }
+  let_successor_launch();
 }
 
 // ------------------------------------------------------------------------------------------------ a short side: one launch
