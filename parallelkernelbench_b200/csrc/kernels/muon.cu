@@ -674,6 +674,36 @@ struct NsInput {
 constexpr int kNsPrepThreads = 256;
 constexpr int kNsMaxParts = 1024;
 
+// u * inv in fp32 for any |u| and inv whose product is in range (either alone may be far from one): inv = m 2^q is taken apart, u is moved half of
+// the way by an exact power of two, and only the other factor rounds.
+struct NsScale {
+  float first, second;
+  __device__ __forceinline__ explicit NsScale(double inv) {
+    int q = 0;
+    const double m = frexp(inv, &q);
+    const int half = q / 2;
+    first = ldexpf(1.f, half);
+    second = ldexpf((float)m, q - half);
+  }
+  __device__ __forceinline__ float operator()(float u) const { return u * first * second; }
+};
+
+// The sum of eight squares as a 64-bit number, formed in fp32 relative to the power of two of the largest: one conversion per eight values.
+__device__ __forceinline__ double square_sum8(const float (&u)[8]) {
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(u[j]));
+  const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);       // (0 and denormal: 2^-126 will do)
+  const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float v = u[j] * down;
+    s = fmaf(v, v, s);
+  }
+  return (double)s * __longlong_as_double((long long)(1023 + 2 * e) << 52);
+}
+
 __device__ __forceinline__ double block_sum_double(double v, double* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -736,11 +766,10 @@ ns_norm_kernel(const NsInput in, long long numel, double* __restrict__ part) {
           for (int j = 0; j < 8; ++j) m[h][j] = fmaf(in.momentum, m[h][j], g[h][j]);
           store8(in.m + base + i + h * step, m[h]);
         }
+        float u[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const double u = in.use(g[h][j], m[h][j]);
-          s += u * u;
-        }
+        for (int j = 0; j < 8; ++j) u[j] = in.use(g[h][j], m[h][j]);
+        s += square_sum8(u);
       }
     }
   } else {
@@ -770,7 +799,7 @@ ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* _
   double sum = 0.0;
   for (int i = threadIdx.x; i < parts; i += kNsPrepThreads) sum += part[b * parts + i];
   sum = block_sum_double(sum, red);
-  const double inv = k / (sqrt(sum) + eps);
+  const NsScale scale(k / (sqrt(sum) + eps));
   const int vecs = pitch / 8;
   const long long total = (long long)rows * vecs, base = b * rows * cols;
   for (long long i = (long long)blockIdx.x * kNsPrepThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kNsPrepThreads) {
@@ -789,7 +818,7 @@ ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* _
       for (int j = 0; j < 8; ++j) u[j] = c + j < cols ? in.use(in.grad(at + j), in.m != nullptr ? in.m[at + j] : 0.f) : 0.f;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = (float)((double)u[j] * inv);
+    for (int j = 0; j < 8; ++j) u[j] = scale(u[j]);
     const long long dst = (b * rows + r) * pitch + c;
     store8(master + dst, u);
     st_global_v4(x16 + dst, U4{pack_half2(u[0], u[1]), pack_half2(u[2], u[3]), pack_half2(u[4], u[5]), pack_half2(u[6], u[7])});
@@ -800,9 +829,9 @@ ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* _
 // ------------------------------------------------------------------------------------------------ a short side: one launch
 // Matrices whose smaller side is at most 128 stay on the chip for the whole call: a cluster owns a matrix, each of its CTAs a slice of
 // S <= 256 along the longer side. The iterate is in tensor memory in fp32, its fp16 copy in shared memory, where the same bytes serve the
-// Gram product (K-major, over the slice) and the update (MN-major, the slice as columns). Only the Gram matrix crosses CTAs: each adds its
-// rows' share of all partial sums, in the order of the CTAs, and hands the rounded rows to all (distributed shared memory); the polynomial is
-// computed by every CTA for itself. What bounds it is latency: five rounds of three short products with two cluster barriers each.
+// Gram product (K-major, over the slice) and the update (MN-major, the slice as columns). Only the Gram matrix crosses CTAs, through scratch that
+// stays in L2: each writes its partial sums, adds its rows' share of all of them in the order of the CTAs, and reads the others' rounded rows; the
+// polynomial is computed by every CTA for itself. (Distributed shared memory moved the 92 KB per CTA at about 17 bytes a cycle: 4 to 9 us a step.) What bounds it is latency: five rounds of three short products with two cluster barriers each.
 constexpr int kSmallSide = 128;
 constexpr int kSmallSlice = 256;
 constexpr int kSmallCluster = 16;
@@ -810,8 +839,9 @@ constexpr int kSmallThreads = 256;
 constexpr int kSmallX = kSmallSlice / 64 * 16384;              // X16: atoms of 64 columns, 128 rows of 128 bytes
 constexpr int kSmallGram = kSmallSide * kSmallSide * 4;        // partial Gram sums, fp32
 constexpr int kSmallA = kSmallSide * kSmallSide * 2;           // A and B, fp16
-constexpr int kSmallSmem = kSmallX + kSmallGram + 2 * kSmallA + 1024;
-static_assert(kSmallGram + 2 * kSmallA >= kSmallSide * kSmallSlice * 4, "u is staged where the Gram matrices come later");
+constexpr int kSmallStage = kSmallSide * kSmallSlice * 4;      // u, fp32; A and B take its place
+constexpr int kSmallSmem = kSmallX + kSmallStage + 1024;
+static_assert(2 * kSmallA <= kSmallStage, "A and B lie where u was staged");
 
 constexpr int kSmallMaxSteps = 16;
 
@@ -826,9 +856,18 @@ struct NsSmallParams {
   float* p;
   __nv_bfloat16* p_bf16;
   float decay, scale;
+  float* gram;               // scratch where a matrix has several CTAs: their partial Gram sums, kSmallGram bytes per CTA
+  __half* rows;              // and the rounded Gram matrix, kSmallA bytes per matrix
   uint32_t* status;
   uint64_t wait_budget_ns;
 };
+
+// 16 bytes from L2: other SMs wrote them since this one may last have read the line
+__device__ __forceinline__ U4 ld_global_l2(const void* p) {
+  U4 v;
+  asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
 
 // byte of value (row, col) in atoms of 64 columns with the 128-byte swizzle
 __device__ __forceinline__ uint32_t sw128_at(int row, int col) {
@@ -848,8 +887,8 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_storage;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t x16 = smem_base, gram = x16 + kSmallX, a16 = gram + kSmallGram, b16 = a16 + kSmallA;
-  float* u_stage = reinterpret_cast<float*>(smem_raw + (gram - smem_u32(smem_raw)));
+  const uint32_t x16 = smem_base, a16 = x16 + kSmallX, b16 = a16 + kSmallA;
+  float* u_stage = reinterpret_cast<float*>(smem_raw + (a16 - smem_u32(smem_raw)));
   volatile int* abort_flag = &abort_storage;
   const uint32_t bar = smem_u32(&bar_storage);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -870,33 +909,54 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
     tmem_relinquish();
   }
 
-  // ---- u of this slice into shared memory (u_stage[c][r], columns of the staging swizzled so that neither side conflicts), its squares' sum
-  auto swz = [](int c) { return (c ^ (c >> 3)) & 31; };
+  // ---- u of this slice into shared memory, u_stage[c][r], and its squares' sum. The rows are swizzled by the column so that eight columns of a row
+  // (a wide matrix) as well as a column for all rows (the reader below) fall into different banks; a tall one has its rows side by side already.
+  auto swz = [&](int c) { return p.tall ? 0 : (c ^ (c >> 3)) & 31; };
   double sum = 0.0;
-  auto take = [&](int r, int c, float g, float m) {
-    const float u = p.in.use(g, m);
-    u_stage[c * kSmallSide + (r ^ swz(c))] = u;
-    sum += (double)u * (double)u;
-  };
-  if (!p.tall && p.vec_in) {
-    const int per_row = (width + 7) / 8, items = p.side * per_row;
-#pragma unroll 2
-    for (int i = threadIdx.x; i < items; i += kSmallThreads) {
-      const int r = i / per_row, c = (i - r * per_row) * 8;
-      const long long at = base + (long long)r * p.longer + c0 + c;
-      float g[8], m[8] = {};
-      load8(p.in, at, g);
-      if (p.in.m != nullptr) {
-        load8(p.in.m + at, m);
+  if (p.vec_in) {
+    // eight values per access, four accesses per tensor in flight
+    const int per = p.tall ? p.side / 8 : (width + 7) / 8, items = p.tall ? width * per : p.side * per;
+    auto where = [&](int i, int& r, int& c) {
+      const int o = i / per, w = (i - o * per) * 8;
+      r = p.tall ? w : o;
+      c = p.tall ? o : w;
+      return base + (p.tall ? (long long)(c0 + c) * p.side + r : (long long)r * p.longer + c0 + c);
+    };
+    for (int i0 = threadIdx.x; i0 < items; i0 += 4 * kSmallThreads) {
+      float g[4][8], m[4][8] = {};
+      int r, c;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m[j] = fmaf(p.in.momentum, m[j], g[j]);
-        store8(p.in.m + at, m);
+      for (int h = 0; h < 4; ++h) {
+        if (i0 + h * kSmallThreads < items) {
+          const long long at = where(i0 + h * kSmallThreads, r, c);
+          load8(p.in, at, g[h]);
+          if (p.in.m != nullptr) load8(p.in.m + at, m[h]);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) take(r, c + j, g[j], m[j]);
+      for (int h = 0; h < 4; ++h) {
+        if (i0 + h * kSmallThreads >= items) break;
+        const long long at = where(i0 + h * kSmallThreads, r, c);
+        if (p.in.m != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m[h][j] = fmaf(p.in.momentum, m[h][j], g[h][j]);
+          store8(p.in.m + at, m[h]);
+        }
+        float u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = p.in.use(g[h][j], m[h][j]);
+        sum += square_sum8(u);
+        if (p.tall) {
+          float4* dst = reinterpret_cast<float4*>(u_stage + c * kSmallSide + r);
+          dst[0] = make_float4(u[0], u[1], u[2], u[3]);
+          dst[1] = make_float4(u[4], u[5], u[6], u[7]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) u_stage[(c + j) * kSmallSide + (r ^ swz(c + j))] = u[j];
+        }
+      }
     }
   } else {
-    // a row of the slice is contiguous where the matrix is tall (its columns are the side), else the columns of a row
     const int inner = p.tall ? p.side : width, items = p.side * width;
 #pragma unroll 8
     for (int i = threadIdx.x; i < items; i += kSmallThreads) {
@@ -909,24 +969,28 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
         m = fmaf(p.in.momentum, p.in.m[at], g);
         p.in.m[at] = m;
       }
-      take(r, c, g, m);
+      const float u = p.in.use(g, m);
+      u_stage[c * kSmallSide + (r ^ swz(c))] = u;
+      sum += (double)u * (double)u;
     }
   }
   sum = block_sum_double(sum, red);
   if (ctas > 1) {
     if (threadIdx.x == 0) norm_part = sum;
     cluster_sync_all();
+    double part[kSmallCluster];          // all reads in flight before the first sum
+#pragma unroll
+    for (int c = 0; c < kSmallCluster; ++c)
+      if (c < ctas) asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(part[c]) : "r"(mapa_shared(smem_u32(&norm_part), (uint32_t)c)) : "memory");
     sum = 0.0;
-    for (int c = 0; c < ctas; ++c) {
-      double v;
-      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(mapa_shared(smem_u32(&norm_part), (uint32_t)c)) : "memory");
-      sum += v;
-    }
+#pragma unroll
+    for (int c = 0; c < kSmallCluster; ++c)
+      if (c < ctas) sum += part[c];
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const double inv = p.k / (sqrt(sum) + p.eps);
+  const NsScale scale(p.k / (sqrt(sum) + p.eps));
   const uint32_t tmem = tmem_holder, tm_acc = tmem + 256;
   // a warp's place in tensor memory: 32 rows, and half of the columns of what it walks
   const int q = warp & 3, half = warp >> 2, row = q * 32 + lane;
@@ -937,7 +1001,7 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
       const bool in = row < p.side && c + j < width;
-      v[j] = in ? (float)((double)u_stage[(c + j) * kSmallSide + (row ^ swz(c + j))] * inv) : 0.f;
+      v[j] = in ? scale(u_stage[(c + j) * kSmallSide + (row ^ swz(c + j))]) : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < 32; j += 8) put8(x16, row, c + j, v + j);
@@ -963,6 +1027,8 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
     tc_fence_after_sync();
   };
   const float alpha = (float)(1.0 / (p.k * p.k));
+  float* my_gram = p.gram + (matrix * ctas + rank) * (kSmallGram / 4);
+  __half* my_rows = p.rows + matrix * (kSmallA / 2);
   constexpr uint32_t kSquare = make_idesc(kSmallSide, kSmallSide, 0, 0, 0, 0);
   const uint32_t idesc_update = make_idesc(kSmallSide, (uint32_t)p.slice, 0, 0, 0, 1);
 #pragma unroll 1
@@ -985,9 +1051,10 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
       tmem_ld_32x32(tm_acc + lanes + c, r);
       tmem_ld_wait();
       if (ctas > 1) {
+        // four columns of all rows side by side: a warp writes 512 bytes, and a CTA's rows below are contiguous as well
 #pragma unroll
         for (int f = 0; f < 8; ++f)
-          st_shared_v4(gram + row * 512u + ((((uint32_t)(c >> 2) + f) ^ (row & 7)) << 4), r[4 * f], r[4 * f + 1], r[4 * f + 2], r[4 * f + 3]);
+          st_global_v4(my_gram + (((c >> 2) + f) * kSmallSide + row) * 4, U4{r[4 * f], r[4 * f + 1], r[4 * f + 2], r[4 * f + 3]});
       } else {
         float v[32];
 #pragma unroll
@@ -998,29 +1065,37 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
     }
     if (ctas > 1) {
       cluster_sync_all();
-      // this CTA's share of the rows: four columns per thread, from every CTA, to every CTA
-      for (int i = (int)threadIdx.x; i < 4096 / ctas; i += kSmallThreads) {
-        const int r = rank * (kSmallSide / ctas) + (i >> 5), f = i & 31;
-        const uint32_t src = gram + r * 512u + ((uint32_t)(f ^ (r & 7)) << 4);
-        float4 part[kSmallCluster];
+      // this CTA's share of the rows, summed over all CTAs: four columns per thread and turn, all reads of a turn in flight at once
+      const int share = kSmallSide / ctas;
+      for (int i = (int)threadIdx.x; i < share * 32; i += kSmallThreads) {
+        const int f = i / share, r = rank * share + i - f * share;
+        const float* src = p.gram + matrix * ctas * (kSmallGram / 4) + (f * kSmallSide + r) * 4;
+        U4 part[kSmallCluster];
 #pragma unroll
         for (int c = 0; c < kSmallCluster; ++c)
-          if (c < ctas) part[c] = ld_shared_cluster_v4(mapa_shared(src, (uint32_t)c));
-        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (c < ctas) part[c] = ld_global_l2(src + c * (kSmallGram / 4));
+        float t[4] = {};
 #pragma unroll
         for (int c = 0; c < kSmallCluster; ++c) {
           if (c < ctas) {
-            t.x += part[c].x; t.y += part[c].y; t.z += part[c].z; t.w += part[c].w;
+            t[0] += __uint_as_float(part[c].x); t[1] += __uint_as_float(part[c].y); t[2] += __uint_as_float(part[c].z); t[3] += __uint_as_float(part[c].w);
           }
         }
-        const uint32_t lo = pack_half2(alpha * t.x, alpha * t.y), hi = pack_half2(alpha * t.z, alpha * t.w);
-        const uint32_t dst = a16 + sw128_at(r, f * 4);
-        for (int c = 0; c < ctas; ++c)
-          asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(mapa_shared(dst, (uint32_t)c)), "r"(lo), "r"(hi) : "memory");
+        *reinterpret_cast<uint2*>(my_rows + r * kSmallSide + f * 4) = make_uint2(pack_half2(alpha * t[0], alpha * t[1]), pack_half2(alpha * t[2], alpha * t[3]));
       }
-      fence_proxy_async_all();
-      tc_fence_before_sync();
       cluster_sync_all();
+      // all rows
+      U4 got[8];
+#pragma unroll
+      for (int h = 0; h < 8; ++h) got[h] = ld_global_l2(my_rows + (h * kSmallThreads + threadIdx.x) * 8);
+#pragma unroll
+      for (int h = 0; h < 8; ++h) {
+        const int i = h * kSmallThreads + (int)threadIdx.x;
+        st_shared_v4(a16 + sw128_at(i >> 4, (i & 15) * 8), got[h].x, got[h].y, got[h].z, got[h].w);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before_sync();
+      __syncthreads();
     } else {
       fence_proxy_async_smem();
       tc_fence_before_sync();
@@ -1029,7 +1104,6 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
     // ---- A A, and B = b A + c A A
     if (warp == 0) {
       const uint32_t lead = elect_one() ? 1u : 0u;
-      fence_proxy_async_all();
       tc_fence_after_sync();
 #pragma unroll
       for (int kk = 0; kk < kSmallSide / 16; ++kk) {
@@ -1262,9 +1336,12 @@ using namespace pkb;
 // bytes of scratch that pkb_newton_schulz wants (0: none) and, in *launches, the kernels that it launches
 extern "C" long long pkb_newton_schulz_scratch(long long batch, int rows, int cols, int steps, int* launches) {
   if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
-  const bool small = small_fits(rows < cols ? rows : cols, rows < cols ? cols : rows, steps);
+  const int side = rows < cols ? rows : cols, longer = rows < cols ? cols : rows;
+  const bool small = small_fits(side, longer, steps);
   if (launches != nullptr) *launches = small ? 1 : 2 + 3 * steps;
-  return small ? 0 : NsScratch(batch, rows, cols).total;
+  if (!small) return NsScratch(batch, rows, cols).total;
+  const int cluster = small_cluster(batch, longer);
+  return cluster > 1 ? batch * ((long long)cluster * kSmallGram + kSmallA) : 0;
 }
 
 // Orthogonalises `batch` matrices [rows, cols] u (see NsInput: g bf16 or fp32, with the momentum m fp32 updated in place where it is not null).
@@ -1309,6 +1386,11 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
     q.p_bf16 = static_cast<__nv_bfloat16*>(p_bf16);
     q.decay = decay;
     q.scale = (float)((p == nullptr ? 1.0 : (double)scale) / k);
+    if (cluster > 1) {
+      PKB_CHECK_ARG(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 255) == 0, "scratch must start on 256 bytes");
+      q.gram = static_cast<float*>(scratch);
+      q.rows = reinterpret_cast<__half*>(static_cast<uint8_t*>(scratch) + batch * cluster * kSmallGram);
+    }
     q.status = status;
     q.wait_budget_ns = kDefaultWaitBudgetNs;
     return launch_small(q, cluster, batch, s);
