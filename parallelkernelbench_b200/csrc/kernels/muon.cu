@@ -831,7 +831,8 @@ ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* _
 // S <= 256 along the longer side. The iterate is in tensor memory in fp32, its fp16 copy in shared memory, where the same bytes serve the
 // Gram product (K-major, over the slice) and the update (MN-major, the slice as columns). Only the Gram matrix crosses CTAs, through scratch that
 // stays in L2: each writes its partial sums, adds its rows' share of all of them in the order of the CTAs, and reads the others' rounded rows; the
-// polynomial is computed by every CTA for itself. (Distributed shared memory moved the 92 KB per CTA at about 17 bytes a cycle: 4 to 9 us a step.) What bounds it is latency: five rounds of three short products with two cluster barriers each.
+// polynomial is computed by every CTA for itself. B is kept as two fp16 numbers, which costs one more product: its rounding is the largest part of
+// the error where the side is short (64 x 2048: 1.7e-3 off 64 bits with one, 1.2e-3 with two). (Distributed shared memory moved the 92 KB per CTA at about 17 bytes a cycle: 4 to 9 us a step.) What bounds it is latency: five rounds of three short products with two cluster barriers each.
 constexpr int kSmallSide = 128;
 constexpr int kSmallSlice = 256;
 constexpr int kSmallCluster = 16;
@@ -841,7 +842,7 @@ constexpr int kSmallGram = kSmallSide * kSmallSide * 4;        // partial Gram s
 constexpr int kSmallA = kSmallSide * kSmallSide * 2;           // A and B, fp16
 constexpr int kSmallStage = kSmallSide * kSmallSlice * 4;      // u, fp32; A and B take its place
 constexpr int kSmallSmem = kSmallX + kSmallStage + 1024;
-static_assert(2 * kSmallA <= kSmallStage, "A and B lie where u was staged");
+static_assert(3 * kSmallA <= kSmallStage, "A and B lie where u was staged");
 
 constexpr int kSmallMaxSteps = 16;
 
@@ -887,7 +888,7 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_storage;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t x16 = smem_base, a16 = x16 + kSmallX, b16 = a16 + kSmallA;
+  const uint32_t x16 = smem_base, a16 = x16 + kSmallX, b16 = a16 + kSmallA, b16_low = b16 + kSmallA;
   float* u_stage = reinterpret_cast<float*>(smem_raw + (a16 - smem_u32(smem_raw)));
   volatile int* abort_flag = &abort_storage;
   const uint32_t bar = smem_u32(&bar_storage);
@@ -1130,6 +1131,9 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
           v[j + 2 * h + 1] = fmaf(cc, __uint_as_float(r[j + 2 * h + 1]), b * f.y);
         }
         put8(b16, row, c + j, v + j);
+#pragma unroll
+        for (int h = 0; h < 8; ++h) v[j + h] -= __half2float(__float2half_rn(v[j + h]));
+        put8(b16_low, row, c + j, v + j);
       }
     }
     fence_proxy_async_smem();
@@ -1140,9 +1144,10 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
       const uint32_t lead = elect_one() ? 1u : 0u;
       tc_fence_after_sync();
 #pragma unroll
-      for (int kk = 0; kk < kSmallSide / 16; ++kk) {
-        const uint32_t alo = smem_desc_lo_kmajor(b16 + (kk >> 2) * 16384u) + (kk & 3) * 2u;
-        const uint32_t blo = smem_desc_lo_mnmajor(x16, 16384u) + kk * 128u;
+      for (int kk = 0; kk < 2 * kSmallSide / 16; ++kk) {
+        const int k = kk & 7;
+        const uint32_t alo = smem_desc_lo_kmajor((kk < 8 ? b16 : b16_low) + (k >> 2) * 16384u) + (k & 3) * 2u;
+        const uint32_t blo = smem_desc_lo_mnmajor(x16, 16384u) + k * 128u;
         umma_f16_ss_p(tm_acc, smem_desc_join(alo), smem_desc_join(blo), idesc_update, kk != 0 ? 1u : 0u, lead);
       }
       umma_commit_p(bar, lead);
