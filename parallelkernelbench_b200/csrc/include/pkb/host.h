@@ -8,6 +8,7 @@
 #include <stdio.h>
 
 #include <array>
+#include <atomic>
 #include <string>
 
 namespace pkb {
@@ -88,6 +89,21 @@ std::array<int, 9> resident_clusters(Kernel kern, int threads, int smem_bytes) {
     }
   }
   return t;
+}
+
+// Raises a kernel's limits on the current device: dynamic shared memory and, where asked for, clusters of more than eight CTAs. Once per
+// kernel and device: the two calls cost as much as a third of a launch.
+template <auto KERN>
+int prepare_kernel(int smem_bytes, bool large_clusters = false) {
+  static std::atomic<uint64_t> done{0};
+  int d = 0;
+  PKB_CHECK_CUDA(cudaGetDevice(&d));
+  const uint64_t bit = d < 64 ? 1ull << d : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return kApiOk;
+  PKB_CHECK_CUDA(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
+  if (large_clusters) PKB_CHECK_CUDA(cudaFuncSetAttribute(KERN, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return kApiOk;
 }
 
 }  // namespace pkb

@@ -755,6 +755,11 @@ int ln_fwd_team(const T* x, long long ldx, LnParam g, LnParam b, T* y, float* me
 
 // The ring takes over from 1025 columns on (a warp per row, as below, has enough rows in flight) where every block has more than two rows; its
 // rows must be whole multiples of 16 bytes, start on 16 bytes and fit 16384 columns (backward in fp32: 8192).
+template <auto KERN>
+struct KernelAt {
+  static constexpr auto value = KERN;
+};
+
 struct LnRingPlan {
   int threads, per, together, blocks, stages, smem;
 };
@@ -776,33 +781,35 @@ bool ln_ring_plan(LnRingPlan& r, long long rows, int cols, int esize, bool backw
 template <typename T>
 int ln_fwd_ring(const LnRingPlan& r, const T* x, long long ldx, LnParam g, LnParam b, T* y, float* mean, float* rstd, long long rows, int cols,
                 float eps, cudaStream_t s) {
-  auto go = [&](auto kern) -> int {
-    PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, r.smem));
+  auto go = [&](auto at) -> int {
+    constexpr auto kern = decltype(at)::value;
+    if (const int rc = prepare_kernel<kern>(128 + kLnRingBytes)) return rc;
     kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, r.stages, status_block_device_ptr());
     PKB_CHECK_CUDA(cudaGetLastError());
     return kApiOk;
   };
-  if (r.threads == 128) return go(ln_fwd_ring_kernel<T, 128, 16, 2>);
-  if (r.threads == 256) return go(ln_fwd_ring_kernel<T, 256, 16, 2>);
-  if (r.per == 16) return go(ln_fwd_ring_kernel<T, 512, 16, 2>);
-  return go(ln_fwd_ring_kernel<T, 512, 32, 1>);
+  if (r.threads == 128) return go(KernelAt<ln_fwd_ring_kernel<T, 128, 16, 2>>{});
+  if (r.threads == 256) return go(KernelAt<ln_fwd_ring_kernel<T, 256, 16, 2>>{});
+  if (r.per == 16) return go(KernelAt<ln_fwd_ring_kernel<T, 512, 16, 2>>{});
+  return go(KernelAt<ln_fwd_ring_kernel<T, 512, 32, 1>>{});
 }
 
 template <typename T>
 int ln_bwd_ring(const LnRingPlan& r, const T* x, long long ldx, const T* dy, long long lddy, LnParam g, const float* mean, const float* rstd,
                 T* dx, float* part, long long rows, int cols, cudaStream_t s) {
-  auto go = [&](auto kern) -> int {
-    PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, r.smem));
+  auto go = [&](auto at) -> int {
+    constexpr auto kern = decltype(at)::value;
+    if (const int rc = prepare_kernel<kern>(128 + kLnRingBytes)) return rc;
     kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, r.stages, status_block_device_ptr());
     PKB_CHECK_CUDA(cudaGetLastError());
     return kApiOk;
   };
-  if (r.threads == 128) return go(ln_bwd_ring_kernel<T, 128, 16>);
-  if (r.threads == 256) return go(ln_bwd_ring_kernel<T, 256, 16>);
+  if (r.threads == 128) return go(KernelAt<ln_bwd_ring_kernel<T, 128, 16>>{});
+  if (r.threads == 256) return go(KernelAt<ln_bwd_ring_kernel<T, 256, 16>>{});
   if constexpr (sizeof(T) == 2) {
-    if (r.per == 32) return go(ln_bwd_ring_kernel<T, 512, 32>);
+    if (r.per == 32) return go(KernelAt<ln_bwd_ring_kernel<T, 512, 32>>{});
   }
-  return go(ln_bwd_ring_kernel<T, 512, 16>);
+  return go(KernelAt<ln_bwd_ring_kernel<T, 512, 16>>{});
 }
 
 template <typename T, int VEC16>

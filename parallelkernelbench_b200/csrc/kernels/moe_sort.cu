@@ -417,8 +417,7 @@ extern "C" int pkb_moe_sort(const void* idx, long long n, int experts, void* off
   PKB_CHECK_ARG(experts >= 1 && experts <= kSortMaxExperts, "1 .. 1024 experts");
   const long long rounds = (n + 31) / 32;
   const int smem = (int)(rounds < kSortWarps ? rounds : kSortWarps) * experts * (int)sizeof(int);
-  PKB_CHECK_CUDA(cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  PKB_CHECK_CUDA(cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (const int rc = prepare_kernel<moe_sort_kernel>(kSortWarps * kSortMaxExperts * (int)sizeof(int), true)) return rc;
   const int ctas = n > 8192 ? kSortCluster : 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);

@@ -1271,17 +1271,14 @@ int ns_gemm(const CUtensorMap& ta, const CUtensorMap& tb, NsParams p, cudaStream
   const long long small_tiles = tiles_of(kSplitTile), tiles = tiles_of(kNsTile);
   PKB_CHECK_ARG(tiles < (1ll << 24), "too many tiles");
   if (const int ctas = split_ctas(small_tiles, (p.K + kGemmBlockK - 1) / kGemmBlockK)) {
-    auto kern = ns_split_kernel<A_MN, B_MN, EPI>;
-    PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem));
-    PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    PKB_CHECK_CUDA(launch_dependent(kern, dim3((unsigned)(small_tiles * ctas)), kNsThreads, kSplitSmem, s, ctas, ta, tb, p));
+    if (const int rc = prepare_kernel<ns_split_kernel<A_MN, B_MN, EPI>>(kSplitSmem, true)) return rc;
+    PKB_CHECK_CUDA(launch_dependent(ns_split_kernel<A_MN, B_MN, EPI>, dim3((unsigned)(small_tiles * ctas)), kNsThreads, kSplitSmem, s, ctas, ta, tb, p));
     return kApiOk;
   }
   int ctas = sm_count() & ~1;
   if (ctas > 2 * tiles) ctas = (int)(2 * tiles);
-  auto kern = ns_gemm_kernel<A_MN, B_MN, EPI>;
-  PKB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem));
-  PKB_CHECK_CUDA(launch_dependent(kern, dim3((unsigned)ctas), kNsThreads, kNsSmem, s, 0, ta, tb, p));
+  if (const int rc = prepare_kernel<ns_gemm_kernel<A_MN, B_MN, EPI>>(kNsSmem)) return rc;
+  PKB_CHECK_CUDA(launch_dependent(ns_gemm_kernel<A_MN, B_MN, EPI>, dim3((unsigned)ctas), kNsThreads, kNsSmem, s, 0, ta, tb, p));
   return kApiOk;
 }
 
@@ -1297,8 +1294,7 @@ int small_cluster(long long batch, int longer) {
 bool small_fits(int side, int longer, int steps) { return side <= kSmallSide && longer <= kSmallCluster * kSmallSlice && steps <= kSmallMaxSteps; }
 
 int launch_small(const NsSmallParams& p, int cluster, long long batch, cudaStream_t s) {
-  PKB_CHECK_CUDA(cudaFuncSetAttribute(ns_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallSmem));
-  PKB_CHECK_CUDA(cudaFuncSetAttribute(ns_small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (const int rc = prepare_kernel<ns_small_kernel>(kSmallSmem, true)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(batch * cluster));
   cfg.blockDim = dim3(kSmallThreads);

@@ -41,20 +41,27 @@ def _coefficients(coefficients, steps: int, longer: int):
     return (ctypes.c_float * len(flat))(*flat)
 
 
-def _launch(g, m, momentum, nesterov, steps, coefficients, eps, out, p, decay, scale, p_bf16) -> None:
-    rows, cols = g.shape[-2:]
-    batch = g.numel() // (rows * cols)
-    if batch > 65535:
-        raise ValueError("at most 65535 matrices at once")
-    if max(rows, cols) >= 1 << 24:
-        raise ValueError("sides of at most 2^24 - 1")
+def _check(g, steps, coefficients, eps):
+    """The coefficients as a C array (None for empty matrices); refuses what the kernels do not take."""
     if isinstance(coefficients, list) or (len(coefficients) and isinstance(coefficients[0], list)):
         coefficients = tuple(tuple(c) if isinstance(c, list) else c for c in coefficients)
     if not steps >= 1 or not eps >= 0:
         raise ValueError("at least one step, and eps >= 0")
     if not len(coefficients):
         raise ValueError("coefficients are one (a, b, c) or one per step")
-    coeff = _coefficients(coefficients, int(steps), max(rows, cols))
+    rows, cols = g.shape[-2:]
+    if not g.numel():
+        return None
+    if g.numel() // (rows * cols) > 65535:
+        raise ValueError("at most 65535 matrices at once")
+    if max(rows, cols) >= 1 << 24:
+        raise ValueError("sides of at most 2^24 - 1")
+    return _coefficients(coefficients, int(steps), max(rows, cols))
+
+
+def _launch(g, m, momentum, nesterov, steps, coeff, eps, out, p, decay, scale, p_bf16) -> None:
+    rows, cols = g.shape[-2:]
+    batch = g.numel() // (rows * cols)
     g = g.contiguous()
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     launches = _I()
@@ -67,16 +74,17 @@ def _launch(g, m, momentum, nesterov, steps, coefficients, eps, out, p, decay, s
 def newton_schulz(g: torch.Tensor, *, steps: int = 5, coefficients=FAST, eps: float = 1e-7) -> torch.Tensor:
     """Orthogonalises the matrices ``g`` (bf16 or fp32 ``[..., rows, cols]``, any sides): ``X = g / (|g|_F + eps)``, then ``steps`` times
     ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``. ``coefficients`` is one ``(a, b, c)`` or a sequence of one per step. Returns bf16 of the
-    same shape. The iterate is held in fp32 and multiplied in fp16 with fp32 sums. A matrix of zeros stays zero; one with a value that is not
+    same shape (at most 65535 matrices). The iterate is held in fp32 and multiplied in fp16 with fp32 sums. A matrix of zeros stays zero; one with a value that is not
     finite comes back as NaN, alone."""
     if g.dtype not in _DT:
         raise TypeError(f"newton_schulz takes bf16 or fp32, got {g.dtype}")
     if g.dim() < 2:
         raise ValueError("newton_schulz takes matrices [..., rows, cols]")
+    coeff = _check(g, steps, coefficients, eps)
     nv.same_cuda_device(g)
-    out = torch.empty(g.shape, dtype=torch.bfloat16, device=g.device)
+    out = g.new_empty(g.shape, dtype=torch.bfloat16)
     if g.numel():
-        _launch(g, None, 0.0, False, steps, coefficients, eps, out, None, 0.0, 0.0, None)
+        _launch(g, None, 0.0, False, steps, coeff, eps, out, None, 0.0, 0.0, None)
     return out
 
 
@@ -99,11 +107,12 @@ def muon_step(p: torch.Tensor, m: torch.Tensor, g: torch.Tensor, *, lr: float, m
         raise ValueError("p, m and g must be matrices [..., rows, cols] of one shape")
     if p_bf16 is not None and (p_bf16.dtype != torch.bfloat16 or p_bf16.shape != p.shape or not p_bf16.is_contiguous()):
         raise ValueError("p_bf16 must be contiguous bf16 of the shape of p")
+    coeff = _check(g, steps, coefficients, eps)
+    if p.numel() and len({p.data_ptr(), m.data_ptr(), g.data_ptr()}) < 3:
+        raise ValueError("p, m and g must be different tensors")
     nv.same_cuda_device(p, m=m, g=g, p_bf16=p_bf16)
     if not p.numel():
         return
-    if m.data_ptr() == p.data_ptr():
-        raise ValueError("p and m must be different tensors")
     if scale is None:
         scale = 0.2 * math.sqrt(max(p.shape[-2:]))
-    _launch(g, m, momentum, nesterov, steps, coefficients, eps, None, p, 1.0 - lr * weight_decay, lr * scale, p_bf16)
+    _launch(g, m, momentum, nesterov, steps, coeff, eps, None, p, 1.0 - lr * weight_decay, lr * scale, p_bf16)

@@ -7,6 +7,8 @@ reference/18_tp_rms_norm.py:9-19).
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _native as nv
@@ -60,8 +62,6 @@ def _ln_check(x: torch.Tensor, gamma, beta=None) -> int:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("layer norm needs at least one column")
     cols = x.shape[-1]
-    if not x.is_cuda:
-        raise ValueError("expected CUDA tensors")
     for name, p in (("gamma", gamma), ("beta", beta)):
         if p is not None:
             if p.dtype not in _DT or p.numel() != cols or not p.is_contiguous():
@@ -75,6 +75,10 @@ def _ln_check(x: torch.Tensor, gamma, beta=None) -> int:
 
 def _ln_forward(x, gamma, beta, eps, stats: bool):
     cols = _ln_check(x, gamma, beta)
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    if not x.is_cuda:
+        raise ValueError("expected CUDA tensors")
     x2 = _rows_of(x, cols)
     rows = x2.shape[0]
     y = nv.contiguous_like(x)
@@ -99,6 +103,12 @@ def layer_norm_fwd(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: tor
     return _ln_forward(x, gamma, beta, eps, True)
 
 
+@functools.lru_cache(maxsize=256)
+def _ln_partials(rows: int, cols: int, dtype: int, device: int) -> int:
+    with torch.cuda.device(device):
+        return nv.bound("pkb_layer_norm_bwd_partials", [_LL, _I, _I])(rows, cols, dtype)
+
+
 def layer_norm_bwd(x: torch.Tensor, gamma: torch.Tensor | None, dy: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor):
     """Backward of :func:`layer_norm_fwd`: ``(dx, dgamma, dbeta)``, ``dx`` in the type of ``x``, the weight gradients fp32 ``[cols]``
     (what a gain of 1 or a bias of 0 would get where there is none). Sums run in a fixed order: the same inputs give the same bits."""
@@ -116,8 +126,7 @@ def layer_norm_bwd(x: torch.Tensor, gamma: torch.Tensor | None, dy: torch.Tensor
         return dx, x.new_zeros(cols, dtype=torch.float32), x.new_zeros(cols, dtype=torch.float32)
     dgamma = x.new_empty(cols, dtype=torch.float32)
     dbeta = torch.empty_like(dgamma)
-    blocks = nv.bound("pkb_layer_norm_bwd_partials", [_LL, _I, _I])(rows, cols, _DT[x.dtype])
-    part = x.new_empty((blocks, 2, cols), dtype=torch.float32)
+    part = x.new_empty((_ln_partials(rows, cols, _DT[x.dtype], x.get_device()), 2, cols), dtype=torch.float32)
     nv.launch("pkb_layer_norm_bwd", _LN_BWD, x, x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), 0 if gamma is None else gamma.data_ptr(),
               0 if gamma is None else _DT[gamma.dtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(),
               part.data_ptr(), rows, cols, _DT[x.dtype], launches=2)
