@@ -28,6 +28,26 @@ __device__ __forceinline__ void ln_load(const T* p, float (&f)[VEC]) {
   }
 }
 
+// the same access as it is, for rows on their way
+template <typename T, int VEC>
+struct LnRaw {
+  typename std::conditional<VEC == 1, T, U4>::type u;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC == 1) u = *p;
+    else u = ld_global_nc_v4(p);
+  }
+  __device__ __forceinline__ void unpack(float (&f)[VEC]) const {
+    if constexpr (VEC == 1) {
+      f[0] = static_cast<float>(u);
+    } else if constexpr (VEC == 8) {
+      const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
+      f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+    } else {
+      f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+    }
+  }
+};
+
 template <typename T, int VEC>
 __device__ __forceinline__ void ln_store(T* p, const float (&f)[VEC]) {
   if constexpr (VEC == 8)
@@ -222,15 +242,15 @@ ln_bwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ dy, 
     const int c = (ch * TPR + t) * VEC;
     if (c < cols) gamma.template load<VEC>(c, g[ch]);
   }
-  float xn[CH][VEC], dn[CH][VEC];
+  LnRaw<T, VEC> xn[CH], dn[CH];
   float mean_n = 0.f, rstd_n = 0.f;
   auto fetch = [&](long long row) {
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (ch * TPR + t) * VEC;
       if (c < cols) {
-        ln_load<T, VEC>(x + row * ldx + c, xn[ch]);
-        ln_load<T, VEC>(dy + row * lddy + c, dn[ch]);
+        xn[ch].load(x + row * ldx + c);
+        dn[ch].load(dy + row * lddy + c);
       }
     }
     mean_n = mean_in[row];
@@ -243,12 +263,10 @@ ln_bwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ dy, 
     float xv[CH][VEC], dv[CH][VEC];
     const float mean = mean_n, rstd = rstd_n;
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        xv[ch][j] = xn[ch][j];
-        dv[ch][j] = dn[ch][j];
-      }
+    for (int ch = 0; ch < CH; ++ch) {
+      xn[ch].unpack(xv[ch]);
+      dn[ch].unpack(dv[ch]);
+    }
     if (row + step < rows) fetch(row + step);
     float s[2] = {0.f, 0.f};
 #pragma unroll
@@ -648,6 +666,291 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
   }
 }
 
+// ---- many wide rows that do not start on 16 bytes -------------------------------------------------
+// The same ring for rows of any width, pitch and address. A bulk copy moves whole 16-byte pieces, so a row comes with up to 15 bytes of its
+// neighbours on either side, and its values lie at their own address modulo 16. No piece is copied that reaches outside the tensor (from its first
+// row's first to its last row's last value): the few values that this leaves out, in the first and last row, are read where they are used.
+// A thread owns the columns t, t + NT, ...: 4- and 2-byte accesses of shared and global memory, 32 neighbours per warp. Against the team form,
+// which takes such rows straight from global memory, us forward / backward: 8192 x 4097 bf16 93 / 191 there.
+struct LnSpan {
+  uintptr_t first, last;          // the tensor's bytes
+  __device__ __forceinline__ LnSpan(const void* base, long long pitch_bytes, long long rows, uint32_t row_bytes)
+      : first(reinterpret_cast<uintptr_t>(base)), last(first + (rows - 1) * pitch_bytes + row_bytes) {}
+  // the part of a row's pieces that may be copied; `at`: the address that the stage's first byte stands for
+  __device__ __forceinline__ void pieces(uintptr_t row, uint32_t row_bytes, uintptr_t& at, uintptr_t& lo, uintptr_t& hi) const {
+    at = row & ~(uintptr_t)15;
+    lo = at < first ? at + 16 : at;
+    hi = (row + row_bytes + 15) & ~(uintptr_t)15;
+    if (hi > last) hi -= 16;
+  }
+};
+
+// one value at a shared-memory address
+template <typename T>
+__device__ __forceinline__ float odd_shared(uint32_t a) {
+  if constexpr (sizeof(T) == 2) {
+    uint16_t u;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(a) : "memory");
+    return __uint_as_float((uint32_t)u << 16);
+  } else {
+    float f;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+    return f;
+  }
+}
+
+// A row in its stage. Pair j of a thread is columns (2 j NT + t, (2 j + 1) NT + t), zero where there is no column.
+template <typename T, int NT>
+struct LnOddRow {
+  const T* global;                // the row
+  uint32_t shared;                // where its first value would be in the stage
+  int from, to;                   // columns that are there
+  __device__ __forceinline__ float one(int c) const { return c >= from && c < to ? odd_shared<T>(shared + c * (int)sizeof(T)) : static_cast<float>(global[c]); }
+  template <int P>
+  __device__ __forceinline__ void load(F2 (&v)[P], int cols) const {
+    const int t = threadIdx.x;
+    if (from == 0 && to >= cols) {          // all rows but the tensor's first and last
+      const uint32_t at = shared + t * (int)sizeof(T);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        float lo = 0.f, hi = 0.f;
+        if ((2 * j + 1) * NT <= cols || 2 * j * NT + t < cols) lo = odd_shared<T>(at + 2 * j * NT * (int)sizeof(T));
+        if ((2 * j + 2) * NT <= cols || (2 * j + 1) * NT + t < cols) hi = odd_shared<T>(at + (2 * j + 1) * NT * (int)sizeof(T));
+        v[j] = f2(lo, hi);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const int c0 = 2 * j * NT + t, c1 = c0 + NT;
+        v[j] = f2(c0 < cols ? one(c0) : 0.f, c1 < cols ? one(c1) : 0.f);
+      }
+    }
+  }
+};
+
+// the pairs of a row, rounded to its type
+template <typename T, int NT, int P>
+__device__ __forceinline__ void odd_store(T* row, int j, F2 v, int cols) {
+  const int t = threadIdx.x;
+  const float2 w = f2_split(v);
+  const float lo[1] = {w.x}, hi[1] = {w.y};
+  if ((2 * j + 1) * NT <= cols || 2 * j * NT + t < cols) ln_store<T, 1>(row + t + 2 * j * NT, lo);
+  if ((2 * j + 2) * NT <= cols || (2 * j + 1) * NT + t < cols) ln_store<T, 1>(row + t + (2 * j + 1) * NT, hi);
+}
+
+template <typename T>
+__device__ __forceinline__ void odd_issue(const LnSpan& span, const T* row, uint32_t row_bytes, uint32_t dst, uint32_t bar, uint32_t& bytes) {
+  uintptr_t at, lo, hi;
+  span.pieces(reinterpret_cast<uintptr_t>(row), row_bytes, at, lo, hi);
+  bytes = (uint32_t)(hi - lo);
+  bulk_load(dst + (uint32_t)(lo - at), reinterpret_cast<const void*>(lo), bytes, bar);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t odd_bytes(const LnSpan& span, const T* row, uint32_t row_bytes) {
+  uintptr_t at, lo, hi;
+  span.pieces(reinterpret_cast<uintptr_t>(row), row_bytes, at, lo, hi);
+  return (uint32_t)(hi - lo);
+}
+template <int NT, typename T>
+__device__ __forceinline__ LnOddRow<T, NT> odd_row(const LnSpan& span, const T* row, uint32_t row_bytes, uint32_t stage) {
+  uintptr_t at, lo, hi;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(row);
+  span.pieces(a, row_bytes, at, lo, hi);
+  return {row, stage + (uint32_t)(a - at), lo > a ? (int)((lo - a) / sizeof(T)) : 0, (int)((hi - a) / sizeof(T))};
+}
+
+template <typename T, int NT, int PER, int R>
+__global__ void __launch_bounds__(NT, 512 / NT)
+ln_fwd_odd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, const LnParam beta, T* __restrict__ y,
+                  float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, int cols, float eps, int stages, uint32_t row_stage,
+                  uint32_t* status) {
+  constexpr int P = PER / 2;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float red[2][R * (NT / 32)];
+  __shared__ int abort_flag;
+  const uint32_t bytes = (uint32_t)cols * sizeof(T);
+  const LnRing ring = ln_ring_init(smem, stages, R * row_stage, &abort_flag);
+  const LnSpan span(x, ldx * (long long)sizeof(T), rows, bytes);
+  const int t = threadIdx.x;
+  const float inv = 1.f / (float)cols;
+  const long long groups = (rows + R - 1) / R;
+  auto issue = [&](long long grp, int stage) {
+    const uint32_t bar = ring.bars + 8 * stage;
+    const int here = (int)min((long long)R, rows - grp * R);
+    uint32_t all = 0, one;
+    for (int i = 0; i < here; ++i) all += odd_bytes(span, x + (grp * R + i) * ldx, bytes);
+    mbar_expect_tx(bar, all);
+    for (int i = 0; i < here; ++i) odd_issue(span, x + (grp * R + i) * ldx, bytes, ring.base + (stage * R + i) * row_stage, bar, one);
+  };
+  if (t == 0)
+    for (int i = 0; i < stages; ++i)
+      if (blockIdx.x + (long long)i * gridDim.x < groups) issue(blockIdx.x + (long long)i * gridDim.x, i);
+  auto col = [&](int k) { return k * NT + t; };
+  auto gains = [&](const LnParam& p, int j) { return f2(col(2 * j) < cols ? p.at(col(2 * j)) : 0.f, col(2 * j + 1) < cols ? p.at(col(2 * j + 1)) : 0.f); };
+  F2 g[P], b[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    g[j] = gains(gamma, j);
+    b[j] = gains(beta, j);
+  }
+  int stage = 0;
+  uint32_t parity = 0;
+  for (long long grp = blockIdx.x; grp < groups; grp += gridDim.x) {
+    if (!ln_ring_wait(ring, stage, parity, &abort_flag, status, grp)) {
+      ln_ring_abandon();
+      return;
+    }
+    const int here = R == 1 ? 1 : (int)min((long long)R, rows - grp * R);
+    F2 v[R][P];
+    float s[R] = {}, q[R] = {}, rstd[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      F2 acc = 0;
+      if (i < here) {
+        odd_row<NT>(span, x + (grp * R + i) * ldx, bytes, ring.base + (stage * R + i) * row_stage).load(v[i], cols);
+#pragma unroll
+        for (int j = 0; j < P; ++j) acc = add2(acc, v[i][j]);
+      }
+      s[i] = f2_sum(acc);
+    }
+    team_sum<R, NT, NT>(s, red[0], 0);
+    if (t == 0 && grp + (long long)stages * gridDim.x < groups) {
+      fence_proxy_async_smem();
+      issue(grp + (long long)stages * gridDim.x, stage);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      s[i] *= inv;
+      const F2 shift = f2(-s[i]);
+      F2 acc = 0;
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        v[i][j] = add2(v[i][j], shift);
+        if ((2 * j + 2) * NT > cols) {        // columns that are not there count nothing
+          const float2 w = f2_split(v[i][j]);
+          v[i][j] = f2(col(2 * j) < cols ? w.x : 0.f, col(2 * j + 1) < cols ? w.y : 0.f);
+        }
+        acc = fma2(v[i][j], v[i][j], acc);
+      }
+      q[i] = f2_sum(acc);
+    }
+    team_sum<R, NT, NT>(q, red[1], 0);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (i >= here) break;
+      rstd[i] = rsqrtf(q[i] * inv + eps);
+      if (t == 0 && mean_out != nullptr) {
+        mean_out[grp * R + i] = s[i];
+        rstd_out[grp * R + i] = rstd[i];
+      }
+      const F2 r2 = f2(rstd[i]);
+      T* yr = y + (grp * R + i) * cols;
+#pragma unroll
+      for (int j = 0; j < P; ++j) odd_store<T, NT, P>(yr, j, fma2(mul2(v[i][j], r2), g[j], b[j]), cols);
+    }
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+}
+
+// Both passes over a row read it from its stage (the registers hold the weights' sums), which is therefore free only after the next row's barrier.
+template <typename T, int NT, int PER>
+__global__ void __launch_bounds__(NT, 512 / NT)
+ln_bwd_odd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ dy, long long lddy, const LnParam gamma,
+                  const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part,
+                  long long rows, int cols, int stages, uint32_t row_stage, uint32_t* status) {
+  constexpr int P = PER / 2;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float red[2][2 * (NT / 32)];
+  __shared__ int abort_flag;
+  const uint32_t bytes = (uint32_t)cols * sizeof(T);
+  const LnRing ring = ln_ring_init(smem, stages, 2 * row_stage, &abort_flag);
+  const LnSpan span_x(x, ldx * (long long)sizeof(T), rows, bytes), span_d(dy, lddy * (long long)sizeof(T), rows, bytes);
+  const int t = threadIdx.x;
+  const float inv = 1.f / (float)cols;
+  auto issue = [&](long long row, int stage) {
+    const uint32_t dst = ring.base + stage * 2 * row_stage, bar = ring.bars + 8 * stage;
+    uint32_t one;
+    mbar_expect_tx(bar, odd_bytes(span_x, x + row * ldx, bytes) + odd_bytes(span_d, dy + row * lddy, bytes));
+    odd_issue(span_x, x + row * ldx, bytes, dst, bar, one);
+    odd_issue(span_d, dy + row * lddy, bytes, dst + row_stage, bar, one);
+  };
+  if (t == 0)
+    for (int i = 0; i < stages; ++i)
+      if (blockIdx.x + (long long)i * gridDim.x < rows) issue(blockIdx.x + (long long)i * gridDim.x, i);
+  auto col = [&](int k) { return k * NT + t; };
+  auto gains = [&](int j) { return f2(col(2 * j) < cols ? gamma.at(col(2 * j)) : 0.f, col(2 * j + 1) < cols ? gamma.at(col(2 * j + 1)) : 0.f); };
+  F2 ag[P] = {}, ab[P] = {};
+  F2 g[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) g[j] = gains(j);
+  int stage = 0, before = -1, it = 0;
+  uint32_t parity = 0;
+  float mean_n = blockIdx.x < rows ? mean_in[blockIdx.x] : 0.f, rstd_n = blockIdx.x < rows ? rstd_in[blockIdx.x] : 0.f;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x, it ^= 1) {
+    const float mean = mean_n, rstd = rstd_n;
+    if (row + gridDim.x < rows) {
+      mean_n = mean_in[row + gridDim.x];
+      rstd_n = rstd_in[row + gridDim.x];
+    }
+    if (!ln_ring_wait(ring, stage, parity, &abort_flag, status, row)) {
+      ln_ring_abandon();
+      return;
+    }
+    const uint32_t at = ring.base + stage * 2 * row_stage;
+    const LnOddRow<T, NT> xr = odd_row<NT>(span_x, x + row * ldx, bytes, at), dr = odd_row<NT>(span_d, dy + row * lddy, bytes, at + row_stage);
+    const F2 shift = f2(-mean), r2 = f2(rstd);
+    F2 s1 = 0, s2 = 0, xv[P], dv[P];
+    xr.load(xv, cols);
+    dr.load(dv, cols);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      // (dy and the gain are zero where there is no column)
+      const F2 xh = mul2(add2(xv[j], shift), r2), gd = mul2(dv[j], g[j]);
+      ag[j] = fma2(dv[j], xh, ag[j]);
+      ab[j] = add2(dv[j], ab[j]);
+      s1 = add2(gd, s1);
+      s2 = fma2(gd, xh, s2);
+    }
+    float s[2] = {f2_sum(s1), f2_sum(s2)};
+    team_sum<2, NT, NT>(s, red[it], 0);
+    const long long ahead = row + (long long)(stages - 1) * gridDim.x;
+    if (t == 0 && before >= 0 && ahead < rows) {
+      fence_proxy_async_smem();
+      issue(ahead, before);
+    }
+    const F2 c1 = f2(-s[0] * inv * rstd), c2 = f2(-s[1] * inv * rstd);
+    T* out = dx + row * cols;
+    xr.load(xv, cols);
+    dr.load(dv, cols);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const F2 xh = mul2(add2(xv[j], shift), r2), gd = mul2(dv[j], g[j]);
+      odd_store<T, NT, P>(out, j, fma2(xh, c2, fma2(gd, r2, c1)), cols);
+    }
+    before = stage;
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+  float* out = part + (long long)blockIdx.x * 2 * cols;
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const float2 a = f2_split(ag[j]), b = f2_split(ab[j]);
+    if (col(2 * j) < cols) {
+      out[col(2 * j)] = a.x;
+      out[cols + col(2 * j)] = b.x;
+    }
+    if (col(2 * j + 1) < cols) {
+      out[col(2 * j + 1)] = a.y;
+      out[cols + col(2 * j + 1)] = b.y;
+    }
+  }
+}
+
 // dgamma, dbeta [2][cols] = sum over the blocks of part[block][2][cols]: 32 columns and 32 strands of blocks per thread block
 __global__ void __launch_bounds__(1024)
 ln_bwd_params_kernel(const float* __restrict__ part, int blocks, long long width, float* __restrict__ dgamma, float* __restrict__ dbeta, int cols) {
@@ -727,15 +1030,23 @@ constexpr int kLnTeamCols = 512 * 16;
 
 bool ln_aligned(const void* p, long long pitch_bytes) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)pitch_bytes) & 15) == 0; }
 
-template <typename F, typename T, int VEC>
+template <typename F, typename T, int VEC, bool BACKWARD>
 int ln_by_width(int cols, F&& f) {
-  // 16 values per thread: 2 (bf16), 4 (fp32) accesses of 16 bytes, or 16 single ones
+  // 16 values per thread, 2 (bf16) or 4 (fp32) accesses of 16 bytes or 16 single ones. Forward a warp takes rows of up to 1024 with twice as many;
+  // backward the sums for the weights leave no registers for that.
   constexpr int CH = 16 / VEC;
-  if (cols <= 32 * 16) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, CH>{});
-  if (cols <= 64 * 16) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, CH>{});
-  if (cols <= 128 * 16) return f(std::integral_constant<int, 128>{}, std::integral_constant<int, CH>{});
-  if (cols <= 256 * 16) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, CH>{});
-  return f(std::integral_constant<int, 512>{}, std::integral_constant<int, CH>{});
+  using One = std::integral_constant<int, CH>;
+  if (cols <= 32 * 16) return f(std::integral_constant<int, 32>{}, One{});
+  if constexpr (BACKWARD) {
+    if (cols <= 64 * 16) return f(std::integral_constant<int, 64>{}, One{});
+  } else if constexpr (VEC > 1) {
+    if (cols <= 32 * 32) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 2 * CH>{});
+  } else {
+    if (cols <= 64 * 16) return f(std::integral_constant<int, 64>{}, One{});
+  }
+  if (cols <= 128 * 16) return f(std::integral_constant<int, 128>{}, One{});
+  if (cols <= 256 * 16) return f(std::integral_constant<int, 256>{}, One{});
+  return f(std::integral_constant<int, 512>{}, One{});
 }
 
 template <typename T, int VEC>
@@ -750,28 +1061,30 @@ int ln_fwd_team(const T* x, long long ldx, LnParam g, LnParam b, T* y, float* me
     PKB_CHECK_CUDA(cudaGetLastError());
     return kApiOk;
   };
-  return ln_by_width<decltype(go)&, T, VEC>(cols, go);
+  return ln_by_width<decltype(go)&, T, VEC, false>(cols, go);
 }
 
-// The ring takes over from 1025 columns on (a warp per row, as below, has enough rows in flight) where every block has more than two rows; its
-// rows must be whole multiples of 16 bytes, start on 16 bytes and fit 16384 columns (backward in fp32: 8192).
+// The rings take over from 1025 columns on (teams of a warp have enough rows in flight) where every block has more than two rows: up to 16384
+// columns, up to 8192 backward in fp32 and where rows start anywhere (with 32 single values per thread 4096 x 15001 bf16 took 222 us forward and
+// 429 backward, the long form 212 and 231).
 template <auto KERN>
 struct KernelAt {
   static constexpr auto value = KERN;
 };
 
 struct LnRingPlan {
-  int threads, per, together, blocks, stages, smem;
+  int threads, per, together, blocks, stages, row_stage, smem;
 };
-bool ln_ring_plan(LnRingPlan& r, long long rows, int cols, int esize, bool backward) {
-  const int most = backward && esize == 4 ? 8192 : 16384;
-  if (cols <= 1024 || cols > most || cols * esize % 16 != 0) return false;
-  r.per = cols > 8192 ? 32 : 16;
+// aligned: rows are whole multiples of 16 bytes that start on 16 bytes
+bool ln_ring_plan(LnRingPlan& r, long long rows, int cols, int esize, bool backward, bool aligned) {
+  if (cols <= 1024 || cols > (!aligned || (backward && esize == 4) ? 8192 : 16384)) return false;
   r.threads = cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
+  r.per = cols > 8192 ? 32 : !aligned && cols <= 10 * r.threads ? 10 : 16;
   const int per_sm = 512 / r.threads;
   r.blocks = sm_count() * per_sm;
-  r.together = !backward && r.per == 16 ? 2 : 1;
-  const int stage = cols * esize * (backward ? 2 : r.together);
+  r.together = !backward && r.per <= 16 ? 2 : 1;
+  r.row_stage = aligned ? cols * esize : (cols * esize + 15) / 16 * 16 + 16;
+  const int stage = r.row_stage * (backward ? 2 : r.together);
   r.stages = kLnRingBytes / per_sm / stage;
   if (r.stages > kLnStages) r.stages = kLnStages;
   r.smem = 128 + r.stages * stage;
@@ -792,6 +1105,47 @@ int ln_fwd_ring(const LnRingPlan& r, const T* x, long long ldx, LnParam g, LnPar
   if (r.threads == 256) return go(KernelAt<ln_fwd_ring_kernel<T, 256, 16, 2>>{});
   if (r.per == 16) return go(KernelAt<ln_fwd_ring_kernel<T, 512, 16, 2>>{});
   return go(KernelAt<ln_fwd_ring_kernel<T, 512, 32, 1>>{});
+}
+
+template <typename T>
+int ln_fwd_odd(const LnRingPlan& r, const T* x, long long ldx, LnParam g, LnParam b, T* y, float* mean, float* rstd, long long rows, int cols,
+               float eps, cudaStream_t s) {
+  auto go = [&](auto at) -> int {
+    constexpr auto kern = decltype(at)::value;
+    if (const int rc = prepare_kernel<kern>(128 + kLnRingBytes)) return rc;
+    kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, r.stages, (uint32_t)r.row_stage, status_block_device_ptr());
+    PKB_CHECK_CUDA(cudaGetLastError());
+    return kApiOk;
+  };
+  if (r.per == 10) {
+    if (r.threads == 128) return go(KernelAt<ln_fwd_odd_kernel<T, 128, 10, 2>>{});
+    if (r.threads == 256) return go(KernelAt<ln_fwd_odd_kernel<T, 256, 10, 2>>{});
+    return go(KernelAt<ln_fwd_odd_kernel<T, 512, 10, 2>>{});
+  }
+  if (r.threads == 128) return go(KernelAt<ln_fwd_odd_kernel<T, 128, 16, 2>>{});
+  if (r.threads == 256) return go(KernelAt<ln_fwd_odd_kernel<T, 256, 16, 2>>{});
+  return go(KernelAt<ln_fwd_odd_kernel<T, 512, 16, 2>>{});
+}
+
+template <typename T>
+int ln_bwd_odd(const LnRingPlan& r, const T* x, long long ldx, const T* dy, long long lddy, LnParam g, const float* mean, const float* rstd,
+               T* dx, float* part, long long rows, int cols, cudaStream_t s) {
+  auto go = [&](auto at) -> int {
+    constexpr auto kern = decltype(at)::value;
+    if (const int rc = prepare_kernel<kern>(128 + kLnRingBytes)) return rc;
+    kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, r.stages, (uint32_t)r.row_stage,
+                                             status_block_device_ptr());
+    PKB_CHECK_CUDA(cudaGetLastError());
+    return kApiOk;
+  };
+  if (r.per == 10) {
+    if (r.threads == 128) return go(KernelAt<ln_bwd_odd_kernel<T, 128, 10>>{});
+    if (r.threads == 256) return go(KernelAt<ln_bwd_odd_kernel<T, 256, 10>>{});
+    return go(KernelAt<ln_bwd_odd_kernel<T, 512, 10>>{});
+  }
+  if (r.threads == 128) return go(KernelAt<ln_bwd_odd_kernel<T, 128, 16>>{});
+  if (r.threads == 256) return go(KernelAt<ln_bwd_odd_kernel<T, 256, 16>>{});
+  return go(KernelAt<ln_bwd_odd_kernel<T, 512, 16>>{});
 }
 
 template <typename T>
@@ -819,7 +1173,8 @@ int ln_fwd_any(const void* xv, long long ldx, LnParam g, LnParam b, void* yv, fl
   T* y = static_cast<T*>(yv);
   const bool vec = cols % VEC16 == 0 && ln_aligned(x, ldx * (long long)sizeof(T)) && ln_aligned(y, 0) && ln_aligned(g.p, 0) && ln_aligned(b.p, 0);
   LnRingPlan ring;
-  if (vec && ln_ring_plan(ring, rows, cols, sizeof(T), false)) return ln_fwd_ring<T>(ring, x, ldx, g, b, y, mean, rstd, rows, cols, eps, s);
+  if (vec && ln_ring_plan(ring, rows, cols, sizeof(T), false, true)) return ln_fwd_ring<T>(ring, x, ldx, g, b, y, mean, rstd, rows, cols, eps, s);
+  if (!vec && ln_ring_plan(ring, rows, cols, sizeof(T), false, false)) return ln_fwd_odd<T>(ring, x, ldx, g, b, y, mean, rstd, rows, cols, eps, s);
   if (cols > kLnTeamCols) {
     const long long most = (long long)sm_count() * 4;
     ln_fwd_long_kernel<T><<<(unsigned)(rows < most ? rows : most), kLnLongThreads, 0, s>>>(x, ldx, g, b, y, mean, rstd, rows, cols, eps);
@@ -838,7 +1193,7 @@ int ln_bwd_team(const T* x, long long ldx, const T* dy, long long lddy, LnParam 
     PKB_CHECK_CUDA(cudaGetLastError());
     return kApiOk;
   };
-  return ln_by_width<decltype(go)&, T, VEC>(cols, go);
+  return ln_by_width<decltype(go)&, T, VEC, true>(cols, go);
 }
 
 // blocks of the backward's team form (rows of a block at once, blocks per SM) or slices of its long form
@@ -859,9 +1214,13 @@ int ln_bwd_any(const void* xv, long long ldx, const void* dyv, long long lddy, L
   const bool vec = cols % VEC16 == 0 && ln_aligned(x, ldx * (long long)sizeof(T)) && ln_aligned(dy, lddy * (long long)sizeof(T)) &&
                    ln_aligned(dx, 0) && ln_aligned(g.p, 0) && ln_aligned(part, 0);
   LnRingPlan ring;
-  if (vec && ln_ring_plan(ring, rows, cols, sizeof(T), true)) {
+  if (vec && ln_ring_plan(ring, rows, cols, sizeof(T), true, true)) {
     blocks = ring.blocks;
     const int rc = ln_bwd_ring<T>(ring, x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, s);
+    if (rc) return rc;
+  } else if (ln_ring_plan(ring, rows, cols, sizeof(T), true, false)) {
+    blocks = ring.blocks;
+    const int rc = ln_bwd_odd<T>(ring, x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, s);
     if (rc) return rc;
   } else if (cols > kLnTeamCols) {
     const long long most = (long long)sm_count() * 4;
@@ -903,8 +1262,10 @@ extern "C" int pkb_layer_norm_fwd(const void* x, long long ldx, const void* gamm
 extern "C" int pkb_layer_norm_bwd_partials(long long rows, int cols, int dtype) {
   if (rows <= 0 || cols <= 0) return 0;
   LnRingPlan ring;
-  const int blocks = ln_bwd_blocks(rows, cols), in_ring = ln_ring_plan(ring, rows, cols, dtype ? 4 : 2, true) ? ring.blocks : 0;
-  return blocks > in_ring ? blocks : in_ring;
+  int blocks = ln_bwd_blocks(rows, cols);
+  for (const bool aligned : {true, false})
+    if (ln_ring_plan(ring, rows, cols, dtype ? 4 : 2, true, aligned) && ring.blocks > blocks) blocks = ring.blocks;
+  return blocks;
 }
 
 // dx [rows, cols] (contiguous, the type of x and dy), dgamma and dbeta fp32 [cols] from the saved statistics.

@@ -64,7 +64,9 @@ def _check(x, dy, gamma, beta, eps, got, stats=None, grads=None):
 SHAPES = [(1, 1), (3, 2), (1, 4096), (3, 7), (5, 8), (7, 512), (7, 513), (9, 520), (9, 1024), (2, 1032), (33, 2048), (3, 2056), (17, 4096), (5, 4097),
           (5, 4104), (3, 8192), (2, 8193), (3, 8200), (2, 20001), (300, 8200), (2500, 64), (1333, 1001), (9001, 33),
           # many wide rows (the ring): every width class, the last row of a round and one more, a row that is no multiple of a thread's access
-          (2400, 1032), (1185, 2048), (1400, 2056), (1184, 4096), (1185, 4096), (3000, 4104), (600, 8192), (700, 8200), (301, 16384), (400, 16392)]
+          (2400, 1032), (1185, 2048), (1400, 2056), (1184, 4096), (1185, 4096), (3000, 4104), (600, 8192), (700, 8200), (301, 16384), (400, 16392),
+          # the same of rows that start anywhere
+          (2400, 1025), (1300, 2047), (1400, 2049), (1301, 4095), (700, 4097), (400, 8191), (330, 8193), (310, 9001), (307, 12280), (303, 12290), (300, 16383)]
 
 
 @pytest.mark.parametrize("dtype,param", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32),
@@ -134,9 +136,11 @@ def test_layouts(view, dtype):
     _layouts(view, dtype, 24)
 
 
-@pytest.mark.parametrize("view", ["pitch", "odd_pitch", "expanded"])
-def test_layouts_of_many_wide_rows(view):
-    _layouts(view, torch.bfloat16, 1300, 4)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("view", ["offset", "pitch", "odd_pitch", "expanded", "odd_expanded", "overlapping"])
+def test_layouts_of_many_wide_rows(view, dtype):
+    """The first and last rows' ends are what copies of whole 16-byte pieces must not reach across."""
+    _layouts(view, dtype, 1300, 4)
 
 
 def _layouts(view, dtype, rows, times=1):
@@ -147,7 +151,7 @@ def _layouts(view, dtype, rows, times=1):
 
     def lay(t):
         if view == "offset":
-            return t.reshape(-1)[1:1 + 23 * n].view(23, n)
+            return t.reshape(-1)[1:1 + (rows - 1) * n].view(rows - 1, n)
         if view == "pitch":
             return t[:, :n]
         if view == "odd_pitch":
@@ -156,6 +160,10 @@ def _layouts(view, dtype, rows, times=1):
             return t[:, :n].reshape(2, 3, 4, n)
         if view == "transposed":
             return t[:, :n].t().contiguous().t()
+        if view == "odd_expanded":
+            return t[:1, 1:n + 1].expand(rows, n)
+        if view == "overlapping":
+            return t.reshape(-1)[3:].as_strided((rows, n), (5, 1), t.storage_offset() + 3)
         return t[:1, :n].expand(rows, n)
 
     xv, dyv, g, b = lay(x), lay(dy), gamma[:n], beta[:n]
