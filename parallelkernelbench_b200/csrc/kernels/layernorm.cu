@@ -60,6 +60,10 @@ __device__ __forceinline__ void ln_store(T* p, const float (&f)[VEC]) {
     *p = f[0];
 }
 
+// The weights' kernel is launched while the last blocks of the backward still run (programmatic dependent launch) and waits for all of them.
+__device__ __forceinline__ void ln_let_successor_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void ln_wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // gain or bias: bf16 or fp32 whatever the rows are, or absent
 struct LnParam {
   const void* p;
@@ -296,6 +300,7 @@ ln_bwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ dy, 
     }
   }
   // the teams' sums, added in the order of the teams
+  ln_let_successor_launch();
   float* out = part + (long long)blockIdx.x * 2 * cols;
   if constexpr (L::kRows == 1) {
 #pragma unroll
@@ -652,6 +657,7 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
       parity ^= 1u;
     }
   }
+  ln_let_successor_launch();
   float* out = part + (long long)blockIdx.x * 2 * cols;
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
@@ -936,6 +942,7 @@ ln_bwd_odd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ 
       parity ^= 1u;
     }
   }
+  ln_let_successor_launch();
   float* out = part + (long long)blockIdx.x * 2 * cols;
 #pragma unroll
   for (int j = 0; j < P; ++j) {
@@ -958,6 +965,7 @@ ln_bwd_params_kernel(const float* __restrict__ part, int blocks, long long width
   const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5;
   const long long i = (long long)blockIdx.x * 32 + lane;
   float a = 0.f;
+  ln_wait_for_predecessor();
   if (i < width) {
 #pragma unroll 8
     for (int b = strand; b < blocks; b += 32) a += part[b * width + i];
@@ -1233,8 +1241,16 @@ int ln_bwd_any(const void* xv, long long ldx, const void* dyv, long long lddy, L
     if (rc) return rc;
   }
   const long long width = 2ll * cols;
-  ln_bwd_params_kernel<<<(unsigned)((width + 31) / 32), 1024, 0, s>>>(part, blocks, width, dgamma, dbeta, cols);
-  PKB_CHECK_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((width + 31) / 32));
+  cfg.blockDim = dim3(1024);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, ln_bwd_params_kernel, (const float*)part, blocks, width, dgamma, dbeta, cols));
   return kApiOk;
 }
 

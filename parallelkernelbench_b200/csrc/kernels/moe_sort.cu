@@ -216,27 +216,29 @@ __device__ __forceinline__ void zero_rows(T* rows, long long n, int nvec, const 
   }
 }
 
-constexpr int kRowUnroll = 2;
+// accesses per thread of the permutation
+constexpr int row_unroll(int vec) { return vec == 1 ? 4 : 2; }
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kRowThreads)
 moe_permute_kernel(const T* __restrict__ x, long long ldx, const int* __restrict__ slots, const int* __restrict__ kept, T* __restrict__ xp,
                    long long tokens, int top_k, int nvec, const RowGrid grid) {
   using V = RowVec<T, VEC>;
+  constexpr int U = row_unroll(VEC);
   long long t;
   int first;
-  if (grid.place(tokens, t, first, kRowUnroll)) {
+  if (grid.place(tokens, t, first, U)) {
     const int team = 1 << grid.team_log2;
     const unsigned n = (unsigned)(tokens * top_k);
-    typename V::Raw v[kRowUnroll];
+    typename V::Raw v[U];
 #pragma unroll
-    for (int u = 0; u < kRowUnroll; ++u)
+    for (int u = 0; u < U; ++u)
       if (first + u * team < nvec) v[u] = V::load(x + t * ldx + (long long)(first + u * team) * VEC);
     for (int j = 0; j < top_k; ++j) {
       const unsigned s = (unsigned)slots[t * top_k + j];
       if (s < n) {
 #pragma unroll
-        for (int u = 0; u < kRowUnroll; ++u)
+        for (int u = 0; u < U; ++u)
           if (first + u * team < nvec) V::store(xp + ((long long)s * nvec + first + u * team) * VEC, v[u]);
       }
     }
@@ -246,42 +248,55 @@ moe_permute_kernel(const T* __restrict__ x, long long ldx, const int* __restrict
 
 // out[t] = sum_j gate[t, j] y[slots[t, j]]; GATED = false: weights of one. One access per row and thread, eight rows in flight: with two
 // accesses per row the registers left two blocks per SM, too few to cover the way from a slot to its row (8192 tokens x 7168, top-8: 210 us).
-constexpr int kGatherAhead = 8;   // rows whose loads are issued before the first of them is added
+constexpr int kGatherAhead = 8;   // accesses in flight per thread before the first of them is added
+// single values: four columns of two rows (four bytes per access of eight rows leave a warp with half a line each)
+constexpr int gather_unroll(int vec) { return vec == 1 ? 4 : 1; }
 
 template <typename T, int VEC, bool GATED>
 __global__ void __launch_bounds__(kRowThreads, 4)
 moe_unpermute_kernel(const T* __restrict__ y, long long ldy, const int* __restrict__ slots, const float* __restrict__ gates, T* __restrict__ out,
                      long long tokens, int top_k, int nvec, const RowGrid grid) {
   using V = RowVec<T, VEC>;
+  constexpr int U = gather_unroll(VEC), kAhead = kGatherAhead / U;
   long long t;
-  int i;
-  if (!grid.place(tokens, t, i) || i >= nvec) return;
+  int first;
+  if (!grid.place(tokens, t, first, U) || first >= nvec) return;
+  const int team = 1 << grid.team_log2;
   const unsigned n = (unsigned)(tokens * top_k);
-  const T* col = y + (long long)i * VEC;
-  float acc[VEC] = {};
-  for (int j0 = 0; j0 < top_k; j0 += kGatherAhead) {
-    typename V::Raw v[kGatherAhead];
-    unsigned s[kGatherAhead];
-    float g[kGatherAhead];
+  float acc[U][VEC] = {};
+  for (int j0 = 0; j0 < top_k; j0 += kAhead) {
+    typename V::Raw v[kAhead][U];
+    unsigned s[kAhead];
+    float g[kAhead];
 #pragma unroll
-    for (int a = 0; a < kGatherAhead; ++a) {
+    for (int a = 0; a < kAhead; ++a) {
       s[a] = j0 + a < top_k ? (unsigned)slots[t * top_k + j0 + a] : n;
       g[a] = GATED && j0 + a < top_k ? gates[t * top_k + j0 + a] : 1.f;
     }
 #pragma unroll
-    for (int a = 0; a < kGatherAhead; ++a)
-      if (s[a] < n) v[a] = V::load(col + (long long)s[a] * ldy);
-#pragma unroll
-    for (int a = 0; a < kGatherAhead; ++a) {
+    for (int a = 0; a < kAhead; ++a) {
       if (s[a] < n) {
-        float f[VEC];
-        V::unpack(v[a], f);
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) acc[c] += GATED ? g[a] * f[c] : f[c];
+        for (int u = 0; u < U; ++u)
+          if (U == 1 || first + u * team < nvec) v[a][u] = V::load(y + (long long)s[a] * ldy + (long long)(first + u * team) * VEC);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      if (s[a] < n) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float f[VEC];
+          V::unpack(v[a][u], f);
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) acc[u][c] += GATED ? g[a] * f[c] : f[c];
+        }
       }
     }
   }
-  V::store(out + (t * nvec + i) * VEC, V::pack(acc));
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (U == 1 || first + u * team < nvec) V::store(out + (t * nvec + first + u * team) * VEC, V::pack(acc[u]));
 }
 
 // A team of TEAM threads per token: dy rows and the dot products in one pass over dout and y.
@@ -309,24 +324,35 @@ moe_unpermute_bwd_kernel(const T* __restrict__ dout, long long lddo, const T* __
       s[a] = in ? (unsigned)slots[t * top_k + j0 + a] : n;
       g[a] = in ? gates[t * top_k + j0 + a] : 0.f;
     }
-    for (int i = in_team; i < nvec; i += TEAM) {
-      float d[VEC];
-      V::unpack(V::load(dout + t * lddo + (long long)i * VEC), d);
-      typename V::Raw v[kBwdExperts];
+    constexpr int U = VEC == 1 ? 4 : 1;           // columns of a thread whose loads are in flight together
+    for (int i0 = in_team; i0 < nvec; i0 += U * TEAM) {
+      float d[U][VEC];
+      typename V::Raw v[U][kBwdExperts];
 #pragma unroll
-      for (int a = 0; a < kBwdExperts; ++a)
-        if (s[a] < n) v[a] = V::load(y + (long long)s[a] * ldy + (long long)i * VEC);
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * TEAM;
+        if (U > 1 && i >= nvec) break;
+        V::unpack(V::load(dout + t * lddo + (long long)i * VEC), d[u]);
 #pragma unroll
-      for (int a = 0; a < kBwdExperts; ++a) {
-        if (s[a] < n) {
-          float f[VEC], o[VEC];
-          V::unpack(v[a], f);
+        for (int a = 0; a < kBwdExperts; ++a)
+          if (s[a] < n) v[u][a] = V::load(y + (long long)s[a] * ldy + (long long)i * VEC);
+      }
 #pragma unroll
-          for (int c = 0; c < VEC; ++c) {
-            dot[a] += d[c] * f[c];
-            o[c] = g[a] * d[c];
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * TEAM;
+        if (U > 1 && i >= nvec) break;
+#pragma unroll
+        for (int a = 0; a < kBwdExperts; ++a) {
+          if (s[a] < n) {
+            float f[VEC], o[VEC];
+            V::unpack(v[u][a], f);
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) {
+              dot[a] += d[u][c] * f[c];
+              o[c] = g[a] * d[u][c];
+            }
+            V::store(dy + ((long long)s[a] * nvec + i) * VEC, V::pack(o));
           }
-          V::store(dy + ((long long)s[a] * nvec + i) * VEC, V::pack(o));
         }
       }
     }
@@ -366,7 +392,7 @@ RowGrid row_grid(long long tokens, int nvec, int unroll, unsigned* blocks) {
 template <typename T, int VEC>
 int permute_rows(const void* x, long long ldx, const int* slots, const int* kept, void* xp, long long tokens, int top_k, int hidden, cudaStream_t s) {
   unsigned blocks;
-  const RowGrid g = row_grid(tokens, hidden / VEC, kRowUnroll, &blocks);
+  const RowGrid g = row_grid(tokens, hidden / VEC, row_unroll(VEC), &blocks);
   moe_permute_kernel<T, VEC><<<blocks, kRowThreads, 0, s>>>(static_cast<const T*>(x), ldx, slots, kept, static_cast<T*>(xp), tokens, top_k, hidden / VEC, g);
   PKB_CHECK_CUDA(cudaGetLastError());
   return kApiOk;
@@ -376,7 +402,7 @@ template <typename T, int VEC>
 int unpermute_rows(const void* y, long long ldy, const int* slots, const float* gates, void* out, long long tokens, int top_k, int hidden,
                    cudaStream_t s) {
   unsigned blocks;
-  const RowGrid g = row_grid(tokens, hidden / VEC, 1, &blocks);
+  const RowGrid g = row_grid(tokens, hidden / VEC, gather_unroll(VEC), &blocks);
   const T* yp = static_cast<const T*>(y);
   T* op = static_cast<T*>(out);
   if (gates != nullptr) moe_unpermute_kernel<T, VEC, true><<<blocks, kRowThreads, 0, s>>>(yp, ldy, slots, gates, op, tokens, top_k, hidden / VEC, g);
