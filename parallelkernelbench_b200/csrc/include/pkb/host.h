@@ -51,6 +51,15 @@ const char* last_error_cstr();
 // memory, so the host can read it after any synchronisation without a copy). nullptr on failure.
 uint32_t* status_block_device_ptr();
 
+// The same for a launch that may be captured: the first call on a device allocates the block, which a capture otherwise forbids.
+inline uint32_t* status_block_for_launch() {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+  uint32_t* status = status_block_device_ptr();
+  (void)cudaThreadExchangeStreamCaptureMode(&mode);
+  return status;
+}
+
 enum TmapDtype : int { kTmapBf16 = 0, kTmapFp8 = 1, kTmapFp32 = 2, kTmapU8 = 3, kTmapFp16 = 4 };
 enum TmapSwizzle : int { kSwizzleNone = 0, kSwizzle32 = 1, kSwizzle64 = 2, kSwizzle128 = 3 };
 

@@ -427,13 +427,15 @@ __device__ __forceinline__ LnRing ln_ring_init(uint8_t* smem, int stages, uint32
   return r;
 }
 
-// false once a row did not come within the budget: the caller leaves, after what is in flight
+// false once a row did not come within the budget. The block then walks its other rows without waiting (their results are of no use), so that
+// nobody is missing at a barrier, copies nothing more, and leaves after what is in flight.
 __device__ __forceinline__ bool ln_ring_wait(const LnRing& r, int stage, uint32_t parity, volatile int* abort_flag, uint32_t* status, long long row) {
   if (mbar_wait(r.bars + 8 * stage, parity, abort_flag)) return true;
   if (threadIdx.x == 0) record_status(status, kStatusMbarTimeout, kLnKernelId, 0, stage, 1, (uint32_t)row);
   return false;
 }
-__device__ __forceinline__ void ln_ring_abandon() {
+__device__ __forceinline__ void ln_ring_leave(bool ok) {
+  if (ok) return;
   const uint64_t t0 = globaltimer_ns();
   while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
 }
@@ -478,11 +480,9 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
   }
   int stage = 0;
   uint32_t parity = 0;
+  bool ok = true;
   for (long long grp = blockIdx.x; grp < groups; grp += gridDim.x) {
-    if (!ln_ring_wait(ring, stage, parity, &abort_flag, status, grp)) {
-      ln_ring_abandon();
-      return;
-    }
+    ok = ok && ln_ring_wait(ring, stage, parity, &abort_flag, status, grp);
     const int here = R == 1 ? 1 : (int)min((long long)R, rows - grp * R);
     F2 v[R][CH][P];
     float s[R], q[R], rstd[R];
@@ -501,7 +501,7 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
       s[i] = f2_sum(acc);
     }
     team_sum<R, NT, NT>(s, red[0], 0);
-    if (t == 0 && grp + (long long)stages * gridDim.x < groups) {
+    if (t == 0 && ok && grp + (long long)stages * gridDim.x < groups) {
       fence_proxy_async_smem();
       issue(grp + (long long)stages * gridDim.x, stage);
     }
@@ -556,6 +556,7 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
       parity ^= 1u;
     }
   }
+  ln_ring_leave(ok);
 }
 
 // A stage holds a row of x and the same row of dy. PER as above; here only the gain is held.
@@ -593,6 +594,7 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
   }
   int stage = 0, it = 0;
   uint32_t parity = 0;
+  bool ok = true;
   float mean_n = blockIdx.x < rows ? mean_in[blockIdx.x] : 0.f, rstd_n = blockIdx.x < rows ? rstd_in[blockIdx.x] : 0.f;
   for (long long row = blockIdx.x; row < rows; row += gridDim.x, it ^= 1) {
     const float mean = mean_n, rstd = rstd_n;
@@ -600,10 +602,7 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
       mean_n = mean_in[row + gridDim.x];
       rstd_n = rstd_in[row + gridDim.x];
     }
-    if (!ln_ring_wait(ring, stage, parity, &abort_flag, status, row)) {
-      ln_ring_abandon();
-      return;
-    }
+    ok = ok && ln_ring_wait(ring, stage, parity, &abort_flag, status, row);
     const F2 shift = f2(-mean), r2 = f2(rstd);
     U4 xr[CH], dr[CH];
     F2 s1 = 0, s2 = 0;
@@ -630,7 +629,7 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
     }
     float s[2] = {f2_sum(s1), f2_sum(s2)};
     team_sum<2, NT, NT>(s, red[it], 0);
-    if (t == 0 && row + (long long)stages * gridDim.x < rows) {
+    if (t == 0 && ok && row + (long long)stages * gridDim.x < rows) {
       fence_proxy_async_smem();
       issue(row + (long long)stages * gridDim.x, stage);
     }
@@ -670,6 +669,7 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
       }
     }
   }
+  ln_ring_leave(ok);
 }
 
 // ---- many wide rows that do not start on 16 bytes -------------------------------------------------
@@ -801,11 +801,9 @@ ln_fwd_odd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, c
   }
   int stage = 0;
   uint32_t parity = 0;
+  bool ok = true;
   for (long long grp = blockIdx.x; grp < groups; grp += gridDim.x) {
-    if (!ln_ring_wait(ring, stage, parity, &abort_flag, status, grp)) {
-      ln_ring_abandon();
-      return;
-    }
+    ok = ok && ln_ring_wait(ring, stage, parity, &abort_flag, status, grp);
     const int here = R == 1 ? 1 : (int)min((long long)R, rows - grp * R);
     F2 v[R][P];
     float s[R] = {}, q[R] = {}, rstd[R];
@@ -820,7 +818,7 @@ ln_fwd_odd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, c
       s[i] = f2_sum(acc);
     }
     team_sum<R, NT, NT>(s, red[0], 0);
-    if (t == 0 && grp + (long long)stages * gridDim.x < groups) {
+    if (t == 0 && ok && grp + (long long)stages * gridDim.x < groups) {
       fence_proxy_async_smem();
       issue(grp + (long long)stages * gridDim.x, stage);
     }
@@ -859,6 +857,7 @@ ln_fwd_odd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, c
       parity ^= 1u;
     }
   }
+  ln_ring_leave(ok);
 }
 
 // Both passes over a row read it from its stage (the registers hold the weights' sums), which is therefore free only after the next row's barrier.
@@ -894,6 +893,7 @@ ln_bwd_odd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ 
   for (int j = 0; j < P; ++j) g[j] = gains(j);
   int stage = 0, before = -1, it = 0;
   uint32_t parity = 0;
+  bool ok = true;
   float mean_n = blockIdx.x < rows ? mean_in[blockIdx.x] : 0.f, rstd_n = blockIdx.x < rows ? rstd_in[blockIdx.x] : 0.f;
   for (long long row = blockIdx.x; row < rows; row += gridDim.x, it ^= 1) {
     const float mean = mean_n, rstd = rstd_n;
@@ -901,10 +901,7 @@ ln_bwd_odd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ 
       mean_n = mean_in[row + gridDim.x];
       rstd_n = rstd_in[row + gridDim.x];
     }
-    if (!ln_ring_wait(ring, stage, parity, &abort_flag, status, row)) {
-      ln_ring_abandon();
-      return;
-    }
+    ok = ok && ln_ring_wait(ring, stage, parity, &abort_flag, status, row);
     const uint32_t at = ring.base + stage * 2 * row_stage;
     const LnOddRow<T, NT> xr = odd_row<NT>(span_x, x + row * ldx, bytes, at), dr = odd_row<NT>(span_d, dy + row * lddy, bytes, at + row_stage);
     const F2 shift = f2(-mean), r2 = f2(rstd);
@@ -923,7 +920,7 @@ ln_bwd_odd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ 
     float s[2] = {f2_sum(s1), f2_sum(s2)};
     team_sum<2, NT, NT>(s, red[it], 0);
     const long long ahead = row + (long long)(stages - 1) * gridDim.x;
-    if (t == 0 && before >= 0 && ahead < rows) {
+    if (t == 0 && ok && before >= 0 && ahead < rows) {
       fence_proxy_async_smem();
       issue(ahead, before);
     }
@@ -956,6 +953,7 @@ ln_bwd_odd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ 
       out[cols + col(2 * j + 1)] = b.y;
     }
   }
+  ln_ring_leave(ok);
 }
 
 // dgamma, dbeta [2][cols] = sum over the blocks of part[block][2][cols]: 32 columns and 32 strands of blocks per thread block
@@ -1105,7 +1103,7 @@ int ln_fwd_ring(const LnRingPlan& r, const T* x, long long ldx, LnParam g, LnPar
   auto go = [&](auto at) -> int {
     constexpr auto kern = decltype(at)::value;
     if (const int rc = prepare_kernel<kern>(128 + kLnRingBytes)) return rc;
-    kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, r.stages, status_block_device_ptr());
+    kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, r.stages, status_block_for_launch());
     PKB_CHECK_CUDA(cudaGetLastError());
     return kApiOk;
   };
@@ -1121,7 +1119,7 @@ int ln_fwd_odd(const LnRingPlan& r, const T* x, long long ldx, LnParam g, LnPara
   auto go = [&](auto at) -> int {
     constexpr auto kern = decltype(at)::value;
     if (const int rc = prepare_kernel<kern>(128 + kLnRingBytes)) return rc;
-    kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, r.stages, (uint32_t)r.row_stage, status_block_device_ptr());
+    kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, r.stages, (uint32_t)r.row_stage, status_block_for_launch());
     PKB_CHECK_CUDA(cudaGetLastError());
     return kApiOk;
   };
@@ -1142,7 +1140,7 @@ int ln_bwd_odd(const LnRingPlan& r, const T* x, long long ldx, const T* dy, long
     constexpr auto kern = decltype(at)::value;
     if (const int rc = prepare_kernel<kern>(128 + kLnRingBytes)) return rc;
     kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, r.stages, (uint32_t)r.row_stage,
-                                             status_block_device_ptr());
+                                             status_block_for_launch());
     PKB_CHECK_CUDA(cudaGetLastError());
     return kApiOk;
   };
@@ -1162,7 +1160,7 @@ int ln_bwd_ring(const LnRingPlan& r, const T* x, long long ldx, const T* dy, lon
   auto go = [&](auto at) -> int {
     constexpr auto kern = decltype(at)::value;
     if (const int rc = prepare_kernel<kern>(128 + kLnRingBytes)) return rc;
-    kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, r.stages, status_block_device_ptr());
+    kern<<<r.blocks, r.threads, r.smem, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, r.stages, status_block_for_launch());
     PKB_CHECK_CUDA(cudaGetLastError());
     return kApiOk;
   };

@@ -1354,11 +1354,7 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
   PKB_CHECK_ARG(batch > 0 && batch <= 65535 && rows > 0 && cols > 0, "1 .. 65535 matrices of at least one row and column");
   PKB_CHECK_ARG(steps >= 1 && coeff != nullptr, "at least one step");
   PKB_CHECK_ARG(g != nullptr && ((out != nullptr) != (p != nullptr)), "g, scratch and one of out and p");
-  // the first call on a device allocates its status block: let that happen inside a graph capture, too
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  PKB_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-  uint32_t* status = status_block_device_ptr();
-  PKB_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  uint32_t* status = status_block_for_launch();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool tall = rows > cols;
   const int side = tall ? cols : rows, longer = tall ? rows : cols;
