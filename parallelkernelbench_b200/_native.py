@@ -133,17 +133,28 @@ def bound(name: str, argtypes: list, restype=ctypes.c_int):
     return f
 
 
-def launch(name: str, argtypes: list, t, *args, launches: int = 1) -> None:
-    """Call the entry point ``name`` with ``args`` and, last, the current stream of the device of ``t``, with that device as the current one."""
+_current = None
+
+
+def _device_calls():
+    """torch's current device and raw stream of a device, looked up once (torch is imported on first use)."""
+    global _current
     import torch
 
+    _current = (torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.cuda.device, torch.empty_like)
+    return _current
+
+
+def launch(name: str, argtypes: list, t, *args, launches: int = 1) -> None:
+    """Call the entry point ``name`` with ``args`` and, last, the current stream of the device of ``t``, with that device as the current one."""
+    current_device, stream_of, device_scope, _ = _current or _device_calls()
     f = _bound.get(name) or bound(name, argtypes)
     device = t.get_device()
-    if device == torch._C._cuda_getDevice():
-        rc = f(*args, torch._C._cuda_getCurrentRawStream(device))
+    if device == current_device():
+        rc = f(*args, stream_of(device))
     else:
-        with torch.cuda.device(device):
-            rc = f(*args, torch._C._cuda_getCurrentRawStream(device))
+        with device_scope(device):
+            rc = f(*args, stream_of(device))
     if rc:
         check(rc, name)
     count_launch(launches)
@@ -161,9 +172,7 @@ def same_cuda_device(first, **tensors) -> None:
 
 def contiguous_like(t):
     """An uninitialised contiguous tensor of the shape and type of ``t`` (``empty_like`` is the cheaper call, but keeps strides)."""
-    import torch
-
-    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+    return (_current or _device_calls())[3](t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def read_status() -> list[int]:

@@ -56,20 +56,25 @@ def _rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
     return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
 
 
+def _ln_param(name: str, p: torch.Tensor, x: torch.Tensor, cols: int) -> None:
+    if p.dtype not in _DT or p.numel() != cols or not p.is_contiguous():
+        raise ValueError(f"{name} must be contiguous bf16 or fp32 with {cols} values")
+    if p.get_device() != x.get_device():
+        raise ValueError(f"{name} is on {p.device}, not on {x.device}")
+
+
 def _ln_check(x: torch.Tensor, gamma, beta=None) -> int:
     if x.dtype not in _DT:
         raise TypeError(f"layer norm takes bf16 or fp32 rows, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("layer norm needs at least one column")
     cols = x.shape[-1]
-    for name, p in (("gamma", gamma), ("beta", beta)):
-        if p is not None:
-            if p.dtype not in _DT or p.numel() != cols or not p.is_contiguous():
-                raise ValueError(f"{name} must be contiguous bf16 or fp32 with {cols} values")
-            if p.get_device() != x.get_device():
-                raise ValueError(f"{name} is on {p.device}, not on {x.device}")
-    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
-        raise TypeError("gamma and beta must have the same dtype")
+    if gamma is not None:
+        _ln_param("gamma", gamma, x, cols)
+    if beta is not None:
+        _ln_param("beta", beta, x, cols)
+        if gamma is not None and beta.dtype != gamma.dtype:
+            raise TypeError("gamma and beta must have the same dtype")
     return cols
 
 
