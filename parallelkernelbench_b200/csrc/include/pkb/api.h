@@ -36,6 +36,32 @@ int pkb_rmsnorm_bf16(const void* x, const void* gamma, void* y, int rows, int co
 int pkb_sum_rmsnorm(const void* src, long long src_stride_elems, int nsrc, int src_is_f32,
                     const void* gamma, void* y, int rows, int cols, float scale, float eps,
                     void* stream);
+// Layer norm of rows x (ldx elements apart, any value) into y [rows, cols]; dtype 0 bf16, 1 fp32; gamma, beta [cols] or null, bf16 or
+// (param_f32) fp32; mean, rstd fp32 [rows], both or neither null.
+int pkb_layer_norm_fwd(const void* x, long long ldx, const void* gamma, const void* beta, int param_f32, void* y, void* mean, void* rstd,
+                       long long rows, int cols, float eps, int dtype, void* stream);
+// Its backward: dx, and dgamma, dbeta fp32 [cols]; partial: pkb_layer_norm_bwd_partials(rows, cols, dtype) x 2 x cols fp32 values.
+int pkb_layer_norm_bwd_partials(long long rows, int cols, int dtype);
+int pkb_layer_norm_bwd(const void* x, long long ldx, const void* dy, long long lddy, const void* gamma, int param_f32, const void* mean,
+                       const void* rstd, void* dx, void* dgamma, void* dbeta, void* partial, long long rows, int cols, int dtype, void* stream);
+
+// ---- tokens sorted by expert and back, one GPU -----------------------------------------------
+// idx int32 [n], values outside [0, experts) are dropped; offsets [experts + 1], order [n], slots [n] int32. experts <= 1024.
+int pkb_moe_sort(const void* idx, long long n, int experts, void* offsets, void* order, void* slots, void* stream);
+// kept: address of offsets[experts] (device). dtype 0 bf16, 1 fp32. See kernels/moe_sort.cu for the formulas.
+int pkb_moe_permute(const void* x, long long ldx, const void* slots, const void* kept, void* xp, long long tokens, int top_k, int hidden, int dtype,
+                    void* stream);
+int pkb_moe_unpermute(const void* y, long long ldy, const void* slots, const void* gates, void* out, long long tokens, int top_k, int hidden,
+                      int dtype, void* stream);
+int pkb_moe_unpermute_bwd(const void* dout, long long lddo, const void* y, long long ldy, const void* slots, const void* gates, const void* kept,
+                          void* dy, void* dgates, long long tokens, int top_k, int hidden, int dtype, void* stream);
+
+// ---- orthogonalised updates ------------------------------------------------------------------
+// Bytes of scratch (256-byte aligned) that pkb_newton_schulz wants for this problem and, where launches is not null, its number of launches.
+long long pkb_newton_schulz_scratch(long long batch, int rows, int cols, int steps, int* launches);
+// coeff: HOST array of `steps` triples. m (fp32 momentum, updated) may be null. One of out (bf16) and p (fp32, updated; p_bf16 its copy or null).
+int pkb_newton_schulz(const void* g, int g_f32, void* m, float momentum, int nesterov, long long batch, int rows, int cols, const float* coeff,
+                      int steps, double eps, void* out, void* p, float decay, float scale, void* p_bf16, void* scratch, void* stream);
 
 #ifdef __cplusplus
 }

@@ -4,6 +4,11 @@
 // The variance is the mean of squared differences from the mean, never E[x^2] - mean^2: a row far from zero loses nothing.
 // A row belongs to a team of TPR threads that holds VEC * CH of its values each: 16-byte accesses where base, row pitch and width
 // allow them (VEC = 8 bf16 or 4 fp32), single values otherwise. All sums are fp32.
+// Forms, by width, alignment and number of rows (ln_fwd_any, ln_bwd_any): teams of 32 to 512 threads straight from global memory; from 1025 columns
+// and a few hundred rows on, rings of rows in shared memory; rows that no team holds in passes. Measured, forward / backward with the weights' sums,
+// us (copy bandwidth): 16384 x 8192 bf16 105 / 140 (78 % / 88 %), 8192 x 4096 31 / 44 (66 / 70), 16384 x 1000 19 / 25, 8192 x 4097 64 / 101,
+// 8192 x 4097 fp32 69 / 100 (59 / 61). A copy of 16384 x 8192 takes 84: what keeps the forward from it is not one thing (a warp per row without any
+// barrier takes as long, prefetching further ahead takes longer).
 #include "pkb/api.h"
 #include "pkb/bulk_copy.cuh"
 #include "pkb/host.h"

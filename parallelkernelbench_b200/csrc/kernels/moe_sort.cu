@@ -6,6 +6,8 @@
 // The row kernels are memory bound. All of them walk the tokens, not the sorted rows: a token's row is read (or written) once for its
 // top_k copies, which are scattered (or gathered) as whole rows; sums over a token's experts run in the order of j in fp32, so nothing
 // depends on timing. Rows behind the last expert's (as many as there are dropped assignments) are written as zeros.
+// 8192 tokens x 7168 bf16, top-8 of 256: sort 13 us, permute 168, unpermute 169, its gradient 313, the permutation's 164: 5.17 GB in 827 us, 95 % of
+// the copy bandwidth. Small calls are bound by the host (11 us a call).
 #include <cooperative_groups.h>
 
 #include "pkb/api.h"

@@ -5,6 +5,10 @@ kernel turns them into slot bases and grouped-GEMM offsets, the dispatch kernel 
 into the destination ranks' receive buffers, and the combine kernel pulls expert outputs back over
 NVLink. The reference synchronises with the host three times per layer call
 (reference: reference/31_fused_moe_fwd.py:60-101).
+
+On one GPU, and for training, ``sort_by_expert`` orders the assignments without the symmetric heap, ``permute_tokens`` and
+``unpermute_tokens`` take the rows to the grouped GEMM and back, and their ``_bwd`` forms are their gradients
+(kernels: csrc/kernels/moe_sort.cu).
 """
 from __future__ import annotations
 
