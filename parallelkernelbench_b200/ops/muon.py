@@ -75,7 +75,7 @@ def newton_schulz(g: torch.Tensor, *, steps: int = 5, coefficients=FAST, eps: fl
     """Orthogonalises the matrices ``g`` (bf16 or fp32 ``[..., rows, cols]``, any sides): ``X = g / (|g|_F + eps)``, then ``steps`` times
     ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``. ``coefficients`` is one ``(a, b, c)`` or a sequence of one per step. Returns bf16 of the
     same shape (at most 65535 matrices). The iterate is held in fp32 and multiplied in fp16 with fp32 sums. A matrix of zeros stays zero; one with a value that is not
-    finite comes back as NaN, alone."""
+    finite comes back as NaN, alone. The same call gives the same bits; alone a matrix may be split over the GPU in another way than in a batch."""
     if g.dtype not in _DT:
         raise TypeError(f"newton_schulz takes bf16 or fp32, got {g.dtype}")
     if g.dim() < 2:

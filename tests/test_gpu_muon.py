@@ -66,7 +66,7 @@ def _check(out, u, **kw):
 # one value, rows and columns of one, slices of the one-launch form (a side of up to 128, the longer up to 4096) that end anywhere, the first
 # sizes beyond it, the edges of tiles (256) and of a CTA's half (128), odd sides, wide and tall, a long inner extent
 SHAPES = [(1, 1), (1, 5), (5, 1), (7, 3), (16, 16), (3, 2000), (64, 2048), (2048, 40), (128, 128), (129, 127), (33, 65), (128, 4096), (3001, 96), (70, 4097),
-          (4100, 128), (129, 300), (256, 256), (257, 255), (333, 1000), (1000, 333),
+          (4100, 128), (129, 300), (1, 5000), (5000, 1), (3, 16001), (9000, 17), (256, 256), (257, 255), (333, 1000), (1000, 333),
           (512, 1024), (640, 512), (1025, 513)]
 
 
@@ -109,6 +109,23 @@ def test_batches_are_matrices_of_their_own(shape):
         else:
             assert torch.equal(out[i], newton_schulz(flat[i]))
     assert torch.equal(out[1], torch.zeros_like(out[1]))
+
+
+@pytest.mark.parametrize("shape", [(4, 200, 300), (4, 513, 257), (4, 40, 4100), (2, 2, 4099, 33), (4, 1300, 1290)])
+def test_a_bad_matrix_stays_alone(shape):
+    """The same batch with and without bad neighbours: bit for bit the same for the others. (Alone a matrix may be split in another way.)"""
+    from parallelkernelbench_b200.ops import newton_schulz
+
+    u = _matrix(shape, "noise").to(torch.bfloat16)
+    flat = u.view(-1, *shape[-2:])
+    clean = newton_schulz(u).view_as(flat)
+    flat[1] = 0
+    flat[2, 0, 0] = float("inf")
+    flat[3, -1, -1] = float("nan")
+    out = newton_schulz(u).view_as(flat)
+    assert torch.equal(out[0], clean[0]) and torch.equal(out[1], torch.zeros_like(out[1]))
+    assert torch.isnan(out[2]).any() and torch.isnan(out[3]).any()
+    _check(out[0], flat[0])
 
 
 @pytest.mark.parametrize("batch,rows,cols", [(7, 64, 512), (40, 100, 72), (70, 12, 1000), (3, 1500, 90)])
@@ -174,7 +191,7 @@ def _step(shape, dtype, nesterov, decay, copy, offset=0):
     return p, m, grad, pb
 
 
-@pytest.mark.parametrize("shape", [(40, 72), (72, 40), (300, 130), (257, 512), (3, 128, 256), (1, 9)])
+@pytest.mark.parametrize("shape", [(40, 72), (72, 40), (300, 130), (257, 512), (3, 128, 256), (1, 9), (2, 200, 333), (4200, 24), (1700, 1411)])
 @pytest.mark.parametrize("dtype,nesterov,decay,copy,offset", [(torch.bfloat16, True, 0.1, True, 0), (torch.float32, False, 0.0, False, 0),
                                                               (torch.bfloat16, False, 0.1, True, 1), (torch.float32, True, 0.1, False, 3)])
 def test_muon_step(shape, dtype, nesterov, decay, copy, offset):
