@@ -231,14 +231,17 @@ ln_fwd_long_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
   }
 }
 
+constexpr int kLnCluster = 16;
+
 // Backward. The blocks are persistent: a thread keeps its columns' sums of dy xhat and dy in registers over all rows of its block and
 // writes them once, to part[block][2][cols]; ln_bwd_params_kernel adds the blocks' sums in a fixed order. The loads of a team's next
 // row are issued before the sums of the current one.
-template <typename T, int VEC, int TPR, int CH>
+// CLUSTER: all blocks are one cluster, which adds the blocks' sums itself through distributed shared memory and writes them to part[2][cols].
+template <typename T, int VEC, int TPR, int CH, bool CLUSTER>
 __global__ void __launch_bounds__(LnTeam<T, VEC, TPR, CH>::kThreads, 512 / LnTeam<T, VEC, TPR, CH>::kThreads)
 ln_bwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ dy, long long lddy, const LnParam gamma,
               const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part,
-              long long rows, int cols) {
+              float* __restrict__ dgamma, float* __restrict__ dbeta, long long rows, int cols) {
   using L = LnTeam<T, VEC, TPR, CH>;
   __shared__ float red[2][2 * (L::kThreads / 32)];
   __shared__ float sums[L::kRows > 1 ? L::kRows * L::kCols : 1];
@@ -305,8 +308,9 @@ ln_bwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ dy, 
     }
   }
   // the teams' sums, added in the order of the teams
-  ln_let_successor_launch();
-  float* out = part + (long long)blockIdx.x * 2 * cols;
+  extern __shared__ float block_sums[];              // CLUSTER: [2][cols]
+  if constexpr (!CLUSTER) ln_let_successor_launch();
+  float* out = CLUSTER ? block_sums : part + (long long)blockIdx.x * 2 * cols;
   if constexpr (L::kRows == 1) {
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch)
@@ -334,6 +338,24 @@ ln_bwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ dy, 
         out[which * cols + c] = a;
       }
     }
+  }
+  if constexpr (CLUSTER) {
+    cluster_sync_all();
+    const int ctas = (int)cluster_nctaid();
+    for (int i = (int)(cluster_ctarank() * L::kThreads + threadIdx.x); i < 2 * cols; i += ctas * L::kThreads) {
+      const uint32_t at = smem_u32(block_sums + i);
+      float v[kLnCluster];
+#pragma unroll
+      for (int c = 0; c < kLnCluster; ++c)
+        if (c < ctas) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[c]) : "r"(mapa_shared(at, (uint32_t)c)) : "memory");
+      float a = 0.f;
+#pragma unroll
+      for (int c = 0; c < kLnCluster; ++c)
+        if (c < ctas) a += v[c];
+      if (i < cols) dgamma[i] = a;
+      else dbeta[i - cols] = a;
+    }
+    cluster_sync_all();      // nobody leaves while its sums may still be read
   }
 }
 
@@ -1195,13 +1217,41 @@ int ln_fwd_any(const void* xv, long long ldx, LnParam g, LnParam b, void* yv, fl
   return vec ? ln_fwd_team<T, VEC16>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, s) : ln_fwd_team<T, 1>(x, ldx, g, b, y, mean, rstd, rows, cols, eps, s);
 }
 
+// threads of a row and rows of a block in the backward's team form
+int ln_bwd_team_threads(int cols) { return cols <= 512 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512; }
+int ln_bwd_team_rows(int cols) { return cols <= 4096 ? 256 / ln_bwd_team_threads(cols) : 1; }
+
+// Small problems in one launch: a cluster of up to 16 blocks, which needs no partial sums in memory and no second kernel (5 us of the host's 19 per
+// call), but has 16 SMs only: up to eight rows per team. Device us, one launch / two: 64 x 128 6.3 / 6.4, 512 x 512 (four rows) 8.4 / 6.4, 128 x 4096
+// (eight) 12.5 / 12.5, 256 x 4096 (16) 16.6 / 18.4, 1000 x 1001 (16) 27.7 / 10.5, 4000 x 64 (32) 26.9 / 8.4.
+bool ln_bwd_one_launch(long long rows, int cols) { return cols <= kLnTeamCols && rows <= 8ll * kLnCluster * ln_bwd_team_rows(cols); }
+
 template <typename T, int VEC>
-int ln_bwd_team(const T* x, long long ldx, const T* dy, long long lddy, LnParam g, const float* mean, const float* rstd, T* dx, float* part,
-                int blocks, long long rows, int cols, cudaStream_t s) {
+int ln_bwd_team(const T* x, long long ldx, const T* dy, long long lddy, LnParam g, const float* mean, const float* rstd, T* dx, float* dgamma,
+                float* dbeta, float* part, int blocks, long long rows, int cols, cudaStream_t s) {
   auto go = [&](auto tpr, auto ch) -> int {
     using L = LnTeam<T, VEC, tpr.value, ch.value>;
-    ln_bwd_kernel<T, VEC, tpr.value, ch.value><<<blocks, L::kThreads, 0, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols);
-    PKB_CHECK_CUDA(cudaGetLastError());
+    if (!ln_bwd_one_launch(rows, cols)) {
+      ln_bwd_kernel<T, VEC, tpr.value, ch.value, false><<<blocks, L::kThreads, 0, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, part, dgamma, dbeta, rows, cols);
+      PKB_CHECK_CUDA(cudaGetLastError());
+      return kApiOk;
+    }
+    constexpr auto kern = ln_bwd_kernel<T, VEC, tpr.value, ch.value, true>;
+    if (const int rc = prepare_kernel<kern>(2 * L::kCols * (int)sizeof(float), true)) return rc;
+    const long long want = (rows + L::kRows - 1) / L::kRows;
+    const unsigned ctas = (unsigned)(want < kLnCluster ? want : kLnCluster);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(L::kThreads);
+    cfg.dynamicSmemBytes = 2 * (size_t)cols * sizeof(float);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    PKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, x, ldx, dy, lddy, g, mean, rstd, dx, (float*)nullptr, dgamma, dbeta, rows, cols));
     return kApiOk;
   };
   return ln_by_width<decltype(go)&, T, VEC, true>(cols, go);
@@ -1210,9 +1260,8 @@ int ln_bwd_team(const T* x, long long ldx, const T* dy, long long lddy, LnParam 
 // blocks of the backward's team form (rows of a block at once, blocks per SM) or slices of its long form
 int ln_bwd_blocks(long long rows, int cols) {
   if (cols > kLnTeamCols) return (int)(rows < 4 * kLnLongSlices ? (rows + 3) / 4 : kLnLongSlices);
-  const int tpr = cols <= 512 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
-  const int threads = tpr > 256 ? tpr : 256, per = threads / tpr;
-  const long long want = (rows + per - 1) / per, most = (long long)sm_count() * (512 / threads);
+  const int per = ln_bwd_team_rows(cols);
+  const long long want = (rows + per - 1) / per, most = (long long)sm_count() * (cols <= 4096 ? 2 : 1);
   return (int)(want < most ? want : most);
 }
 
@@ -1239,9 +1288,9 @@ int ln_bwd_any(const void* xv, long long ldx, const void* dyv, long long lddy, L
     ln_bwd_long_params_kernel<T><<<dim3((unsigned)((cols + 63) / 64), (unsigned)blocks), 256, 0, s>>>(x, ldx, dy, lddy, mean, rstd, part, rows, cols);
     PKB_CHECK_CUDA(cudaGetLastError());
   } else {
-    const int rc = vec ? ln_bwd_team<T, VEC16>(x, ldx, dy, lddy, g, mean, rstd, dx, part, blocks, rows, cols, s)
-                       : ln_bwd_team<T, 1>(x, ldx, dy, lddy, g, mean, rstd, dx, part, blocks, rows, cols, s);
-    if (rc) return rc;
+    const int rc = vec ? ln_bwd_team<T, VEC16>(x, ldx, dy, lddy, g, mean, rstd, dx, dgamma, dbeta, part, blocks, rows, cols, s)
+                       : ln_bwd_team<T, 1>(x, ldx, dy, lddy, g, mean, rstd, dx, dgamma, dbeta, part, blocks, rows, cols, s);
+    if (rc || ln_bwd_one_launch(rows, cols)) return rc;
   }
   const long long width = 2ll * cols;
   cudaLaunchConfig_t cfg = {};
@@ -1277,9 +1326,9 @@ extern "C" int pkb_layer_norm_fwd(const void* x, long long ldx, const void* gamm
 }
 
 // Blocks whose partial sums pkb_layer_norm_bwd writes: its scratch is [this][2][cols] fp32.
-// (An upper bound over the forms that rows of this width may take: alignment decides between them.)
+// (An upper bound over the forms that rows of this width may take: alignment decides between them.) 0: one launch, no scratch.
 extern "C" int pkb_layer_norm_bwd_partials(long long rows, int cols, int dtype) {
-  if (rows <= 0 || cols <= 0) return 0;
+  if (rows <= 0 || cols <= 0 || ln_bwd_one_launch(rows, cols)) return 0;
   LnRingPlan ring;
   int blocks = ln_bwd_blocks(rows, cols);
   for (const bool aligned : {true, false})
@@ -1292,8 +1341,9 @@ extern "C" int pkb_layer_norm_bwd(const void* x, long long ldx, const void* dy, 
                                   const void* rstd, void* dx, void* dgamma, void* dbeta, void* partial, long long rows, int cols, int dtype,
                                   void* stream) {
   PKB_CHECK_ARG(rows > 0 && cols > 0, "empty problem");
-  PKB_CHECK_ARG(x && dy && mean && rstd && dx && dgamma && dbeta && partial, "null pointer");
+  PKB_CHECK_ARG(x && dy && mean && rstd && dx && dgamma && dbeta, "null pointer");
   PKB_CHECK_ARG(dtype == 0 || dtype == 1, "dtype must be 0 (bf16) or 1 (fp32)");
+  PKB_CHECK_ARG(partial != nullptr || ln_bwd_one_launch(rows, cols), "scratch for the partial sums");
   const LnParam g{gamma, param_f32, 1.f};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto f = [](void* p) { return static_cast<float*>(p); };

@@ -336,7 +336,7 @@ def permute_tokens(x: torch.Tensor, srt: ExpertSort) -> torch.Tensor:
     ``out[slots[t, j]] = x[t]``. Rows from ``offsets[E]`` on are zero."""
     x = _rows_arg(x, srt.tokens, "x")
     n = _sort_arg(srt, x)
-    out = x.new_empty((n, x.shape[1]))
+    out = x.new_empty(n, x.shape[1])
     if n:
         nv.launch("pkb_moe_permute", _PERMUTE, x, x.data_ptr(), x.stride(0), srt.slots.data_ptr(), _kept_ptr(srt), out.data_ptr(), srt.tokens,
                   srt.top_k, x.shape[1], _DT[x.dtype])
@@ -349,7 +349,7 @@ def unpermute_tokens(y: torch.Tensor, srt: ExpertSort, gates: torch.Tensor | Non
     y = _rows_arg(y, srt.tokens * srt.top_k, "y")
     n = _sort_arg(srt, y)
     g = None if gates is None else _gates_arg(gates, srt, y)
-    out = (y.new_empty if n else y.new_zeros)((srt.tokens, y.shape[1]))
+    out = (y.new_empty if n else y.new_zeros)(srt.tokens, y.shape[1])
     if n:
         nv.launch("pkb_moe_unpermute", _UNPERMUTE, y, y.data_ptr(), y.stride(0), srt.slots.data_ptr(), 0 if g is None else g.data_ptr(),
                   out.data_ptr(), srt.tokens, srt.top_k, y.shape[1], _DT[y.dtype])

@@ -87,8 +87,10 @@ def _ln_forward(x, gamma, beta, eps, stats: bool):
     x2 = _rows_of(x, cols)
     rows = x2.shape[0]
     y = nv.contiguous_like(x)
-    mean = x.new_empty(x.shape[:-1], dtype=torch.float32) if stats else None
-    rstd = torch.empty_like(mean) if stats else None
+    mean = rstd = None
+    if stats:
+        mean = x.new_empty(rows, dtype=torch.float32) if x.dim() == 2 else x.new_empty(x.shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
     if rows:
         param = gamma if gamma is not None else beta
         nv.launch("pkb_layer_norm_fwd", _LN_FWD, x, x2.data_ptr(), x2.stride(0), 0 if gamma is None else gamma.data_ptr(),
@@ -129,10 +131,11 @@ def layer_norm_bwd(x: torch.Tensor, gamma: torch.Tensor | None, dy: torch.Tensor
     dx = nv.contiguous_like(x)
     if not rows:
         return dx, x.new_zeros(cols, dtype=torch.float32), x.new_zeros(cols, dtype=torch.float32)
-    dgamma = x.new_empty(cols, dtype=torch.float32)
+    dgamma = torch.empty_like(gamma) if gamma is not None and gamma.dtype == torch.float32 and gamma.dim() == 1 else x.new_empty(cols, dtype=torch.float32)
     dbeta = torch.empty_like(dgamma)
-    part = x.new_empty((_ln_partials(rows, cols, _DT[x.dtype], x.get_device()), 2, cols), dtype=torch.float32)
+    blocks = _ln_partials(rows, cols, _DT[x.dtype], x.get_device())
+    part = x.new_empty(blocks * 2 * cols, dtype=torch.float32) if blocks else None
     nv.launch("pkb_layer_norm_bwd", _LN_BWD, x, x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), 0 if gamma is None else gamma.data_ptr(),
               0 if gamma is None else _DT[gamma.dtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(),
-              part.data_ptr(), rows, cols, _DT[x.dtype], launches=2)
+              part.data_ptr() if blocks else 0, rows, cols, _DT[x.dtype], launches=2 if blocks else 1)
     return dx, dgamma, dbeta

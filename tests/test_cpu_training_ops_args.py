@@ -170,7 +170,8 @@ def test_native_entry_points():
         "forward without columns": lambda: lib.pkb_layer_norm_fwd(P, LL(8), P, P, 0, P, P, P, LL(1), 0, one, 0, None),
         "forward with half of the statistics": lambda: lib.pkb_layer_norm_fwd(P, LL(8), P, P, 0, P, P, None, LL(1), 8, one, 0, None),
         "forward of an unknown type": lambda: lib.pkb_layer_norm_fwd(P, LL(8), P, P, 0, P, P, P, LL(1), 8, one, 2, None),
-        "backward without scratch": lambda: lib.pkb_layer_norm_bwd(P, LL(8), P, LL(8), P, 0, P, P, P, P, P, None, LL(1), 8, 0, None),
+        "backward without scratch": lambda: lib.pkb_layer_norm_bwd(P, LL(8), P, LL(8), P, 0, P, P, P, P, P, None, LL(1 << 20), 8, 0, None),
+        "backward without a result": lambda: lib.pkb_layer_norm_bwd(P, LL(8), P, LL(8), P, 0, P, P, P, P, None, P, LL(1), 8, 0, None),
         "backward of an unknown type": lambda: lib.pkb_layer_norm_bwd(P, LL(8), P, LL(8), P, 0, P, P, P, P, P, P, LL(1), 8, 3, None),
         "sort of nothing": lambda: lib.pkb_moe_sort(P, LL(0), 4, P, P, P, None),
         "sort of too many": lambda: lib.pkb_moe_sort(P, LL(1 << 31), 4, P, P, P, None),
@@ -194,4 +195,4 @@ def test_native_entry_points():
     assert size(1, 16, 16) == 0                                     # one CTA keeps all
     assert size(1, 128, 4096) == 16 * 65536 + 32768 and size(1, 4096, 128) == size(1, 128, 4096)
     assert size(1, 300, 300) >= 300 * 304 * 8 and size(3, 300, 300) >= 3 * size(1, 300, 300) - 4096
-    assert lib.pkb_layer_norm_bwd_partials(LL(0), 8, 0) == 0 and lib.pkb_layer_norm_bwd_partials(LL(1), 8, 0) == 1
+    assert lib.pkb_layer_norm_bwd_partials(LL(0), 8, 0) == 0 and lib.pkb_layer_norm_bwd_partials(LL(1), 8, 0) == 0 and lib.pkb_layer_norm_bwd_partials(LL(1 << 20), 8, 0) > 0

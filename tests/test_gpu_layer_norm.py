@@ -63,6 +63,8 @@ def _check(x, dy, gamma, beta, eps, got, stats=None, grads=None):
 # addresses, rows beyond the teams, more rows than the grid takes at a time
 SHAPES = [(1, 1), (3, 2), (1, 4096), (3, 7), (5, 8), (7, 512), (7, 513), (9, 520), (9, 1024), (2, 1032), (33, 2048), (3, 2056), (17, 4096), (5, 4097),
           (5, 4104), (3, 8192), (2, 8193), (3, 8200), (2, 20001), (300, 8200), (2500, 64), (1333, 1001), (9001, 33),
+          # the last rows that a cluster's launch takes backward, and one more, at every team's width; a few hundred wide rows
+          (1024, 500), (1025, 500), (512, 1000), (513, 1000), (257, 2048), (129, 4096), (400, 4104), (129, 8192),
           # many wide rows (the ring): every width class, the last row of a round and one more, a row that is no multiple of a thread's access
           (2400, 1032), (1185, 2048), (1400, 2056), (1184, 4096), (1185, 4096), (3000, 4104), (600, 8192), (700, 8200), (301, 16384), (400, 16392),
           # the same of rows that start anywhere
