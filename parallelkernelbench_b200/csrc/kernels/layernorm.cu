@@ -5,7 +5,7 @@
 // A row belongs to a team of TPR threads that holds VEC * CH of its values each: 16-byte accesses where base, row pitch and width
 // allow them (VEC = 8 bf16 or 4 fp32), single values otherwise. All sums are fp32.
 // Forms, by width, alignment and number of rows (ln_fwd_any, ln_bwd_any): teams of 32 to 512 threads straight from global memory; from 1025 columns
-// and a few hundred rows on, rings of rows in shared memory; rows that no team holds in passes. Measured, forward / backward with the weights' sums,
+// and a few hundred rows on, rings of rows in shared memory; rows that no team holds in passes; backward a few rows in one launch of a cluster. Measured, forward / backward with the weights' sums,
 // us (copy bandwidth): 16384 x 8192 bf16 105 / 140 (78 % / 88 %), 8192 x 4096 31 / 44 (66 / 70), 16384 x 1000 19 / 25, 8192 x 4097 64 / 101,
 // 8192 x 4097 fp32 69 / 100 (59 / 61). A copy of 16384 x 8192 takes 84: what keeps the forward from it is not one thing (a warp per row without any
 // barrier takes as long, prefetching further ahead takes longer).
@@ -732,7 +732,8 @@ __device__ __forceinline__ float odd_shared(uint32_t a) {
   }
 }
 
-// A row in its stage. Pair j of a thread is columns (2 j NT + t, (2 j + 1) NT + t), zero where there is no column.
+// A row in its stage. Pair j of a thread is columns (2 j NT + t, (2 j + 1) NT + t), `none` where there is no column: the row's mean in the backward, so
+// that xhat is zero there whatever the row's size and deviation (0 - mean may leave fp32 when it is multiplied with rstd).
 template <typename T, int NT>
 struct LnOddRow {
   const T* global;                // the row
@@ -740,13 +741,13 @@ struct LnOddRow {
   int from, to;                   // columns that are there
   __device__ __forceinline__ float one(int c) const { return c >= from && c < to ? odd_shared<T>(shared + c * (int)sizeof(T)) : static_cast<float>(global[c]); }
   template <int P>
-  __device__ __forceinline__ void load(F2 (&v)[P], int cols) const {
+  __device__ __forceinline__ void load(F2 (&v)[P], int cols, float none = 0.f) const {
     const int t = threadIdx.x;
     if (from == 0 && to >= cols) {          // all rows but the tensor's first and last
       const uint32_t at = shared + t * (int)sizeof(T);
 #pragma unroll
       for (int j = 0; j < P; ++j) {
-        float lo = 0.f, hi = 0.f;
+        float lo = none, hi = none;
         if ((2 * j + 1) * NT <= cols || 2 * j * NT + t < cols) lo = odd_shared<T>(at + 2 * j * NT * (int)sizeof(T));
         if ((2 * j + 2) * NT <= cols || (2 * j + 1) * NT + t < cols) hi = odd_shared<T>(at + (2 * j + 1) * NT * (int)sizeof(T));
         v[j] = f2(lo, hi);
@@ -755,7 +756,7 @@ struct LnOddRow {
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         const int c0 = 2 * j * NT + t, c1 = c0 + NT;
-        v[j] = f2(c0 < cols ? one(c0) : 0.f, c1 < cols ? one(c1) : 0.f);
+        v[j] = f2(c0 < cols ? one(c0) : none, c1 < cols ? one(c1) : none);
       }
     }
   }
@@ -933,11 +934,11 @@ ln_bwd_odd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ 
     const LnOddRow<T, NT> xr = odd_row<NT>(span_x, x + row * ldx, bytes, at), dr = odd_row<NT>(span_d, dy + row * lddy, bytes, at + row_stage);
     const F2 shift = f2(-mean), r2 = f2(rstd);
     F2 s1 = 0, s2 = 0, xv[P], dv[P];
-    xr.load(xv, cols);
+    xr.load(xv, cols, mean);
     dr.load(dv, cols);
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-      // (dy and the gain are zero where there is no column)
+      // (dy, the gain and xhat are zero where there is no column)
       const F2 xh = mul2(add2(xv[j], shift), r2), gd = mul2(dv[j], g[j]);
       ag[j] = fma2(dv[j], xh, ag[j]);
       ab[j] = add2(dv[j], ab[j]);
@@ -953,7 +954,7 @@ ln_bwd_odd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ 
     }
     const F2 c1 = f2(-s[0] * inv * rstd), c2 = f2(-s[1] * inv * rstd);
     T* out = dx + row * cols;
-    xr.load(xv, cols);
+    xr.load(xv, cols, mean);
     dr.load(dv, cols);
 #pragma unroll
     for (int j = 0; j < P; ++j) {

@@ -117,6 +117,25 @@ def test_constant_rows():
     assert torch.equal(layer_norm(torch.full((3, 1), 7.5, device="cuda"), None, torch.full((1,), 2.0, device="cuda")), torch.full((3, 1), 2.0, device="cuda"))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_backward_of_large_constant_rows(dtype):
+    """xhat is zero although mean * rstd leaves fp32: so dx = rstd (g - mean(g)), with the sum of the mean's error. Team form, then the rings."""
+    from parallelkernelbench_b200.ops import layer_norm_bwd
+
+    for rows, cols in ((5, 1101), (1300, 1101), (1300, 1104), (700, 5000), (700, 5001)):
+        _, dy, gamma, _ = _inputs(rows, cols, dtype, torch.float32)
+        x = torch.full_like(dy, 2.0 ** 110)
+        mean, rstd = torch.full((rows,), 2.0 ** 110, device="cuda"), torch.full((rows,), 2.0 ** 20, device="cuda")
+        dx, dgamma, dbeta = (t.double() for t in layer_norm_bwd(x, gamma, dy, mean, rstd))
+        g = dy.double() * gamma.double()
+        want = 2.0 ** 20 * (g - g.mean(1, keepdim=True))
+        slack = 2.0 ** 20 * ((cols / 512 + 64) * U * g.abs().mean(1, keepdim=True) + 4 * U * g.abs())
+        half = torch.finfo(dtype).eps / 2
+        assert ((dx - want).abs() <= half * want.abs() + slack * (1 + half)).all()
+        assert not dgamma.any()
+        assert ((dbeta - dy.double().sum(0)).abs() <= (rows + 16) * U * dy.double().abs().sum(0)).all()
+
+
 def test_a_bad_row_stays_alone():
     from parallelkernelbench_b200.ops import layer_norm_bwd, layer_norm_fwd
 
