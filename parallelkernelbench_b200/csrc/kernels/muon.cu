@@ -679,12 +679,12 @@ constexpr int kNsPrepThreads = 256;
 constexpr int kNsMaxParts = 1024;
 
 // u * inv in fp32 for any |u| and inv whose product is in range (either alone may be far from one): inv = m 2^q is taken apart, u is moved half of
-// the way by an exact power of two, and only the other factor rounds.
+// the way by an exact power of two, and only the other factor rounds. Of a matrix of zeros nothing is divided: it stays zero for any eps.
 struct NsScale {
   float first, second;
-  __device__ __forceinline__ explicit NsScale(double inv) {
+  __device__ __forceinline__ NsScale(double k, double square_sum, double eps) {
     int q = 0;
-    const double m = frexp(inv, &q);
+    const double m = square_sum == 0.0 ? 0.0 : frexp(k / (sqrt(square_sum) + eps), &q);
     const int half = q / 2;
     first = ldexpf(1.f, half);
     second = ldexpf((float)m, q - half);
@@ -803,7 +803,7 @@ ns_start_kernel(const NsInput in, int rows, int cols, int pitch, const double* _
   double sum = 0.0;
   for (int i = threadIdx.x; i < parts; i += kNsPrepThreads) sum += part[b * parts + i];
   sum = block_sum_double(sum, red);
-  const NsScale scale(k / (sqrt(sum) + eps));
+  const NsScale scale(k, sum, eps);
   const int vecs = pitch / 8;
   const long long total = (long long)rows * vecs, base = b * rows * cols;
   for (long long i = (long long)blockIdx.x * kNsPrepThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kNsPrepThreads) {
@@ -995,7 +995,7 @@ ns_small_kernel(const __grid_constant__ NsSmallParams p) {
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const NsScale scale(p.k / (sqrt(sum) + p.eps));
+  const NsScale scale(p.k, sum, p.eps);
   const uint32_t tmem = tmem_holder, tm_acc = tmem + 256;
   // a warp's place in tensor memory: 32 rows, and half of the columns of what it walks
   const int q = warp & 3, half = warp >> 2, row = q * 32 + lane;

@@ -157,6 +157,15 @@ def test_scale_of_the_input(factor):
     _check(newton_schulz(u), u)
 
 
+@pytest.mark.parametrize("shape", [(96, 160), (9, 1000), (200, 264)])
+@pytest.mark.parametrize("eps", [0.0, 1e-300, 1e-7])
+def test_zeros_stay_zero(shape, eps):
+    from parallelkernelbench_b200.ops import newton_schulz
+
+    out = newton_schulz(torch.zeros(shape, device="cuda"), eps=eps)
+    assert torch.equal(out, torch.zeros_like(out))
+
+
 def test_layouts():
     from parallelkernelbench_b200.ops import newton_schulz
 
