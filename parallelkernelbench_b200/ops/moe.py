@@ -302,8 +302,8 @@ def sort_by_expert(expert_idx: torch.Tensor, num_experts: int) -> ExpertSort:
 def _rows_arg(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
     if t.dtype not in _DT:
         raise TypeError(f"{name} must be bf16 or fp32, got {t.dtype}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
-        raise ValueError(f"{name} must have {rows} rows of at least one column, got {tuple(t.shape)}")
+    if t.dim() != 2 or t.shape[0] != rows or not 1 <= t.shape[1] <= 1 << 30:
+        raise ValueError(f"{name} must have {rows} rows of at least one column (at most 2^30), got {tuple(t.shape)}")
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 

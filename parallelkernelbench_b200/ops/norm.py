@@ -48,6 +48,7 @@ _P, _I, _LL, _F = nv.c_void_p, nv.c_int, nv.c_ll, nv.c_float
 _LN_FWD = [_P, _LL, _P, _P, _I, _P, _P, _P, _LL, _I, _F, _I, _P]
 _LN_BWD = [_P, _LL, _P, _LL, _P, _I, _P, _P, _P, _P, _P, _P, _LL, _I, _I, _P]
 _DT = {torch.bfloat16: 0, torch.float32: 1}
+_MAX_COLS = 1 << 30       # the kernels count columns in 32 bits
 
 
 def _rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
@@ -66,8 +67,8 @@ def _ln_param(name: str, p: torch.Tensor, x: torch.Tensor, cols: int) -> None:
 def _ln_check(x: torch.Tensor, gamma, beta=None) -> int:
     if x.dtype not in _DT:
         raise TypeError(f"layer norm takes bf16 or fp32 rows, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("layer norm needs at least one column")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= _MAX_COLS:
+        raise ValueError("layer norm needs at least one column, and at most 2^30")
     cols = x.shape[-1]
     if gamma is not None:
         _ln_param("gamma", gamma, x, cols)

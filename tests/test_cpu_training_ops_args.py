@@ -53,6 +53,23 @@ def test_layer_norm_wrappers():
         layer_norm_bwd(x, g, x, mean, rstd)
 
 
+def test_widths_beyond_32_bits():
+    """A width is a 32-bit number in the kernels: one that does not fit is refused, not cut off."""
+    from parallelkernelbench_b200.ops import layer_norm, layer_norm_bwd
+    from parallelkernelbench_b200.ops.moe import ExpertSort, permute_tokens, unpermute_tokens, unpermute_tokens_bwd
+
+    for cols in ((1 << 30) + 1, (1 << 32) + 8):
+        x = torch.zeros(1, 1).expand(1, cols)
+        with pytest.raises(ValueError, match="column"):
+            layer_norm(x)
+        with pytest.raises(ValueError, match="column"):
+            layer_norm_bwd(x, None, x, torch.zeros(1), torch.zeros(1))
+        srt = ExpertSort(torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), 1, 1)
+        for call in (lambda: permute_tokens(x, srt), lambda: unpermute_tokens(x, srt), lambda: unpermute_tokens_bwd(x, x, srt, torch.ones(1, 1))):
+            with pytest.raises(ValueError, match="column"):
+                call()
+
+
 def test_expert_sort_wrappers():
     from parallelkernelbench_b200.ops.moe import (ExpertSort, permute_tokens, permute_tokens_bwd, sort_by_expert, unpermute_tokens,
                                                   unpermute_tokens_bwd)
