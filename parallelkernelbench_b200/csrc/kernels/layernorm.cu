@@ -1110,12 +1110,12 @@ struct LnRingPlan {
   int threads, per, together, blocks, stages, row_stage, smem;
 };
 // aligned: rows are whole multiples of 16 bytes that start on 16 bytes
-bool ln_ring_plan(LnRingPlan& r, long long rows, int cols, int esize, bool backward, bool aligned) {
+bool ln_ring_plan(LnRingPlan& r, long long rows, int cols, int esize, bool backward, bool aligned, int sms) {
   if (cols <= 1024 || cols > (!aligned || (backward && esize == 4) ? 8192 : 16384)) return false;
   r.threads = cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
   r.per = cols > 8192 ? 32 : !aligned && cols <= 10 * r.threads ? 10 : 16;
   const int per_sm = 512 / r.threads;
-  r.blocks = sm_count() * per_sm;
+  r.blocks = sms * per_sm;
   r.together = !backward && r.per <= 16 ? 2 : 1;
   r.row_stage = aligned ? cols * esize : (cols * esize + 15) / 16 * 16 + 16;
   const int stage = r.row_stage * (backward ? 2 : r.together);
@@ -1207,8 +1207,8 @@ int ln_fwd_any(const void* xv, long long ldx, LnParam g, LnParam b, void* yv, fl
   T* y = static_cast<T*>(yv);
   const bool vec = cols % VEC16 == 0 && ln_aligned(x, ldx * (long long)sizeof(T)) && ln_aligned(y, 0) && ln_aligned(g.p, 0) && ln_aligned(b.p, 0);
   LnRingPlan ring;
-  if (vec && ln_ring_plan(ring, rows, cols, sizeof(T), false, true)) return ln_fwd_ring<T>(ring, x, ldx, g, b, y, mean, rstd, rows, cols, eps, s);
-  if (!vec && ln_ring_plan(ring, rows, cols, sizeof(T), false, false)) return ln_fwd_odd<T>(ring, x, ldx, g, b, y, mean, rstd, rows, cols, eps, s);
+  if (vec && ln_ring_plan(ring, rows, cols, sizeof(T), false, true, sm_count())) return ln_fwd_ring<T>(ring, x, ldx, g, b, y, mean, rstd, rows, cols, eps, s);
+  if (!vec && ln_ring_plan(ring, rows, cols, sizeof(T), false, false, sm_count())) return ln_fwd_odd<T>(ring, x, ldx, g, b, y, mean, rstd, rows, cols, eps, s);
   if (cols > kLnTeamCols) {
     const long long most = (long long)sm_count() * 4;
     ln_fwd_long_kernel<T><<<(unsigned)(rows < most ? rows : most), kLnLongThreads, 0, s>>>(x, ldx, g, b, y, mean, rstd, rows, cols, eps);
@@ -1232,7 +1232,7 @@ int ln_bwd_team(const T* x, long long ldx, const T* dy, long long lddy, LnParam 
                 float* dbeta, float* part, int blocks, long long rows, int cols, cudaStream_t s) {
   auto go = [&](auto tpr, auto ch) -> int {
     using L = LnTeam<T, VEC, tpr.value, ch.value>;
-    if (!ln_bwd_one_launch(rows, cols)) {
+    if (blocks > 0) {
       ln_bwd_kernel<T, VEC, tpr.value, ch.value, false><<<blocks, L::kThreads, 0, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, part, dgamma, dbeta, rows, cols);
       PKB_CHECK_CUDA(cudaGetLastError());
       return kApiOk;
@@ -1258,12 +1258,29 @@ int ln_bwd_team(const T* x, long long ldx, const T* dy, long long lddy, LnParam 
   return ln_by_width<decltype(go)&, T, VEC, true>(cols, go);
 }
 
-// blocks of the backward's team form (rows of a block at once, blocks per SM) or slices of its long form
-int ln_bwd_blocks(long long rows, int cols) {
-  if (cols > kLnTeamCols) return (int)(rows < 4 * kLnLongSlices ? (rows + 3) / 4 : kLnLongSlices);
-  const int per = ln_bwd_team_rows(cols);
-  const long long want = (rows + per - 1) / per, most = (long long)sm_count() * (cols <= 4096 ? 2 : 1);
-  return (int)(want < most ? want : most);
+// How the backward goes. What it writes (the blocks' partial sums) and what the caller is told to bring follow from this one decision.
+struct LnBwdForm {
+  enum Kind { kCluster, kRing, kOdd, kLong, kTeam } kind;
+  LnRingPlan ring;
+  int blocks;       // that write partial sums [2][cols] each; 0: none
+};
+LnBwdForm ln_bwd_form(long long rows, int cols, int esize, bool aligned, int sms) {
+  LnBwdForm f = {};
+  if (ln_bwd_one_launch(rows, cols)) {
+    f.kind = LnBwdForm::kCluster;
+  } else if (ln_ring_plan(f.ring, rows, cols, esize, true, aligned, sms)) {
+    f.kind = aligned ? LnBwdForm::kRing : LnBwdForm::kOdd;
+    f.blocks = f.ring.blocks;
+  } else if (cols > kLnTeamCols) {      // row slices of the weights' sums
+    f.kind = LnBwdForm::kLong;
+    f.blocks = (int)(rows < 4 * kLnLongSlices ? (rows + 3) / 4 : kLnLongSlices);
+  } else {                              // rows of a block at once, blocks per SM
+    f.kind = LnBwdForm::kTeam;
+    const int per = ln_bwd_team_rows(cols);
+    const long long want = (rows + per - 1) / per, most = (long long)sms * (cols <= 4096 ? 2 : 1);
+    f.blocks = (int)(want < most ? want : most);
+  }
+  return f;
 }
 
 template <typename T, int VEC16>
@@ -1271,27 +1288,25 @@ int ln_bwd_any(const void* xv, long long ldx, const void* dyv, long long lddy, L
                float* dgamma, float* dbeta, float* part, long long rows, int cols, cudaStream_t s) {
   const T *x = static_cast<const T*>(xv), *dy = static_cast<const T*>(dyv);
   T* dx = static_cast<T*>(dxv);
-  int blocks = ln_bwd_blocks(rows, cols);
   const bool vec = cols % VEC16 == 0 && ln_aligned(x, ldx * (long long)sizeof(T)) && ln_aligned(dy, lddy * (long long)sizeof(T)) &&
                    ln_aligned(dx, 0) && ln_aligned(g.p, 0) && ln_aligned(part, 0);
-  LnRingPlan ring;
-  if (vec && ln_ring_plan(ring, rows, cols, sizeof(T), true, true)) {
-    blocks = ring.blocks;
-    const int rc = ln_bwd_ring<T>(ring, x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, s);
+  const LnBwdForm form = ln_bwd_form(rows, cols, sizeof(T), vec, sm_count());
+  PKB_CHECK_ARG(part != nullptr || form.blocks == 0, "scratch for the partial sums");
+  if (form.kind == LnBwdForm::kRing) {
+    const int rc = ln_bwd_ring<T>(form.ring, x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, s);
     if (rc) return rc;
-  } else if (ln_ring_plan(ring, rows, cols, sizeof(T), true, false)) {
-    blocks = ring.blocks;
-    const int rc = ln_bwd_odd<T>(ring, x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, s);
+  } else if (form.kind == LnBwdForm::kOdd) {
+    const int rc = ln_bwd_odd<T>(form.ring, x, ldx, dy, lddy, g, mean, rstd, dx, part, rows, cols, s);
     if (rc) return rc;
-  } else if (cols > kLnTeamCols) {
+  } else if (form.kind == LnBwdForm::kLong) {
     const long long most = (long long)sm_count() * 4;
     ln_bwd_long_dx_kernel<T><<<(unsigned)(rows < most ? rows : most), kLnLongThreads, 0, s>>>(x, ldx, dy, lddy, g, mean, rstd, dx, rows, cols);
-    ln_bwd_long_params_kernel<T><<<dim3((unsigned)((cols + 63) / 64), (unsigned)blocks), 256, 0, s>>>(x, ldx, dy, lddy, mean, rstd, part, rows, cols);
+    ln_bwd_long_params_kernel<T><<<dim3((unsigned)((cols + 63) / 64), (unsigned)form.blocks), 256, 0, s>>>(x, ldx, dy, lddy, mean, rstd, part, rows, cols);
     PKB_CHECK_CUDA(cudaGetLastError());
   } else {
-    const int rc = vec ? ln_bwd_team<T, VEC16>(x, ldx, dy, lddy, g, mean, rstd, dx, dgamma, dbeta, part, blocks, rows, cols, s)
-                       : ln_bwd_team<T, 1>(x, ldx, dy, lddy, g, mean, rstd, dx, dgamma, dbeta, part, blocks, rows, cols, s);
-    if (rc || ln_bwd_one_launch(rows, cols)) return rc;
+    const int rc = vec ? ln_bwd_team<T, VEC16>(x, ldx, dy, lddy, g, mean, rstd, dx, dgamma, dbeta, part, form.blocks, rows, cols, s)
+                       : ln_bwd_team<T, 1>(x, ldx, dy, lddy, g, mean, rstd, dx, dgamma, dbeta, part, form.blocks, rows, cols, s);
+    if (rc || form.kind == LnBwdForm::kCluster) return rc;
   }
   const long long width = 2ll * cols;
   cudaLaunchConfig_t cfg = {};
@@ -1303,7 +1318,7 @@ int ln_bwd_any(const void* xv, long long ldx, const void* dyv, long long lddy, L
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  PKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, ln_bwd_params_kernel, (const float*)part, blocks, width, dgamma, dbeta, cols));
+  PKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, ln_bwd_params_kernel, (const float*)part, form.blocks, width, dgamma, dbeta, cols));
   return kApiOk;
 }
 
@@ -1326,15 +1341,17 @@ extern "C" int pkb_layer_norm_fwd(const void* x, long long ldx, const void* gamm
                : ln_fwd_any<__nv_bfloat16, 8>(x, ldx, g, b, y, static_cast<float*>(mean), static_cast<float*>(rstd), rows, cols, eps, s);
 }
 
-// Blocks whose partial sums pkb_layer_norm_bwd writes: its scratch is [this][2][cols] fp32.
-// (An upper bound over the forms that rows of this width may take: alignment decides between them.) 0: one launch, no scratch.
+// Blocks whose partial sums pkb_layer_norm_bwd writes on a GPU of `sms` SMs (0: the current device): its scratch is [this][2][cols] fp32.
+// aligned: 1 where base, pitch and width of x and dy and the addresses of gamma, dx and the scratch are multiples of 16 bytes, else 0.
+extern "C" int pkb_layer_norm_bwd_blocks(long long rows, int cols, int dtype, int aligned, int sms) {
+  if (rows <= 0 || cols <= 0) return 0;
+  return ln_bwd_form(rows, cols, dtype ? 4 : 2, aligned != 0, sms > 0 ? sms : sm_count()).blocks;
+}
+
+// The same whatever the alignment: the larger of the two. 0: one launch, no scratch.
 extern "C" int pkb_layer_norm_bwd_partials(long long rows, int cols, int dtype) {
-  if (rows <= 0 || cols <= 0 || ln_bwd_one_launch(rows, cols)) return 0;
-  LnRingPlan ring;
-  int blocks = ln_bwd_blocks(rows, cols);
-  for (const bool aligned : {true, false})
-    if (ln_ring_plan(ring, rows, cols, dtype ? 4 : 2, true, aligned) && ring.blocks > blocks) blocks = ring.blocks;
-  return blocks;
+  const int a = pkb_layer_norm_bwd_blocks(rows, cols, dtype, 1, 0), b = pkb_layer_norm_bwd_blocks(rows, cols, dtype, 0, 0);
+  return a > b ? a : b;
 }
 
 // dx [rows, cols] (contiguous, the type of x and dy), dgamma and dbeta fp32 [cols] from the saved statistics.
@@ -1344,7 +1361,6 @@ extern "C" int pkb_layer_norm_bwd(const void* x, long long ldx, const void* dy, 
   PKB_CHECK_ARG(rows > 0 && cols > 0, "empty problem");
   PKB_CHECK_ARG(x && dy && mean && rstd && dx && dgamma && dbeta, "null pointer");
   PKB_CHECK_ARG(dtype == 0 || dtype == 1, "dtype must be 0 (bf16) or 1 (fp32)");
-  PKB_CHECK_ARG(partial != nullptr || ln_bwd_one_launch(rows, cols), "scratch for the partial sums");
   const LnParam g{gamma, param_f32, 1.f};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto f = [](void* p) { return static_cast<float*>(p); };

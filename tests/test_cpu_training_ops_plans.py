@@ -1,0 +1,39 @@
+"""What the layer-norm and orthogonalisation entry points decide on the host before any launch, so without a GPU."""
+import ctypes
+
+import pytest
+
+LL = ctypes.c_longlong
+
+
+def _blocks(rows, cols, dtype, aligned, sms):
+    from parallelkernelbench_b200 import _native as nv
+
+    return nv.cuda_lib().pkb_layer_norm_bwd_blocks(LL(rows), cols, dtype, aligned, sms)
+
+
+@pytest.mark.parametrize("sms", [1, 16, 36, 60, 64, 132, 148, 160])
+def test_backward_without_scratch_writes_none(sms):
+    """A backward that is told to bring no scratch (one launch of a cluster) must not take a form that writes partial sums, whatever the alignment and
+    however few SMs there are: on 60 of them 128 rows of 8192 columns are also enough rows for the ring."""
+    for dtype in (0, 1):
+        for cols in (1, 64, 512, 513, 1024, 1025, 1032, 2048, 2049, 4096, 4097, 8192, 8193, 16384, 16392):
+            team_rows = 1 if cols > 4096 else 256 // (32 if cols <= 512 else 64 if cols <= 1024 else 128 if cols <= 2048 else 256)
+            most = 8 * 16 * team_rows
+            for rows in {1, 2, 2 * sms, 2 * sms + 1, 4 * sms + 1, 8 * sms + 1, most - 1, most, most + 1, 5000}:
+                both = [_blocks(rows, cols, dtype, aligned, sms) for aligned in (0, 1)]
+                if cols <= 8192 and rows <= most:
+                    assert both == [0, 0], (rows, cols, dtype, both)
+                else:
+                    assert min(both) >= 1, (rows, cols, dtype, both)
+
+
+def test_scratch_holds_what_either_alignment_writes():
+    from parallelkernelbench_b200 import _native as nv
+
+    for dtype in (0, 1):
+        for cols in (33, 1001, 1032, 4096, 8192, 9001, 16384, 20001):
+            for rows in (1, 100, 257, 600, 1300, 2400, 9001):
+                told = nv.cuda_lib().pkb_layer_norm_bwd_partials(LL(rows), cols, dtype)
+                assert told == max(_blocks(rows, cols, dtype, aligned, 0) for aligned in (0, 1)) <= 4 * 160
+    assert _blocks(0, 8, 0, 1, 0) == _blocks(8, 0, 0, 1, 0) == 0
