@@ -42,8 +42,9 @@ int pkb_layer_norm_fwd(const void* x, long long ldx, const void* gamma, const vo
                        long long rows, int cols, float eps, int dtype, void* stream);
 // Its backward: dx, and dgamma, dbeta fp32 [cols]; partial: pkb_layer_norm_bwd_partials(rows, cols, dtype) x 2 x cols fp32 values.
 int pkb_layer_norm_bwd_partials(long long rows, int cols, int dtype);
-// What it writes of that on a GPU of `sms` SMs (0: the current device), for tensors on 16 bytes throughout or not.
+// What it writes of that on a GPU of `sms` SMs (0: the current device), for tensors on 16 bytes throughout or not, and its number of launches.
 int pkb_layer_norm_bwd_blocks(long long rows, int cols, int dtype, int aligned, int sms);
+int pkb_layer_norm_bwd_launches(long long rows, int cols, int dtype, int aligned, int sms);
 int pkb_layer_norm_bwd(const void* x, long long ldx, const void* dy, long long lddy, const void* gamma, int param_f32, const void* mean,
                        const void* rstd, void* dx, void* dgamma, void* dbeta, void* partial, long long rows, int cols, int dtype, void* stream);
 

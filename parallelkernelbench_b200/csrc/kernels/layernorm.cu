@@ -1263,6 +1263,7 @@ struct LnBwdForm {
   enum Kind { kCluster, kRing, kOdd, kLong, kTeam } kind;
   LnRingPlan ring;
   int blocks;       // that write partial sums [2][cols] each; 0: none
+  int launches() const { return kind == kCluster ? 1 : kind == kLong ? 3 : 2; }
 };
 LnBwdForm ln_bwd_form(long long rows, int cols, int esize, bool aligned, int sms) {
   LnBwdForm f = {};
@@ -1348,7 +1349,13 @@ extern "C" int pkb_layer_norm_bwd_blocks(long long rows, int cols, int dtype, in
   return ln_bwd_form(rows, cols, dtype ? 4 : 2, aligned != 0, sms > 0 ? sms : sm_count()).blocks;
 }
 
-// The same whatever the alignment: the larger of the two. 0: one launch, no scratch.
+// The kernels that pkb_layer_norm_bwd launches, arguments as above.
+extern "C" int pkb_layer_norm_bwd_launches(long long rows, int cols, int dtype, int aligned, int sms) {
+  if (rows <= 0 || cols <= 0) return 0;
+  return ln_bwd_form(rows, cols, dtype ? 4 : 2, aligned != 0, sms > 0 ? sms : sm_count()).launches();
+}
+
+// pkb_layer_norm_bwd_blocks whatever the alignment: the larger of the two. 0: one launch, no scratch.
 extern "C" int pkb_layer_norm_bwd_partials(long long rows, int cols, int dtype) {
   const int a = pkb_layer_norm_bwd_blocks(rows, cols, dtype, 1, 0), b = pkb_layer_norm_bwd_blocks(rows, cols, dtype, 0, 0);
   return a > b ? a : b;

@@ -112,9 +112,21 @@ def layer_norm_fwd(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: tor
 
 
 @functools.lru_cache(maxsize=256)
-def _ln_partials(rows: int, cols: int, dtype: int, device: int) -> int:
+def _ln_plan(rows: int, cols: int, dtype: int, device: int) -> tuple[int, int, int]:
+    """Blocks that write partial sums (at most), and launches where everything lies on 16 bytes and where it does not."""
+    launches = nv.bound("pkb_layer_norm_bwd_launches", [_LL, _I, _I, _I, _I])
     with torch.cuda.device(device):
-        return nv.bound("pkb_layer_norm_bwd_partials", [_LL, _I, _I])(rows, cols, dtype)
+        return (nv.bound("pkb_layer_norm_bwd_partials", [_LL, _I, _I])(rows, cols, dtype), launches(rows, cols, dtype, 1, 0),
+                launches(rows, cols, dtype, 0, 0))
+
+
+def _on_16_bytes(gamma, dx, *rows) -> bool:
+    """Base, pitch and width of ``rows``, and the addresses of ``gamma`` and ``dx``, as the backward's 16-byte accesses want them."""
+    size = dx.element_size()
+    bits = dx.data_ptr() | (0 if gamma is None else gamma.data_ptr()) | rows[0].shape[1] * size
+    for t in rows:
+        bits |= t.data_ptr() | t.stride(0) * size
+    return bits % 16 == 0
 
 
 def layer_norm_bwd(x: torch.Tensor, gamma: torch.Tensor | None, dy: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor):
@@ -134,9 +146,11 @@ def layer_norm_bwd(x: torch.Tensor, gamma: torch.Tensor | None, dy: torch.Tensor
         return dx, x.new_zeros(cols, dtype=torch.float32), x.new_zeros(cols, dtype=torch.float32)
     dgamma = torch.empty_like(gamma) if gamma is not None and gamma.dtype == torch.float32 and gamma.dim() == 1 else x.new_empty(cols, dtype=torch.float32)
     dbeta = torch.empty_like(dgamma)
-    blocks = _ln_partials(rows, cols, _DT[x.dtype], x.get_device())
+    blocks, launches, launches_off = _ln_plan(rows, cols, _DT[x.dtype], x.get_device())
+    if launches != launches_off and not _on_16_bytes(gamma, dx, x2, dy2):
+        launches = launches_off
     part = x.new_empty(blocks * 2 * cols, dtype=torch.float32) if blocks else None
     nv.launch("pkb_layer_norm_bwd", _LN_BWD, x, x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), 0 if gamma is None else gamma.data_ptr(),
               0 if gamma is None else _DT[gamma.dtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(),
-              part.data_ptr() if blocks else 0, rows, cols, _DT[x.dtype], launches=2 if blocks else 1)
+              part.data_ptr() if blocks else 0, rows, cols, _DT[x.dtype], launches=launches)
     return dx, dgamma, dbeta

@@ -37,3 +37,16 @@ def test_scratch_holds_what_either_alignment_writes():
                 told = nv.cuda_lib().pkb_layer_norm_bwd_partials(LL(rows), cols, dtype)
                 assert told == max(_blocks(rows, cols, dtype, aligned, 0) for aligned in (0, 1)) <= 4 * 160
     assert _blocks(0, 8, 0, 1, 0) == _blocks(8, 0, 0, 1, 0) == 0
+
+
+def test_launches_of_the_backward():
+    """One launch of a cluster, two with the weights' sums, three where a row goes in passes."""
+    from parallelkernelbench_b200 import _native as nv
+
+    def launches(rows, cols, dtype, aligned):
+        return nv.cuda_lib().pkb_layer_norm_bwd_launches(LL(rows), cols, dtype, aligned, 148)
+
+    assert launches(4, 4096, 0, 1) == launches(4, 4097, 1, 0) == 1
+    assert launches(4000, 64, 0, 1) == launches(8192, 4096, 0, 1) == launches(8192, 4097, 1, 0) == launches(400, 16384, 0, 1) == 2
+    assert launches(3, 8193, 0, 0) == launches(400, 16384, 0, 0) == launches(400, 16384, 1, 1) == launches(4, 20000, 0, 1) == 3
+    assert launches(0, 8, 0, 1) == launches(8, 0, 0, 1) == 0
