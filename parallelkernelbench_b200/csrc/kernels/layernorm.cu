@@ -1,7 +1,9 @@
 // Layer norm, forward and backward (memory bound: a row is read once and stays in registers between its sums and its results).
 //   mean = sum x / N, rstd = 1 / sqrt(sum (x - mean)^2 / N + eps), y = (x - mean) rstd gamma + beta
 //   g = dy gamma, xhat = (x - mean) rstd, dx = rstd (g - mean(g) - xhat mean(g xhat)), dgamma = sum_rows dy xhat, dbeta = sum_rows dy
-// The variance is the mean of squared differences from the mean, never E[x^2] - mean^2: a row far from zero loses nothing.
+// Forward, a row's sum gives a first mean m0, rounded to fp32 like every value near it. From d = x - m0, which is small and nearly exact, come
+// delta = sum d / N, mean = m0 + delta, variance = (sum d^2 - delta sum d) / N and y = (d - delta) rstd gamma + beta: with m0 alone a constant row of 1e5
+// at 1000 columns (sum / N an ulp off) came out at -0.93 instead of 0. Never E[x^2] - mean^2.
 // A row belongs to a team of TPR threads that holds VEC * CH of its values each: 16-byte accesses where base, row pitch and width
 // allow them (VEC = 8 bf16 or 4 fp32), single values otherwise. All sums are fp32.
 // Forms, by width, alignment and number of rows (ln_fwd_any, ln_bwd_any): teams of 32 to 512 threads straight from global memory; from 1025 columns
@@ -136,6 +138,62 @@ __device__ __forceinline__ void team_sum(float (&v)[K], float* red, int team) {
   }
 }
 
+// The same for K = 2 or 4 with fewer shuffles (K = 4 over 16 warps: 13 instead of 36): the first exchanges halve the values that a lane still adds
+// for, lane l ending up with value l / (32 / K), and a value's lanes share the warps' sums among them. 16384 x 8192 bf16 forward 121 us without, 111
+// with, backward 143 and 140. (The backward kernels outside the aligned ring have no registers left for the exchanges: 8192 x 4097 bf16 101 and 113.)
+template <int K, int TPR, int NT>
+__device__ __forceinline__ void team_sum_shared(float (&v)[K], float* red, int team) {
+  static_assert(K == 1 || K == 2 || K == 4, "values per lane");
+  if constexpr (K == 1) {
+    team_sum<1, TPR, NT>(v, red, team);
+  } else {
+    constexpr unsigned kAll = 0xffffffffu;
+    constexpr int G = 32 / K;       // lanes per value
+    const int lane = threadIdx.x & 31;
+    const bool up = lane & 16;
+    float s;
+    if constexpr (K == 2) {
+      s = (up ? v[1] : v[0]) + __shfl_xor_sync(kAll, up ? v[0] : v[1], 16);
+      s += __shfl_xor_sync(kAll, s, 8);
+    } else {
+      const bool odd = lane & 8;
+      const float a = (up ? v[2] : v[0]) + __shfl_xor_sync(kAll, up ? v[0] : v[2], 16);
+      const float b = (up ? v[3] : v[1]) + __shfl_xor_sync(kAll, up ? v[1] : v[3], 16);
+      s = (odd ? b : a) + __shfl_xor_sync(kAll, odd ? a : b, 8);
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+    if constexpr (TPR > 32) {
+      constexpr int W = TPR / 32, S = W < G ? W : G;       // warps, lanes that add different warps' sums
+      if (lane % G == 0) red[lane / G * (NT / 32) + (threadIdx.x >> 5)] = s;
+      team_sync<TPR, NT>(team);
+      const float* r = red + lane / G * (NT / 32) + team * W + lane % S;
+      s = r[0];
+#pragma unroll
+      for (int i = S; i < W; i += S) s += r[i];
+#pragma unroll
+      for (int o = S / 2; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = __shfl_sync(kAll, s, k * G);
+  }
+}
+
+// A row's statistics from its first mean m0, the sum of its differences from it and the sum of their squares (see the top). The quotient takes its
+// remainder into account, so that it is exact where it can be: a constant row, whose differences are one number of a few bits, has no variance and
+// nothing left of it. (With divisions here and for m0: 16384 x 8192 bf16 116 us instead of 111.)
+struct LnStats {
+  float delta, mean, rstd;
+  __device__ __forceinline__ LnStats(float m0, float sum, float squares, int cols, float inv, float eps) {
+    delta = sum * inv;
+    delta = fmaf(fmaf(-delta, (float)cols, sum), inv, delta);
+    mean = m0 + delta;
+    float q = fmaf(-sum, delta, squares);
+    if (!(q >= 0.f)) q = isfinite(squares) ? 0.f : squares;      // rounding, or squares that left fp32
+    rstd = rsqrtf(fmaf(q, inv, eps));
+  }
+};
+
 template <typename T, int VEC, int TPR, int CH>
 struct LnTeam {
   static constexpr int kThreads = TPR > 256 ? TPR : 256;
@@ -143,12 +201,13 @@ struct LnTeam {
   static constexpr int kCols = TPR * VEC * CH;      // widest row
 };
 
+// (Single values: at most 64 registers, so that 1024 threads are resident: 16384 x 1001 bf16 38 us, 42 without.)
 template <typename T, int VEC, int TPR, int CH>
-__global__ void __launch_bounds__(LnTeam<T, VEC, TPR, CH>::kThreads)
+__global__ void __launch_bounds__(LnTeam<T, VEC, TPR, CH>::kThreads, VEC == 1 ? 1024 / LnTeam<T, VEC, TPR, CH>::kThreads : 0)
 ln_fwd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, const LnParam beta, T* __restrict__ y,
               float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, int cols, float eps) {
   using L = LnTeam<T, VEC, TPR, CH>;
-  __shared__ float red[2][L::kThreads / 32];
+  __shared__ float red[2][2 * (L::kThreads / 32)];
   const int team = threadIdx.x / TPR, t = threadIdx.x % TPR;
   const float inv = 1.f / (float)cols;
   for (long long row = (long long)blockIdx.x * L::kRows + team; row < rows; row += (long long)gridDim.x * L::kRows) {
@@ -169,20 +228,24 @@ ln_fwd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, const
 #pragma unroll
       for (int j = 0; j < VEC; ++j) s[0] += v[ch][j];
     team_sum<1, TPR, L::kThreads>(s, red[0], team);
-    const float mean = s[0] * inv;
-    float q[1] = {0.f};
+    const float m0 = s[0] * inv;
+    float q[2] = {0.f, 0.f};
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       if ((ch * TPR + t) * VEC < cols) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) q[0] += (v[ch][j] - mean) * (v[ch][j] - mean);
+        for (int j = 0; j < VEC; ++j) {
+          v[ch][j] -= m0;
+          q[0] += v[ch][j];
+          q[1] += v[ch][j] * v[ch][j];
+        }
       }
     }
-    team_sum<1, TPR, L::kThreads>(q, red[1], team);
-    const float rstd = rsqrtf(q[0] * inv + eps);
+    team_sum_shared<2, TPR, L::kThreads>(q, red[1], team);
+    const LnStats st(m0, q[0], q[1], cols, inv, eps);
     if (t == 0 && mean_out != nullptr) {
-      mean_out[row] = mean;
-      rstd_out[row] = rstd;
+      mean_out[row] = st.mean;
+      rstd_out[row] = st.rstd;
     }
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
@@ -192,7 +255,7 @@ ln_fwd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, const
         gamma.template load<VEC>(c, g);
         beta.template load<VEC>(c, b);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[ch][j] = (v[ch][j] - mean) * rstd * g[j] + b[j];
+        for (int j = 0; j < VEC; ++j) v[ch][j] = (v[ch][j] - st.delta) * st.rstd * g[j] + b[j];
         ln_store<T, VEC>(y + row * cols + c, v[ch]);
       }
     }
@@ -206,26 +269,27 @@ template <typename T>
 __global__ void __launch_bounds__(kLnLongThreads)
 ln_fwd_long_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, const LnParam beta, T* __restrict__ y,
                    float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, int cols, float eps) {
-  __shared__ float red[2][kLnLongThreads / 32];
+  __shared__ float red[2][2 * (kLnLongThreads / 32)];
   const float inv = 1.f / (float)cols;
   for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * ldx;
-    float s[1] = {0.f}, q[1] = {0.f};
+    float s[1] = {0.f}, q[2] = {0.f, 0.f};
     for (int c = threadIdx.x; c < cols; c += kLnLongThreads) s[0] += static_cast<float>(xr[c]);
     team_sum<1, kLnLongThreads, kLnLongThreads>(s, red[0], 0);
-    const float mean = s[0] * inv;
+    const float m0 = s[0] * inv;
     for (int c = threadIdx.x; c < cols; c += kLnLongThreads) {
-      const float d = static_cast<float>(xr[c]) - mean;
-      q[0] += d * d;
+      const float d = static_cast<float>(xr[c]) - m0;
+      q[0] += d;
+      q[1] += d * d;
     }
-    team_sum<1, kLnLongThreads, kLnLongThreads>(q, red[1], 0);
-    const float rstd = rsqrtf(q[0] * inv + eps);
+    team_sum_shared<2, kLnLongThreads, kLnLongThreads>(q, red[1], 0);
+    const LnStats st(m0, q[0], q[1], cols, inv, eps);
     if (threadIdx.x == 0 && mean_out != nullptr) {
-      mean_out[row] = mean;
-      rstd_out[row] = rstd;
+      mean_out[row] = st.mean;
+      rstd_out[row] = st.rstd;
     }
     for (int c = threadIdx.x; c < cols; c += kLnLongThreads) {
-      const float f[1] = {(static_cast<float>(xr[c]) - mean) * rstd * gamma.at(c) + beta.at(c)};
+      const float f[1] = {((static_cast<float>(xr[c]) - m0) - st.delta) * st.rstd * gamma.at(c) + beta.at(c)};
       ln_store<T, 1>(y + row * cols + c, f);
     }
   }
@@ -478,7 +542,7 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
   constexpr int VEC = 16 / sizeof(T), CH = PER / VEC, P = VEC / 2;
   constexpr bool kHoldGain = PER <= 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float red[2][R * (NT / 32)];
+  __shared__ float red[2][2 * R * (NT / 32)];
   __shared__ int abort_flag;
   const uint32_t bytes = (uint32_t)cols * sizeof(T);
   const LnRing ring = ln_ring_init(smem, stages, R * bytes, &abort_flag);
@@ -512,7 +576,7 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
     ok = ok && ln_ring_wait(ring, stage, parity, &abort_flag, status, grp);
     const int here = R == 1 ? 1 : (int)min((long long)R, rows - grp * R);
     F2 v[R][CH][P];
-    float s[R], q[R], rstd[R];
+    float s[R], q[2 * R], rstd[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       F2 acc = 0;
@@ -527,7 +591,7 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
       }
       s[i] = f2_sum(acc);
     }
-    team_sum<R, NT, NT>(s, red[0], 0);
+    team_sum_shared<R, NT, NT>(s, red[0], 0);
     if (t == 0 && ok && grp + (long long)stages * gridDim.x < groups) {
       fence_proxy_async_smem();
       issue(grp + (long long)stages * gridDim.x, stage);
@@ -536,26 +600,31 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
     for (int i = 0; i < R; ++i) {
       s[i] *= inv;
       const F2 shift = f2(-s[i]);
-      F2 acc = 0;
+      F2 sum = 0, squares = 0;
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch) {
         if ((ch * NT + t) * VEC < cols) {
 #pragma unroll
           for (int j = 0; j < P; ++j) {
             v[i][ch][j] = add2(v[i][ch][j], shift);
-            acc = fma2(v[i][ch][j], v[i][ch][j], acc);
+            sum = add2(sum, v[i][ch][j]);
+            squares = fma2(v[i][ch][j], v[i][ch][j], squares);
           }
         }
       }
-      q[i] = f2_sum(acc);
+      q[2 * i] = f2_sum(sum);
+      q[2 * i + 1] = f2_sum(squares);
     }
-    team_sum<R, NT, NT>(q, red[1], 0);
+    team_sum_shared<2 * R, NT, NT>(q, red[1], 0);
+    F2 shift[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      rstd[i] = rsqrtf(q[i] * inv + eps);
+      const LnStats st(s[i], q[2 * i], q[2 * i + 1], cols, inv, eps);
+      rstd[i] = st.rstd;
+      shift[i] = f2(-st.delta);
       if (t == 0 && i < here && mean_out != nullptr) {
-        mean_out[grp * R + i] = s[i];
-        rstd_out[grp * R + i] = rstd[i];
+        mean_out[grp * R + i] = st.mean;
+        rstd_out[grp * R + i] = st.rstd;
       }
     }
 #pragma unroll
@@ -572,7 +641,7 @@ ln_fwd_ring_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, 
           if (i < here) {
             const F2 r2 = f2(rstd[i]);
 #pragma unroll
-            for (int j = 0; j < P; ++j) v[i][ch][j] = fma2(mul2(v[i][ch][j], r2), g[kAt * ch][j], b[kAt * ch][j]);
+            for (int j = 0; j < P; ++j) v[i][ch][j] = fma2(mul2(add2(v[i][ch][j], shift[i]), r2), g[kAt * ch][j], b[kAt * ch][j]);
             ln_store_pairs<T, VEC>(y + (grp * R + i) * cols + c, v[i][ch]);
           }
         }
@@ -655,7 +724,7 @@ ln_bwd_ring_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__
       }
     }
     float s[2] = {f2_sum(s1), f2_sum(s2)};
-    team_sum<2, NT, NT>(s, red[it], 0);
+    team_sum_shared<2, NT, NT>(s, red[it], 0);
     if (t == 0 && ok && row + (long long)stages * gridDim.x < rows) {
       fence_proxy_async_smem();
       issue(row + (long long)stages * gridDim.x, stage);
@@ -800,7 +869,7 @@ ln_fwd_odd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, c
                   uint32_t* status) {
   constexpr int P = PER / 2;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float red[2][R * (NT / 32)];
+  __shared__ float red[2][2 * R * (NT / 32)];
   __shared__ int abort_flag;
   const uint32_t bytes = (uint32_t)cols * sizeof(T);
   const LnRing ring = ln_ring_init(smem, stages, R * row_stage, &abort_flag);
@@ -834,7 +903,7 @@ ln_fwd_odd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, c
     ok = ok && ln_ring_wait(ring, stage, parity, &abort_flag, status, grp);
     const int here = R == 1 ? 1 : (int)min((long long)R, rows - grp * R);
     F2 v[R][P];
-    float s[R] = {}, q[R] = {}, rstd[R];
+    float s[R] = {}, q[2 * R] = {};
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       F2 acc = 0;
@@ -845,7 +914,7 @@ ln_fwd_odd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, c
       }
       s[i] = f2_sum(acc);
     }
-    team_sum<R, NT, NT>(s, red[0], 0);
+    team_sum_shared<R, NT, NT>(s, red[0], 0);
     if (t == 0 && ok && grp + (long long)stages * gridDim.x < groups) {
       fence_proxy_async_smem();
       issue(grp + (long long)stages * gridDim.x, stage);
@@ -854,7 +923,7 @@ ln_fwd_odd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, c
     for (int i = 0; i < R; ++i) {
       s[i] *= inv;
       const F2 shift = f2(-s[i]);
-      F2 acc = 0;
+      F2 sum = 0, squares = 0;
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         v[i][j] = add2(v[i][j], shift);
@@ -862,23 +931,25 @@ ln_fwd_odd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, c
           const float2 w = f2_split(v[i][j]);
           v[i][j] = f2(col(2 * j) < cols ? w.x : 0.f, col(2 * j + 1) < cols ? w.y : 0.f);
         }
-        acc = fma2(v[i][j], v[i][j], acc);
+        sum = add2(sum, v[i][j]);
+        squares = fma2(v[i][j], v[i][j], squares);
       }
-      q[i] = f2_sum(acc);
+      q[2 * i] = f2_sum(sum);
+      q[2 * i + 1] = f2_sum(squares);
     }
-    team_sum<R, NT, NT>(q, red[1], 0);
+    team_sum_shared<2 * R, NT, NT>(q, red[1], 0);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (i >= here) break;
-      rstd[i] = rsqrtf(q[i] * inv + eps);
+      const LnStats st(s[i], q[2 * i], q[2 * i + 1], cols, inv, eps);
       if (t == 0 && mean_out != nullptr) {
-        mean_out[grp * R + i] = s[i];
-        rstd_out[grp * R + i] = rstd[i];
+        mean_out[grp * R + i] = st.mean;
+        rstd_out[grp * R + i] = st.rstd;
       }
-      const F2 r2 = f2(rstd[i]);
+      const F2 r2 = f2(st.rstd), shift = f2(-st.delta);
       T* yr = y + (grp * R + i) * cols;
 #pragma unroll
-      for (int j = 0; j < P; ++j) odd_store<T, NT, P>(yr, j, fma2(mul2(v[i][j], r2), g[j], b[j]), cols);
+      for (int j = 0; j < P; ++j) odd_store<T, NT, P>(yr, j, fma2(mul2(add2(v[i][j], shift), r2), g[j], b[j]), cols);
     }
     if (++stage == stages) {
       stage = 0;

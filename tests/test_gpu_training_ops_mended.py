@@ -22,3 +22,53 @@ def test_layer_norm_backward_counts_its_launches(rows, cols, dtype, shift, launc
     before = nv.launches()
     layer_norm_bwd(x, None, x, mean, rstd)
     assert nv.launches() - before == launches
+
+
+# every form of the forward: teams with wide and single accesses, the ring at each of its widths, the ring of rows that start anywhere, rows in passes
+MEAN_SHAPES = [(5, 1000), (5, 1001), (2, 4097), (3, 7168), (9, 520), (9, 40), (2400, 1032), (1185, 4000), (400, 7168), (303, 12288), (1300, 1101), (700, 4097),
+               (310, 7169), (3, 9000), (2, 16400)]
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", MEAN_SHAPES)
+def test_layer_norm_of_constant_rows(rows, cols, dtype):
+    """Every difference from the first mean is the same small multiple of a step of fp32, so their sum, its quotient and what they leave are exact: the
+    mean is the constant, the deviation is eps alone, and the result is the bias."""
+    from parallelkernelbench_b200.ops import layer_norm_bwd, layer_norm_fwd
+
+    values = torch.tensor([1e5, 99840.0, -1000.0, 0.1, 1e3, -3e4, 123.456, 7e-3], device="cuda").to(dtype)
+    x = values[torch.arange(rows, device="cuda") % len(values)][:, None].expand(rows, cols).contiguous()
+    beta = torch.randn(cols, device="cuda", generator=_gen(3))
+    y, mean, rstd = layer_norm_fwd(x, None, beta)
+    assert torch.equal(y, beta.to(dtype).expand(rows, cols))
+    assert torch.equal(mean, x[:, 0].float())
+    assert ((rstd.double() * 1e-5 ** 0.5 - 1).abs() <= 2.0 ** -21).all()
+    dy = torch.randn(rows, cols, device="cuda", generator=_gen(4)).to(dtype)
+    dx, dgamma, _ = layer_norm_bwd(x, None, dy, mean, rstd)
+    assert not dgamma.any()
+    want = rstd.double()[:, None] * (dy.double() - dy.double().mean(1, keepdim=True))
+    slack = rstd.double()[:, None] * ((cols / 512 + 64) * U * dy.double().abs().mean(1, keepdim=True) + 4 * U * dy.double().abs())
+    assert ((dx.double() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + 1.01 * slack).all()
+
+
+@pytest.mark.parametrize("center", [1e3, -3e4, 1e5])
+@pytest.mark.parametrize("rows,cols", MEAN_SHAPES)
+def test_layer_norm_of_nearly_constant_rows(rows, cols, center):
+    """Rows a few steps of fp32 wide. With K = cols / 512 + 64 terms on the way of a sum, the first mean m0 is off by K U |x|; x - m0 is exact (the two
+    are within a factor of two of one another); its mean is then off by e = K U (mean|x - mean| + K U |x|) and is all that separates the result
+    from (x - mean) rstd, besides the variance's K U, halved by the root, and a few roundings of the result."""
+    from parallelkernelbench_b200.ops import layer_norm_fwd
+
+    g = _gen(cols)
+    x = center + 0.02 * torch.randn(rows, cols, device="cuda", generator=g)
+    y, mean, rstd = layer_norm_fwd(x)
+    xd = x.double()
+    m = xd.mean(1, keepdim=True)
+    d = xd - m
+    r = 1 / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-5)
+    k = cols / 512 + 64
+    e = k * U * (d.abs().mean(1, keepdim=True) + k * U * xd.abs().mean(1, keepdim=True))
+    assert ((mean.double()[:, None] - m).abs() <= U * m.abs() + e).all()
+    assert ((rstd.double()[:, None] - r).abs() <= r * (k * U + (e * r) ** 2)).all()
+    assert ((y.double() - d * r).abs() <= e * r + (k * U + (e * r) ** 2) * (d * r).abs() + 4 * U * (d * r).abs()).all()
