@@ -1265,23 +1265,26 @@ int split_ctas(long long tiles, int num_k) {
   return 1;
 }
 
+long long ns_tiles(long long batch, int rows, int cols, int size, bool symmetric) {
+  const long long num_m = (rows + size - 1) / size, num_n = (cols + size - 1) / size;
+  return (symmetric ? num_m * (num_m + 1) / 2 : num_m * num_n) * batch;
+}
+
+// One product. launch = false: only what can fail before a launch does (the kernel's limits), so that a call fails before it has changed anything.
 template <bool A_MN, bool B_MN, int EPI>
-int ns_gemm(const CUtensorMap& ta, const CUtensorMap& tb, NsParams p, cudaStream_t s) {
+int ns_gemm(const CUtensorMap& ta, const CUtensorMap& tb, NsParams p, cudaStream_t s, bool launch) {
   constexpr bool kSym = EPI == kNsGram || EPI == kNsPoly;
-  auto tiles_of = [&](int size) {
-    const long long num_m = (p.rows + size - 1) / size, num_n = (p.cols + size - 1) / size;
-    return (kSym ? num_m * (num_m + 1) / 2 : num_m * num_n) * p.batch;
-  };
-  const long long small_tiles = tiles_of(kSplitTile), tiles = tiles_of(kNsTile);
-  PKB_CHECK_ARG(tiles < (1ll << 24), "too many tiles");
+  const long long small_tiles = ns_tiles(p.batch, p.rows, p.cols, kSplitTile, kSym), tiles = ns_tiles(p.batch, p.rows, p.cols, kNsTile, kSym);
   if (const int ctas = split_ctas(small_tiles, (p.K + kGemmBlockK - 1) / kGemmBlockK)) {
     if (const int rc = prepare_kernel<ns_split_kernel<A_MN, B_MN, EPI>>(kSplitSmem, true)) return rc;
+    if (!launch) return kApiOk;
     PKB_CHECK_CUDA(launch_dependent(ns_split_kernel<A_MN, B_MN, EPI>, dim3((unsigned)(small_tiles * ctas)), kNsThreads, kSplitSmem, s, ctas, ta, tb, p));
     return kApiOk;
   }
   int ctas = sm_count() & ~1;
   if (ctas > 2 * tiles) ctas = (int)(2 * tiles);
   if (const int rc = prepare_kernel<ns_gemm_kernel<A_MN, B_MN, EPI>>(kNsSmem)) return rc;
+  if (!launch) return kApiOk;
   PKB_CHECK_CUDA(launch_dependent(ns_gemm_kernel<A_MN, B_MN, EPI>, dim3((unsigned)ctas), kNsThreads, kNsSmem, s, 0, ta, tb, p));
   return kApiOk;
 }
@@ -1358,10 +1361,11 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
   PKB_CHECK_ARG(batch > 0 && batch <= 65535 && rows > 0 && cols > 0, "1 .. 65535 matrices of at least one row and column");
   PKB_CHECK_ARG(steps >= 1 && coeff != nullptr, "at least one step");
   PKB_CHECK_ARG(g != nullptr && ((out != nullptr) != (p != nullptr)), "g, scratch and one of out and p");
-  uint32_t* status = status_block_for_launch();
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool tall = rows > cols;
   const int side = tall ? cols : rows, longer = tall ? rows : cols;
+  PKB_CHECK_ARG(small_fits(side, longer, steps) || ns_tiles(batch, rows, cols, kNsTile, false) < (1ll << 24), "too many tiles of 256 x 256");
+  uint32_t* status = status_block_for_launch();
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const long long pitch = pad8(cols), pitch_a = pad8(side), numel = (long long)rows * cols;
   const double k = ldexp(1.0, (int)lrint(log2((double)longer) / 2));
   const NsInput in{g, g_f32, static_cast<float*>(m), momentum, nesterov};
@@ -1411,14 +1415,6 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
     if (n > cap) n = cap;
     return (int)(n < 1 ? 1 : n);
   };
-  const int parts = blocks_for(vec ? numel / 16 : numel, kNsMaxParts);
-  if (vec) ns_norm_kernel<true><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
-  else ns_norm_kernel<false><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
-  PKB_CHECK_CUDA(cudaGetLastError());
-  const int start_blocks = blocks_for((long long)rows * (pitch / 8), 1 << 20);
-  PKB_CHECK_CUDA(launch_dependent(ns_start_kernel, dim3((unsigned)start_blocks, (unsigned)batch), kNsPrepThreads, 0, s, 0, in, rows, cols, (int)pitch,
-                                  part, parts, eps, k, (int)(aligned && cols % 8 == 0), master, x[0]));
-
   // maps of X as an operand whose rows lie along K (boxes of 64 columns x 128 rows) and as one whose rows are K (64 x 64), and of A and B
   CUtensorMap xk[2], xm[2], ak, bk;
   int rc;
@@ -1438,8 +1434,8 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
   q.vec_out = cols % 4 == 0 && aligned_out;
   q.status = status;
   q.wait_budget_ns = kDefaultWaitBudgetNs;
-  for (int step = 0; step < steps; ++step) {
-    const float *co = coeff + 3 * step;
+  auto step_products = [&](int step, bool launch) -> int {
+    const float* co = coeff + 3 * step;
     const int cur = step & 1;
     NsParams e = q;
     e.rows = e.cols = side;
@@ -1447,14 +1443,14 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
     e.K = longer;
     e.out16 = a16;
     e.alpha = (float)(1.0 / (k * k));
-    rc = tall ? ns_gemm<true, true, kNsGram>(xm[cur], xm[cur], e, s) : ns_gemm<false, false, kNsGram>(xk[cur], xk[cur], e, s);
+    int rc = tall ? ns_gemm<true, true, kNsGram>(xm[cur], xm[cur], e, s, launch) : ns_gemm<false, false, kNsGram>(xk[cur], xk[cur], e, s, launch);
     if (rc) return rc;
     e.K = side;
     e.a16 = a16;
     e.out16 = b16;
     e.alpha = co[2];
     e.beta = co[1];
-    rc = ns_gemm<false, false, kNsPoly>(ak, ak, e, s);
+    rc = ns_gemm<false, false, kNsPoly>(ak, ak, e, s, launch);
     if (rc) return rc;
     NsParams u = q;
     u.rows = rows;
@@ -1465,18 +1461,34 @@ extern "C" int pkb_newton_schulz(const void* g, int g_f32, void* m, float moment
     u.master = master;
     u.beta = co[0];
     if (step + 1 < steps) {
-      rc = tall ? ns_gemm<false, false, kNsUpdate>(xk[cur], bk, u, s) : ns_gemm<false, true, kNsUpdate>(bk, xm[cur], u, s);
+      rc = tall ? ns_gemm<false, false, kNsUpdate>(xk[cur], bk, u, s, launch) : ns_gemm<false, true, kNsUpdate>(bk, xm[cur], u, s, launch);
     } else if (p == nullptr) {
       u.final_out = out;
       u.alpha = (float)(1.0 / k);
-      rc = tall ? ns_gemm<false, false, kNsResult>(xk[cur], bk, u, s) : ns_gemm<false, true, kNsResult>(bk, xm[cur], u, s);
+      rc = tall ? ns_gemm<false, false, kNsResult>(xk[cur], bk, u, s, launch) : ns_gemm<false, true, kNsResult>(bk, xm[cur], u, s, launch);
     } else {
       u.final_out = p;
       u.p_bf16 = static_cast<__nv_bfloat16*>(p_bf16);
       u.alpha = (float)(scale / k);
       u.decay = decay;
-      rc = tall ? ns_gemm<false, false, kNsStep>(xk[cur], bk, u, s) : ns_gemm<false, true, kNsStep>(bk, xm[cur], u, s);
+      rc = tall ? ns_gemm<false, false, kNsStep>(xk[cur], bk, u, s, launch) : ns_gemm<false, true, kNsStep>(bk, xm[cur], u, s, launch);
     }
+    return rc;
+  };
+  // whatever can fail without a launch fails here: the first launch updates the momentum
+  for (const int step : {0, steps - 1}) {
+    rc = step_products(step, false);
+    if (rc) return rc;
+  }
+  const int parts = blocks_for(vec ? numel / 16 : numel, kNsMaxParts);
+  if (vec) ns_norm_kernel<true><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
+  else ns_norm_kernel<false><<<dim3((unsigned)parts, (unsigned)batch), kNsPrepThreads, 0, s>>>(in, numel, part);
+  PKB_CHECK_CUDA(cudaGetLastError());
+  const int start_blocks = blocks_for((long long)rows * (pitch / 8), 1 << 20);
+  PKB_CHECK_CUDA(launch_dependent(ns_start_kernel, dim3((unsigned)start_blocks, (unsigned)batch), kNsPrepThreads, 0, s, 0, in, rows, cols, (int)pitch,
+                                  part, parts, eps, k, (int)(aligned && cols % 8 == 0), master, x[0]));
+  for (int step = 0; step < steps; ++step) {
+    rc = step_products(step, true);
     if (rc) return rc;
   }
   return kApiOk;

@@ -50,3 +50,16 @@ def test_launches_of_the_backward():
     assert launches(4000, 64, 0, 1) == launches(8192, 4096, 0, 1) == launches(8192, 4097, 1, 0) == launches(400, 16384, 0, 1) == 2
     assert launches(3, 8193, 0, 0) == launches(400, 16384, 0, 0) == launches(400, 16384, 1, 1) == launches(4, 20000, 0, 1) == 3
     assert launches(0, 8, 0, 1) == launches(8, 0, 0, 1) == 0
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(65535, 1, 65537), (65535, 65537, 1), (64, 1 << 17, 1 << 17)])
+def test_too_many_tiles_are_refused_before_anything_changes(batch, rows, cols):
+    """The refusal comes before the first launch, which updates the momentum: here, where no launch can succeed, it is still the answer."""
+    from parallelkernelbench_b200 import _native as nv
+
+    p = ctypes.c_void_p(4096)
+    coeff = (ctypes.c_float * 3)(1.5, -0.5, 0.0)
+    f, d = ctypes.c_float, ctypes.c_double
+    lib = nv.cuda_lib()
+    rc = lib.pkb_newton_schulz(p, 0, p, f(0.9), 1, LL(batch), rows, cols, coeff, 1, d(1e-7), None, p, f(1), f(1), None, p, None)
+    assert rc != 0 and b"too many tiles" in lib.pkb_last_error(), lib.pkb_last_error()
