@@ -24,15 +24,20 @@ FAST = (3.4445, -4.7750, 2.0315)
 @functools.lru_cache(maxsize=64)
 def _coefficients(coefficients, steps: int, longer: int):
     """The steps' coefficients as a C array. The products run in fp16: what the singular values (at most 1 at the start), the Gram matrix and
-    the polynomial can reach has to stay inside its range."""
+    the polynomial can reach has to stay inside its range. At the other end a matrix of many small singular values has entries of 1 / sqrt(shorter
+    side) after the scaling; fp16 holds them to 11 bits down to 2^-14. So that 16384 rows (2^-7) keep these, small singular values, which a step
+    multiplies by ``a``, may not shrink below 2^-6 of themselves on the way."""
     per_step = coefficients if isinstance(coefficients[0], tuple) else (coefficients,) * steps
     if len(per_step) != steps or any(len(c) != 3 for c in per_step):
         raise ValueError("coefficients are one (a, b, c) or one per step")
-    top = 1.0
+    top = small = 1.0
     k = 2.0 ** round(math.log2(longer) / 2)
     for a, b, c in per_step:
         if not all(math.isfinite(v) for v in (a, b, c)):
             raise ValueError("coefficients must be finite")
+        small *= abs(a)
+        if small < 2.0 ** -6:
+            raise ValueError("coefficients whose linear terms shrink small singular values to less than 1/64 leave the range of fp16")
         inner = abs(b) * top ** 2 + abs(c) * top ** 4
         top = 1.01 * max(abs(a * s + b * s ** 3 + c * s ** 5) for s in (top * i / 512 for i in range(513)))
         if not max(inner, top * top, top * k) <= 3e4:
@@ -73,7 +78,8 @@ def _launch(g, m, momentum, nesterov, steps, coeff, eps, out, p, decay, scale, p
 
 def newton_schulz(g: torch.Tensor, *, steps: int = 5, coefficients=FAST, eps: float = 1e-7) -> torch.Tensor:
     """Orthogonalises the matrices ``g`` (bf16 or fp32 ``[..., rows, cols]``, any sides): ``X = g / (|g|_F + eps)``, then ``steps`` times
-    ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``. ``coefficients`` is one ``(a, b, c)`` or a sequence of one per step. Returns bf16 of the
+    ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``. ``coefficients`` is one ``(a, b, c)`` or a sequence of one per step; they must keep the
+    singular values within what fp16 products hold (refused otherwise: growth beyond 3e4, and linear terms whose product falls under 1/64). Returns bf16 of the
     same shape (at most 65535 matrices). The iterate is held in fp32 and multiplied in fp16 with fp32 sums. A matrix of zeros stays zero; one with a value that is not
     finite comes back as NaN, alone. The same call gives the same bits; alone a matrix may be split over the GPU in another way than in a batch."""
     if g.dtype not in _DT:

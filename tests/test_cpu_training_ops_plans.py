@@ -63,3 +63,21 @@ def test_too_many_tiles_are_refused_before_anything_changes(batch, rows, cols):
     lib = nv.cuda_lib()
     rc = lib.pkb_newton_schulz(p, 0, p, f(0.9), 1, LL(batch), rows, cols, coeff, 1, d(1e-7), None, p, f(1), f(1), None, p, None)
     assert rc != 0 and b"too many tiles" in lib.pkb_last_error(), lib.pkb_last_error()
+
+
+def test_coefficients_that_shrink_the_iterate_are_refused():
+    """Two steps of (0, 1, 1) on 1101 x 1413 of noise leave singular values of 1e-5 and less: as fp16 entries they are zero, and so was the result."""
+    import torch
+
+    from parallelkernelbench_b200.ops import muon_step, newton_schulz
+
+    g = torch.zeros(4, 6)
+    for bad, steps in (((0.0, 1.0, 1.0), 1), ((0.0, 1.0, 1.0), 2), ((0.01, 1.0, 0.0), 1), ((0.2, 1.0, 0.0), 3), (((1.5, -0.5, 0.0), (0.0, 1.0, 0.0), (2.0, 0.0, 0.0)), 3)):
+        with pytest.raises(ValueError, match="shrink"):
+            newton_schulz(g, coefficients=bad, steps=steps)
+        with pytest.raises(ValueError, match="shrink"):
+            muon_step(g, g.clone(), g.clone(), lr=0.1, coefficients=bad, steps=steps)
+    # what comes through ends at the next check, as a tensor on the CPU
+    for good, steps in (((3.4445, -4.7750, 2.0315), 5), ((1.5, -0.5, 0.0), 16), ((2.0, -1.5, 0.5), 8), ((0.5, 0.5, 0.0), 6), (((-1.5, 0.5, 0.0), (2.0, -1.0, 0.0)), 2)):
+        with pytest.raises(ValueError, match="CUDA"):
+            newton_schulz(g, coefficients=good, steps=steps)
