@@ -94,6 +94,18 @@ def newton_schulz(g: torch.Tensor, *, steps: int = 5, coefficients=FAST, eps: fl
     return out
 
 
+def _check_apart(p, m, g, p_bf16) -> None:
+    """No byte of what a step writes in place belongs to another of its tensors (all but ``g`` are contiguous)."""
+    n, at_p, at_m, at_g = p.numel(), p.data_ptr(), m.data_ptr(), g.data_ptr()
+    of_g = (n if g.is_contiguous() else sum((k - 1) * s for k, s in zip(g.shape, g.stride())) + 1) * g.element_size()
+    apart = (at_p + 4 * n <= at_m or at_m + 4 * n <= at_p) and (at_p + 4 * n <= at_g or at_g + of_g <= at_p) and (at_m + 4 * n <= at_g or at_g + of_g <= at_m)
+    if apart and p_bf16 is not None:
+        at = p_bf16.data_ptr()
+        apart = all(at + 2 * n <= other or other + size <= at for other, size in ((at_p, 4 * n), (at_m, 4 * n), (at_g, of_g)))
+    if not apart:
+        raise ValueError("p, m, g and p_bf16 must be different tensors that do not overlap")
+
+
 def muon_step(p: torch.Tensor, m: torch.Tensor, g: torch.Tensor, *, lr: float, momentum: float = 0.95, nesterov: bool = True,
               weight_decay: float = 0.0, scale: float | None = None, steps: int = 5, coefficients=FAST, eps: float = 1e-7,
               p_bf16: torch.Tensor | None = None) -> None:
@@ -103,7 +115,7 @@ def muon_step(p: torch.Tensor, m: torch.Tensor, g: torch.Tensor, *, lr: float, m
         p <- p * (1 - lr * weight_decay) - lr * scale * newton_schulz(u)
 
     ``scale`` defaults to ``0.2 * sqrt(max(rows, cols))``: an update of about Adam's root mean square, so that its learning rate and decay carry
-    over. ``p_bf16`` receives a bf16 copy. Leading dimensions are matrices of their own (the experts of a MoE layer)."""
+    over. ``p_bf16`` receives a bf16 copy. None of the tensors may overlap another. Leading dimensions are matrices of their own (the experts of a MoE layer)."""
     for name, t in (("p", p), ("m", m)):
         if t.dtype != torch.float32 or not t.is_contiguous():
             raise TypeError(f"{name} must be contiguous fp32")
@@ -114,8 +126,8 @@ def muon_step(p: torch.Tensor, m: torch.Tensor, g: torch.Tensor, *, lr: float, m
     if p_bf16 is not None and (p_bf16.dtype != torch.bfloat16 or p_bf16.shape != p.shape or not p_bf16.is_contiguous()):
         raise ValueError("p_bf16 must be contiguous bf16 of the shape of p")
     coeff = _check(g, steps, coefficients, eps)
-    if p.numel() and len({p.data_ptr(), m.data_ptr(), g.data_ptr()}) < 3:
-        raise ValueError("p, m and g must be different tensors")
+    if p.numel():
+        _check_apart(p, m, g, p_bf16)
     nv.same_cuda_device(p, m=m, g=g, p_bf16=p_bf16)
     if not p.numel():
         return

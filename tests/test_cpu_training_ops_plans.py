@@ -81,3 +81,25 @@ def test_coefficients_that_shrink_the_iterate_are_refused():
     for good, steps in (((3.4445, -4.7750, 2.0315), 5), ((1.5, -0.5, 0.0), 16), ((2.0, -1.5, 0.5), 8), ((0.5, 0.5, 0.0), 6), (((-1.5, 0.5, 0.0), (2.0, -1.0, 0.0)), 2)):
         with pytest.raises(ValueError, match="CUDA"):
             newton_schulz(g, coefficients=good, steps=steps)
+
+
+def test_tensors_of_a_step_do_not_overlap():
+    """Weight, momentum, gradient and copy are written or read while others are written: not only the same tensor but any shared byte is refused."""
+    import torch
+
+    from parallelkernelbench_b200.ops import muon_step
+
+    buf = torch.zeros(200)
+    at = lambda i, n=24: buf[i:i + n].view(4, 6)  # noqa: E731
+    half = torch.zeros(400, dtype=torch.bfloat16)
+    g = torch.zeros(4, 6)
+    cases = [(at(0), at(23), g, None), (at(0), at(30), at(40), None), (at(10), at(60), at(12, 24), None), (at(10), at(60), buf[50:].as_strided((4, 6), (20, 1)), None),
+             (at(0), at(30), g, buf[:12].view(torch.bfloat16).view(4, 6)), (at(0), at(30), half[:24].view(4, 6), half[20:44].view(4, 6))]
+    for p, m, grad, copy in cases:
+        with pytest.raises(ValueError, match="different"):
+            muon_step(p, m, grad, lr=0.1, p_bf16=copy)
+    # side by side they end at the next check, as tensors on the CPU
+    for p, m, grad, copy in ((at(0), at(24), at(48), None), (at(48), at(0), buf[72:].as_strided((4, 6), (1, 4)), buf[100:112].view(torch.bfloat16).view(4, 6)),
+                             (at(0), at(24), g[:1].expand(4, 6), half[:24].view(4, 6))):
+        with pytest.raises(ValueError, match="CUDA"):
+            muon_step(p, m, grad, lr=0.1, p_bf16=copy)
