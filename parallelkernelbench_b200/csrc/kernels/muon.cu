@@ -1254,14 +1254,46 @@ cudaError_t launch_dependent(void (*kern)(Params...), dim3 grid, int threads, in
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
+// [i]: clusters of 2^i CTAs of a kernel that are resident at once (a cluster stays inside a group of SMs: 148, 74, 33, 15 and 7 on a whole GPU, which
+// is also the answer where there is no device to ask).
+using NsResident = std::array<int, 5>;
+template <auto KERN>
+const NsResident& ns_resident(int threads, int smem) {
+  static const NsResident table = [&] {
+    NsResident t = {148, 74, 33, 15, 7};
+    if (prepare_kernel<KERN>(smem, true) != kApiOk) {
+      (void)cudaGetLastError();
+      return t;
+    }
+    for (int i = 0; i < 5; ++i) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1u << i);
+      cfg.blockDim = dim3((unsigned)threads);
+      cfg.dynamicSmemBytes = (size_t)smem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1u << i;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&t[i], KERN, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        t[i] = 0;
+      }
+    }
+    return t;
+  }();
+  return table;
+}
+
 // CTAs that share a tile of the split form, 0 where the pairs' form is taken: that one's tiles are four times as large, so it needs the GPU
 // filled, which 128 x 128 tiles in one wave say it is not.
 int split_ctas(long long tiles, int num_k) {
   if (tiles > sm_count()) return 0;
-  // clusters of 16, 8, 4, 2 that are resident at once (a cluster stays inside a group of 16 to 20 SMs), and at least two blocks of K each
-  const struct { int ctas, resident; } sizes[] = {{16, 7}, {8, 15}, {4, 33}, {2, 74}};
-  for (const auto& z : sizes)
-    if (tiles <= z.resident && num_k >= 2 * z.ctas) return z.ctas;
+  // the largest cluster of which all are resident at once, with at least two blocks of K for each CTA
+  const NsResident& resident = ns_resident<ns_split_kernel<false, false, kNsPoly>>(kNsThreads, kSplitSmem);
+  for (int i = 4; i > 0; --i)
+    if (tiles <= resident[i] && num_k >= 2 << i) return 1 << i;
   return 1;
 }
 
@@ -1289,16 +1321,20 @@ int ns_gemm(const CUtensorMap& ta, const CUtensorMap& tb, NsParams p, cudaStream
   return kApiOk;
 }
 
-// CTAs per matrix: as few as hold it, then more (down to slices of 64) while all matrices together leave SMs idle. A cluster stays inside a
-// group of 16 to 20 SMs, so seven or more clusters of 16 are resident at once.
+// CTAs per matrix: as few as hold it, then more (down to slices of 64) while the clusters of all matrices are resident at once.
 int small_cluster(long long batch, int longer) {
-  int c = 1;
-  while (c * kSmallSlice < longer) c *= 2;
-  while (c < kSmallCluster && c * 64 < longer && batch * c * 2 <= 112) c *= 2;
-  return c;
+  const NsResident& resident = ns_resident<ns_small_kernel>(kSmallThreads, kSmallSmem);
+  int i = 0;
+  while ((kSmallSlice << i) < longer) ++i;
+  while (i < 4 && (64 << i) < longer && batch <= resident[i + 1]) ++i;
+  return 1 << i;
 }
 
-bool small_fits(int side, int longer, int steps) { return side <= kSmallSide && longer <= kSmallCluster * kSmallSlice && steps <= kSmallMaxSteps; }
+// (clusters of more than eight CTAs are not to be had everywhere)
+bool small_fits(int side, int longer, int steps) {
+  if (side > kSmallSide || longer > kSmallCluster * kSmallSlice || steps > kSmallMaxSteps) return false;
+  return longer <= 8 * kSmallSlice || ns_resident<ns_small_kernel>(kSmallThreads, kSmallSmem)[4] > 0;
+}
 
 int launch_small(const NsSmallParams& p, int cluster, long long batch, cudaStream_t s) {
   if (const int rc = prepare_kernel<ns_small_kernel>(kSmallSmem, true)) return rc;

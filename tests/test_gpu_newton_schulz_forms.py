@@ -99,3 +99,12 @@ def test_the_whole_step(shape, nesterov, dtype, offset):
     want = p0 * (1 - lr * decay) - lr * scale * o
     assert (p.double() - want).norm() <= 2.0 ** -22 * (p0.norm() + lr * scale * o.norm()) + 1e-4 * lr * scale * o.norm()
     assert torch.equal(copy, p.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(7, 100, 2000), (8, 100, 2000), (15, 64, 1000), (16, 64, 1000), (34, 1000, 64), (75, 64, 500), (149, 60, 250), (8, 90, 4000)])
+def test_batches_around_what_is_resident(batch, rows, cols):
+    """As many clusters of 16, 8, 4 and 2 as a GPU holds at once, and one more, which waits or takes smaller ones."""
+    u = matrix((batch, rows, cols), "noise", "cuda")
+    got = _plain(u, 5)
+    for i in (0, batch // 2, batch - 1):
+        _hold(got[i], u[i], (FAST,) * 5)
