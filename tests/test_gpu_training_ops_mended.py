@@ -72,3 +72,33 @@ def test_layer_norm_of_nearly_constant_rows(rows, cols, center):
     assert ((mean.double()[:, None] - m).abs() <= U * m.abs() + e).all()
     assert ((rstd.double()[:, None] - r).abs() <= r * (k * U + (e * r) ** 2)).all()
     assert ((y.double() - d * r).abs() <= e * r + (k * U + (e * r) ** 2) * (d * r).abs() + 4 * U * (d * r).abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("spread", [0.1, 0.3])
+def test_layer_norm_of_millions_of_columns(spread, dtype):
+    """A sum's error must not grow with the width: rows one constant distance above and below their mean, whose squares round the same way in every
+    addition. 32 terms are added in fp32, the runs in 64 bits, and 512 threads by a tree of 9: K = 32 + 9 + 1 roundings of 2^-24, taken as 64."""
+    from parallelkernelbench_b200.ops import layer_norm_bwd, layer_norm_fwd
+
+    cols, k = (1 << 22) + 3, 64
+    sign = 1.0 - 2.0 * (torch.arange(cols, device="cuda") % 2)
+    x = torch.stack([1.0 + spread * sign, torch.full_like(sign, spread), spread * sign.flip(0) - 0.7]).to(dtype)
+    dy = torch.stack([sign * spread + 0.01, torch.full_like(sign, 0.3), torch.randn(cols, device="cuda", generator=_gen(9))]).to(dtype)
+    y, mean, rstd = layer_norm_fwd(x, None, None, 1e-5)
+    xd, half = x.double(), torch.finfo(dtype).eps / 2
+    m = xd.mean(1, keepdim=True)
+    d = xd - m
+    r = 1 / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-5)
+    e = k * U * (d.abs().mean(1, keepdim=True) + k * U * xd.abs().mean(1, keepdim=True))
+    assert ((mean.double()[:, None] - m).abs() <= U * m.abs() + e).all()
+    assert ((rstd.double()[:, None] - r).abs() <= r * (k * U + (e * r) ** 2)).all()
+    e_x = e * r + (k * U + (e * r) ** 2) * (d * r).abs() + 4 * U * (d * r).abs()
+    assert ((y.double() - d * r).abs() <= half * (d * r).abs() + e_x * (1 + half)).all()
+    dx, _, dbeta = layer_norm_bwd(x, None, dy, mean, rstd)
+    xh, g = (xd - mean.double()[:, None]) * rstd.double()[:, None], dy.double()
+    c1, c2 = g.mean(1, keepdim=True), (g * xh).mean(1, keepdim=True)
+    want = rstd.double()[:, None] * (g - c1 - xh * c2)
+    slack = rstd.double()[:, None] * (k * U * (g.abs().mean(1, keepdim=True) + xh.abs() * (g * xh).abs().mean(1, keepdim=True)) + 8 * U * (g.abs() + (xh * c2).abs()))
+    assert ((dx.double() - want).abs() <= half * want.abs() + slack * (1 + half)).all()
+    assert ((dbeta.double() - g.sum(0)).abs() <= 4 * U * g.abs().sum(0)).all()
