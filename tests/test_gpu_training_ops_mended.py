@@ -102,3 +102,58 @@ def test_layer_norm_of_millions_of_columns(spread, dtype):
     slack = rstd.double()[:, None] * (k * U * (g.abs().mean(1, keepdim=True) + xh.abs() * (g * xh).abs().mean(1, keepdim=True)) + 8 * U * (g.abs() + (xh * c2).abs()))
     assert ((dx.double() - want).abs() <= half * want.abs() + slack * (1 + half)).all()
     assert ((dbeta.double() - g.sum(0)).abs() <= 4 * U * g.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(1300, 4096), (1300, 4097), (2401, 1032), (301, 16384), (700, 333), (3, 9000)])
+def test_layer_norm_bad_rows_stay_alone(rows, cols, dtype):
+    """Rows that share their barriers and shuffles with others: NaN and infinities reach nobody else, nor the rows' own statistics of other rows."""
+    from parallelkernelbench_b200.ops import layer_norm_bwd, layer_norm_fwd
+
+    g = _gen(rows + cols)
+    x = torch.randn(rows, cols, device="cuda", generator=g).to(dtype)
+    dy = torch.randn(rows, cols, device="cuda", generator=g).to(dtype)
+    good = layer_norm_fwd(x)
+    want = layer_norm_bwd(x, None, dy, *good[1:])[0]
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for i, (r, c, v) in enumerate([(0, 0, float("nan")), (rows // 2, cols - 1, float("inf")), (rows - 1, cols // 2, float("-inf"))]):
+        x[r, c] = v
+        bad[r] = True
+    y, mean, rstd = layer_norm_fwd(x)
+    dx = layer_norm_bwd(x, None, dy, mean, rstd)[0]
+    for got, before in ((y, good[0]), (mean, good[1]), (rstd, good[2]), (dx, want)):
+        assert torch.equal(got[~bad], before[~bad])
+    assert torch.isnan(y[bad]).all() and torch.isnan(dx[bad]).all()
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are captured: what the library asks the device for once must not end the capture."""
+    code = """
+import torch
+from parallelkernelbench_b200.ops import layer_norm_bwd, layer_norm_fwd, muon_step, newton_schulz
+from parallelkernelbench_b200.ops.moe import permute_tokens, sort_by_expert
+t = lambda *s: torch.randn(*s, device="cuda")
+u, v, w, x = t(3, 64, 900), t(333, 700), t(4, 600, 900), t(1300, 4096)
+idx = torch.randint(0, 16, (9000, 2), device="cuda", dtype=torch.int32)
+p, m = t(333, 700), t(333, 700)
+def run():
+    y, mean, rstd = layer_norm_fwd(x)
+    srt = sort_by_expert(idx, 16)
+    return [newton_schulz(u), newton_schulz(v), newton_schulz(w), y, *layer_norm_bwd(x, None, y, mean, rstd), srt.slots, permute_tokens(idx.float(), srt)]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = run()
+    muon_step(p, m, v, lr=0.0)
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, run()))
+print("the same")
+"""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stderr[-2000:]
