@@ -663,6 +663,23 @@ __device__ __forceinline__ float2 unpack_bf16x2(uint32_t u) {
   __nv_bfloat162 v = *reinterpret_cast<__nv_bfloat162*>(&u);
   return __bfloat1622float2(v);
 }
+// 16 bytes of a row as fp32: N = 8 bf16 or 4 fp32 values; and back, rounded to nearest
+template <int N>
+__device__ __forceinline__ void unpack16(const U4& u, float (&f)[N]) {
+  static_assert(N == 8 || N == 4, "16 bytes");
+  if constexpr (N == 8) {
+    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+  } else {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  }
+}
+template <int N>
+__device__ __forceinline__ U4 pack16(const float (&f)[N]) {
+  static_assert(N == 8 || N == 4, "16 bytes");
+  if constexpr (N == 8) return U4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+  else return U4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+}
 // x / s rounded to nearest, given inv = 1 / s rounded to nearest: q0 = x * inv is within an ulp, the residual x - q0 * s is
 // exact in an FMA, and one correction step lands on the correctly rounded quotient (x and s normal, no overflow).
 __device__ __forceinline__ float div_rn_by(float x, float s, float inv) {

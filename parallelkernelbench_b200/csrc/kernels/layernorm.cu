@@ -23,16 +23,8 @@ namespace {
 // one row access: VEC values of type T at p as fp32, and back (rounded to nearest)
 template <typename T, int VEC>
 __device__ __forceinline__ void ln_load(const T* p, float (&f)[VEC]) {
-  if constexpr (VEC == 8) {
-    const U4 u = ld_global_nc_v4(p);
-    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
-    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
-  } else if constexpr (VEC == 4) {
-    const U4 u = ld_global_nc_v4(p);
-    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
-  } else {
-    f[0] = static_cast<float>(*p);
-  }
+  if constexpr (VEC == 1) f[0] = static_cast<float>(*p);
+  else unpack16(ld_global_nc_v4(p), f);
 }
 
 // the same access as it is, for rows on their way
@@ -44,23 +36,14 @@ struct LnRaw {
     else u = ld_global_nc_v4(p);
   }
   __device__ __forceinline__ void unpack(float (&f)[VEC]) const {
-    if constexpr (VEC == 1) {
-      f[0] = static_cast<float>(u);
-    } else if constexpr (VEC == 8) {
-      const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
-      f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
-    } else {
-      f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
-    }
+    if constexpr (VEC == 1) f[0] = static_cast<float>(u);
+    else unpack16(u, f);
   }
 };
 
 template <typename T, int VEC>
 __device__ __forceinline__ void ln_store(T* p, const float (&f)[VEC]) {
-  if constexpr (VEC == 8)
-    st_global_v4(p, U4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])});
-  else if constexpr (VEC == 4)
-    st_global_v4(p, U4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])});
+  if constexpr (VEC > 1) st_global_v4(p, pack16(f));
   else if constexpr (sizeof(T) == 2)
     *p = __float2bfloat16_rn(f[0]);
   else
@@ -91,13 +74,12 @@ struct LnParam {
     } else if (f32) {
 #pragma unroll
       for (int j = 0; j < VEC; j += 4) {
-        const U4 u = ld_global_v4(static_cast<const float*>(p) + c + j);
-        f[j] = __uint_as_float(u.x); f[j + 1] = __uint_as_float(u.y); f[j + 2] = __uint_as_float(u.z); f[j + 3] = __uint_as_float(u.w);
+        float q[4];
+        unpack16(ld_global_v4(static_cast<const float*>(p) + c + j), q);
+        f[j] = q[0]; f[j + 1] = q[1]; f[j + 2] = q[2]; f[j + 3] = q[3];
       }
     } else if constexpr (VEC == 8) {
-      const U4 u = ld_global_v4(static_cast<const __nv_bfloat16*>(p) + c);
-      const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), g = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
-      f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = g.x; f[5] = g.y; f[6] = d.x; f[7] = d.y;
+      unpack16(ld_global_v4(static_cast<const __nv_bfloat16*>(p) + c), f);
     } else {
       const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + c);
       const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
@@ -179,14 +161,13 @@ __device__ __forceinline__ void team_sum_shared(float (&v)[K], float* red, int t
   }
 }
 
-// A row's statistics from its first mean m0, the sum of its differences from it and the sum of their squares (see the top). The quotient takes its
-// remainder into account, so that it is exact where it can be: a constant row, whose differences are one number of a few bits, has no variance and
-// nothing left of it. (With divisions here and for m0: 16384 x 8192 bf16 116 us instead of 111.)
+// A row's statistics from its first mean m0, the sum of its differences from it and the sum of their squares (see the top). The quotient is
+// rounded once, so that it is exact where it can be: a constant row, whose differences are one number of a few bits, has no variance and nothing left
+// of it. (With divisions here and for m0: 16384 x 8192 bf16 116 us instead of 111.)
 struct LnStats {
   float delta, mean, rstd;
   __device__ __forceinline__ LnStats(float m0, float sum, float squares, int cols, float inv, float eps) {
-    delta = sum * inv;
-    delta = fmaf(fmaf(-delta, (float)cols, sum), inv, delta);
+    delta = div_rn_by(sum, (float)cols, inv);
     mean = m0 + delta;
     float q = fmaf(-sum, delta, squares);
     if (!(q >= 0.f)) q = isfinite(squares) ? 0.f : squares;      // rounding, or squares that left fp32
@@ -867,11 +848,10 @@ __device__ __forceinline__ void odd_store(T* row, int j, F2 v, int cols) {
 }
 
 template <typename T>
-__device__ __forceinline__ void odd_issue(const LnSpan& span, const T* row, uint32_t row_bytes, uint32_t dst, uint32_t bar, uint32_t& bytes) {
+__device__ __forceinline__ void odd_issue(const LnSpan& span, const T* row, uint32_t row_bytes, uint32_t dst, uint32_t bar) {
   uintptr_t at, lo, hi;
   span.pieces(reinterpret_cast<uintptr_t>(row), row_bytes, at, lo, hi);
-  bytes = (uint32_t)(hi - lo);
-  bulk_load(dst + (uint32_t)(lo - at), reinterpret_cast<const void*>(lo), bytes, bar);
+  bulk_load(dst + (uint32_t)(lo - at), reinterpret_cast<const void*>(lo), (uint32_t)(hi - lo), bar);
 }
 template <typename T>
 __device__ __forceinline__ uint32_t odd_bytes(const LnSpan& span, const T* row, uint32_t row_bytes) {
@@ -905,10 +885,10 @@ ln_fwd_odd_kernel(const T* __restrict__ x, long long ldx, const LnParam gamma, c
   auto issue = [&](long long grp, int stage) {
     const uint32_t bar = ring.bars + 8 * stage;
     const int here = (int)min((long long)R, rows - grp * R);
-    uint32_t all = 0, one;
+    uint32_t all = 0;
     for (int i = 0; i < here; ++i) all += odd_bytes(span, x + (grp * R + i) * ldx, bytes);
     mbar_expect_tx(bar, all);
-    for (int i = 0; i < here; ++i) odd_issue(span, x + (grp * R + i) * ldx, bytes, ring.base + (stage * R + i) * row_stage, bar, one);
+    for (int i = 0; i < here; ++i) odd_issue(span, x + (grp * R + i) * ldx, bytes, ring.base + (stage * R + i) * row_stage, bar);
   };
   if (t == 0)
     for (int i = 0; i < stages; ++i)
@@ -1001,10 +981,9 @@ ln_bwd_odd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ 
   const float inv = 1.f / (float)cols;
   auto issue = [&](long long row, int stage) {
     const uint32_t dst = ring.base + stage * 2 * row_stage, bar = ring.bars + 8 * stage;
-    uint32_t one;
     mbar_expect_tx(bar, odd_bytes(span_x, x + row * ldx, bytes) + odd_bytes(span_d, dy + row * lddy, bytes));
-    odd_issue(span_x, x + row * ldx, bytes, dst, bar, one);
-    odd_issue(span_d, dy + row * lddy, bytes, dst + row_stage, bar, one);
+    odd_issue(span_x, x + row * ldx, bytes, dst, bar);
+    odd_issue(span_d, dy + row * lddy, bytes, dst + row_stage, bar);
   };
   if (t == 0)
     for (int i = 0; i < stages; ++i)

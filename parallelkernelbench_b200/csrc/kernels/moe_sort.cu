@@ -172,23 +172,15 @@ struct RowVec {
     else return U4{0u, 0u, 0u, 0u};
   }
   static __device__ __forceinline__ void unpack(const Raw& v, float (&f)[VEC]) {
-    if constexpr (VEC == 1) {
-      f[0] = static_cast<float>(v);
-    } else if constexpr (VEC == 4) {
-      f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
-    } else {
-      const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
-      f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
-    }
+    if constexpr (VEC == 1) f[0] = static_cast<float>(v);
+    else unpack16(v, f);
   }
   static __device__ __forceinline__ Raw pack(const float (&f)[VEC]) {
     if constexpr (VEC == 1) {
       if constexpr (sizeof(T) == 2) return __float2bfloat16_rn(f[0]);
       else return f[0];
-    } else if constexpr (VEC == 4) {
-      return U4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
     } else {
-      return U4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+      return pack16(f);
     }
   }
 };

@@ -728,9 +728,7 @@ __device__ __forceinline__ void load8(const NsInput& in, long long i, float (&g)
 #pragma unroll
     for (int j = 0; j < 8; ++j) g[j] = __uint_as_float(w[j]);
   } else {
-    const U4 u = ld_global_nc_v4(static_cast<const __nv_bfloat16*>(in.g) + i);
-    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
-    g[0] = a.x; g[1] = a.y; g[2] = b.x; g[3] = b.y; g[4] = c.x; g[5] = c.y; g[6] = d.x; g[7] = d.y;
+    unpack16(ld_global_nc_v4(static_cast<const __nv_bfloat16*>(in.g) + i), g);
   }
 }
 __device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
