@@ -5,12 +5,14 @@
 // delta = sum d / N, mean = m0 + delta, variance = (sum d^2 - delta sum d) / N and y = (d - delta) rstd gamma + beta: with m0 alone a constant row of 1e5
 // at 1000 columns (sum / N an ulp off) came out at -0.93 instead of 0. Never E[x^2] - mean^2.
 // A row belongs to a team of TPR threads that holds VEC * CH of its values each: 16-byte accesses where base, row pitch and width
-// allow them (VEC = 8 bf16 or 4 fp32), single values otherwise. All sums are fp32.
+// allow them (VEC = 8 bf16 or 4 fp32), single values otherwise. All sums are fp32 (of rows in passes runs of 32, added in 64 bits).
 // Forms, by width, alignment and number of rows (ln_fwd_any, ln_bwd_any): teams of 32 to 512 threads straight from global memory; from 1025 columns
-// and a few hundred rows on, rings of rows in shared memory; rows that no team holds in passes; backward a few rows in one launch of a cluster. Measured, forward / backward with the weights' sums,
-// us (copy bandwidth): 16384 x 8192 bf16 105 / 140 (78 % / 88 %), 8192 x 4096 31 / 44 (66 / 70), 16384 x 1000 19 / 25, 8192 x 4097 64 / 101,
-// 8192 x 4097 fp32 69 / 100 (59 / 61). A copy of 16384 x 8192 takes 84: what keeps the forward from it is not one thing (a warp per row without any
-// barrier takes as long, prefetching further ahead takes longer).
+// and a few hundred rows on, rings of rows in shared memory; rows that no team holds in passes; backward a few rows in one launch of a cluster.
+// Measured, forward / backward with the weights' sums, us (of the copy bandwidth): 16384 x 8192 bf16 111 / 140 (74 % / 88 %), 8192 x 4096 33 / 45 (62 / 68),
+// 16384 x 1000 19 / 25, 8192 x 4097 70 / 101, 8192 x 4097 fp32 73 / 104 (56 / 59). Of these 11 to 12 forward and 16 to 18 backward are start and end (launches,
+// the first rows' way, the blocks' last rows, the weights' sums); what each further row adds at 4096 and 8192 columns is 89 and 82 % of the copy bandwidth
+// forward and all of it backward (8192 to 65536 rows of 4096: 33, 57, 103, 195 us and 45, 75, 135, 254). A copy of 16384 x 8192 takes 84: what keeps the
+// forward from it is not one thing (a warp per row without any barrier takes as long, prefetching further ahead takes longer).
 #include "pkb/api.h"
 #include "pkb/bulk_copy.cuh"
 #include "pkb/host.h"

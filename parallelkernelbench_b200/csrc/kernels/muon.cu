@@ -13,7 +13,7 @@
 // diagonal are computed and each is stored twice.
 // Three forms, by size: a short side (m <= 128) in one launch; few tiles, each shared by a cluster; tiles of CTA pairs that fill the GPU. A call in us:
 // 16 x 16 19, 8 x 1024 x 128 53, 333 x 1000 114 (105 in a graph: 17 launches of about 6), 1024 x 1024 125, 2048 x 2048 254; with the optimiser step
-// 4096 x 4096 1395 and 28672 x 4096 7254, 71 % and 75 % of what the tensor cores sustain under the power cap (the products' tensor pipe is active in
+// 4096 x 4096 1396 and 28672 x 4096 7281, 71 % and 75 % of what the tensor cores sustain under the power cap (the products' tensor pipe is active in
 // 86 to 88 % of the cycles; the rest is the tail of their last tiles and the passes over momentum and weight).
 #include <cuda_fp16.h>
 #include <math.h>
