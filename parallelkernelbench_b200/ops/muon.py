@@ -79,11 +79,15 @@ def _launch(g, m, momentum, nesterov, steps, coeff, eps, out, p, decay, scale, p
 def newton_schulz(g: torch.Tensor, *, steps: int = 5, coefficients=FAST, eps: float = 1e-7) -> torch.Tensor:
     """Orthogonalises the matrices ``g`` (bf16 or fp32 ``[..., rows, cols]``, any sides): ``X = g / (|g|_F + eps)``, then ``steps`` times
     ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``. ``coefficients`` is one ``(a, b, c)`` or a sequence of one per step; they must keep the
-    singular values within what fp16 products hold (refused otherwise: growth beyond 3e4, and linear terms whose product falls under 1/64). Returns bf16 of the
-    same shape (at most 65535 matrices). The iterate is held in fp32 and multiplied in fp16 with fp32 sums: against 64 bits five steps are 1.1e-3 to
+    singular values within what fp16 products hold (refused otherwise: growth beyond 3e4, and linear terms whose product falls under 1/64).
+    Returns bf16 of the same shape (at most 65535 matrices).
+
+    The iterate is held in fp32 and multiplied in fp16 with fp32 sums: against 64 bits five steps are 1.1e-3 to
     2.1e-3 off (2-norm) for noise and 3e-4 to 9e-4 for matrices of few directions, before the rounding to bf16 adds its 1.7e-3. Up to 128 x 4096 the
     polynomial keeps 22 bits (1.1e-3 to 1.6e-3), in larger matrices 11 (1.1e-3 to 2.1e-3, the most where the sides differ most).
-    A matrix of zeros stays zero; one with a value that is not finite comes back as NaN, alone. The same call gives the same bits; alone a matrix may be split over the GPU in another way than in a batch."""
+
+    A matrix of zeros stays zero; one with a value that is not finite comes back as NaN, alone. The same call gives the same bits; alone a matrix may
+    be split over the GPU in another way than in a batch."""
     if g.dtype not in _DT:
         raise TypeError(f"newton_schulz takes bf16 or fp32, got {g.dtype}")
     if g.dim() < 2:
@@ -117,8 +121,9 @@ def muon_step(p: torch.Tensor, m: torch.Tensor, g: torch.Tensor, *, lr: float, m
         p <- p * (1 - lr * weight_decay) - lr * scale * newton_schulz(u)
 
     ``scale`` defaults to ``0.2 * sqrt(max(rows, cols))``: an update of about Adam's root mean square, so that its learning rate and decay carry
-    over. ``p_bf16`` receives a bf16 copy. None of the tensors may overlap another. The products' error (:func:`newton_schulz`) enters
-    as ``lr * scale`` times it: a step of 3e-4 moves weights of standard deviation 0.02 to within 2e-6 to 5e-6 of a computation in 64 bits. Leading dimensions are matrices of their own (the experts of a MoE layer)."""
+    over. ``p_bf16`` receives a bf16 copy. Leading dimensions are matrices of their own (the experts of a MoE layer). None of the tensors may overlap
+    another. The products' error (:func:`newton_schulz`) enters as ``lr * scale`` times it: a step of 3e-4 moves weights of standard deviation
+    0.02 to within 2e-6 to 5e-6 (2-norm) of a computation in 64 bits."""
     for name, t in (("p", p), ("m", m)):
         if t.dtype != torch.float32 or not t.is_contiguous():
             raise TypeError(f"{name} must be contiguous fp32")

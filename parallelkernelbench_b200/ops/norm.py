@@ -102,8 +102,8 @@ def _ln_forward(x, gamma, beta, eps, stats: bool):
 
 def layer_norm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) * rsqrt(var + eps) * gamma + beta`` over the last dimension. ``x`` is bf16 or fp32 ``[..., cols]`` (any row pitch,
-    any width), ``gamma`` and ``beta`` bf16 or fp32 ``[cols]`` or None (1 and 0); fp32 inside, one rounding to the type of ``x``. A constant row,
-    however far from zero, comes out as ``beta``."""
+    any width), ``gamma`` and ``beta`` bf16 or fp32 ``[cols]`` or None (1 and 0); fp32 inside, one rounding to the type of ``x``. A constant row
+    comes out as ``beta``, as long as its sum fits fp32."""
     return _ln_forward(x, gamma, beta, eps, False)[0]
 
 
